@@ -64,8 +64,8 @@ def reference_root(explicit: str | None = None) -> str | None:
             cands.append(json.load(f).get("reference_path"))
     except (OSError, ValueError):
         pass
-    for c in cands:
-        if c and os.path.isdir(c):
+    for c in cands:  # an empty mount point is not a checkout
+        if c and os.path.isdir(os.path.join(c, "replknet", "kernels")):
             return c
     return None
 

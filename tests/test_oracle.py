@@ -131,3 +131,11 @@ def test_backward_restatement_matches_torch_autograd(oracle_mod, B, H, W, C, K):
     np.testing.assert_allclose(dx, xt.grad.permute(0, 2, 3, 1).numpy(), rtol=1e-12, atol=1e-12)
     np.testing.assert_allclose(dw, wt.grad.squeeze(1).permute(1, 2, 0).numpy(), rtol=1e-12, atol=1e-12)
     np.testing.assert_allclose(db, bt.grad.numpy(), rtol=1e-12, atol=1e-12)
+
+
+def test_an_empty_reference_directory_is_no_checkout(tmp_path):
+    """The build of the reference's kernels skips a mount point that holds nothing, as it skips a missing one."""
+    from oracle import build_ref
+    assert build_ref.reference_root(str(tmp_path)) != str(tmp_path)
+    (tmp_path / "replknet" / "kernels").mkdir(parents=True)
+    assert build_ref.reference_root(str(tmp_path)) == str(tmp_path)
