@@ -3,8 +3,8 @@
 Compiles every ``*.cu`` in this directory with nvcc
 (``-gencode arch=compute_100a,code=sm_100a``) and the planner with g++, in
 parallel, into ``depthwise_conv_b200/_build/``, then links the shared library
-into the package directory.  Objects are rebuilt only when a source or any
-header is newer.  The library depends on the CUDA runtime only (no torch).
+into the package directory.  An object is rebuilt only when its source or a
+header that it includes is newer.  The library depends on the CUDA runtime only (no torch).
 
     python -m depthwise_conv_b200.csrc.build        # or: python build.py
     python -m depthwise_conv_b200.csrc.build --regcaps   # regenerate dw_regcaps.inc first
@@ -48,15 +48,25 @@ def _nvcc() -> str:
     raise RuntimeError("nvcc not found: the engine needs the CUDA toolkit to build")
 
 
-def _headers_mtime() -> float:
-    paths = [os.path.join(HERE, f) for f in os.listdir(HERE) if f.endswith((".cuh", ".h", ".inc"))]
-    paths += [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE) if f.endswith(".h")]
-    paths.append(os.path.abspath(__file__))
-    return max(os.path.getmtime(p) for p in paths)
+_INCLUDE = re.compile(r'^\s*#include\s+"([^"]+)"', re.M)
 
 
-def _compile(src: str, obj: str, hdr_mtime: float) -> str:
-    if os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(src), hdr_mtime):
+def _inputs_mtime(src: str) -> float:
+    """Newest time of a source, of every local header it includes (directly or not) and of this script."""
+    seen, todo = set(), [os.path.realpath(src)]
+    while todo:
+        path = todo.pop()
+        if path in seen or not os.path.exists(path):
+            continue
+        seen.add(path)
+        with open(path) as f:
+            for name in _INCLUDE.findall(f.read()):
+                todo += [os.path.realpath(os.path.join(d, name)) for d in (os.path.dirname(path), INCLUDE)]
+    return max(os.path.getmtime(p) for p in (*seen, os.path.abspath(__file__)))
+
+
+def _compile(src: str, obj: str) -> str:
+    if os.path.exists(obj) and os.path.getmtime(obj) >= _inputs_mtime(src):
         return f"up to date: {os.path.basename(obj)}"
     if src.endswith(".cu"):
         cmd = [_nvcc(), *ARCH, *NVCC_FLAGS, "-I", INCLUDE, "-c", src, "-o", obj]
@@ -76,11 +86,10 @@ def build(verbose: bool = False, jobs: int | None = None) -> str:
     """Compile and link the library; returns its path."""
     os.makedirs(BUILD, exist_ok=True)
     srcs = sorted(f for f in os.listdir(HERE) if f.endswith((".cu", ".cpp")))
-    hdr = _headers_mtime()
     objs = [os.path.join(BUILD, os.path.splitext(s)[0] + ".o") for s in srcs]
     jobs = jobs or max(1, min(len(srcs), os.cpu_count() or 4))
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
-        for msg in ex.map(lambda so: _compile(os.path.join(HERE, so[0]), so[1], hdr), zip(srcs, objs)):
+        for msg in ex.map(lambda so: _compile(os.path.join(HERE, so[0]), so[1]), zip(srcs, objs)):
             if verbose:
                 print(msg)
     newest_obj = max(os.path.getmtime(o) for o in objs)
