@@ -29,11 +29,16 @@ ERR_BAD_ARG = 8
 # dwb_act / dwb_accum
 ACT_NONE, ACT_RELU, ACT_GELU = 0, 1, 2
 ACT_CODES = {"none": ACT_NONE, "relu": ACT_RELU, "gelu": ACT_GELU}
+# act codes of the group norm entry points, which also take SiLU
+ACT_SILU = 3
+NORM_ACT_CODES = {**ACT_CODES, "silu": ACT_SILU}
+# dwb_dtype
+F16, BF16, F32 = 0, 1, 2
 ACCUM_F32, ACCUM_MIXED = 0, 1
 ACCUM_DEFAULT = ACCUM_MIXED  # DWB_ACCUM_DEFAULT
 
 # Every entry point the header declares, with its ctypes signature.
-_p, _i, _i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64
+_p, _i, _i64, _d = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_double
 
 
 class Problem(ctypes.Structure):
@@ -92,6 +97,13 @@ SIGNATURES = {
     "dwb_conv2d_nhwc_bwd_weight": ([_p, _p, _p, _i64, _i64, _i64, _i64, _i, _p], _i),
     "dwb_conv2d_nhwc_bwd_weight_workspace": ([_i64, _i64, _i64, _i64, _i, ctypes.POINTER(_i64)], _i),
     "dwb_conv2d_nhwc_bwd_weight_det": ([_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i, _p], _i),
+    "dwb_act8_encode_nhwc": ([_p, _p, _p, _i64, _i64, _i, _p], _i),
+    "dwb_act8_decode_nhwc": ([_p, _p, _p, _i64, _i64, _i, _p], _i),
+    "dwb_conv2d_nhwc_bwd_weight_act8_workspace": ([_i64, _i64, _i64, _i64, _i, ctypes.POINTER(_i64)], _i),
+    "dwb_conv2d_nhwc_bwd_weight_act8": ([_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i, _p], _i),
+    "dwb_group_norm_act_workspace": ([_i64, _i64, _i64, _i64, _i, _i, ctypes.POINTER(_i64)], _i),
+    "dwb_group_norm_act_nhwc_fwd": ([_p] * 9 + [_i64] * 5 + [_i, _d, _i, _i, _i, _p], _i),
+    "dwb_group_norm_act_nhwc_bwd": ([_p] * 12 + [_i64] * 5 + [_i, _i, _i, _i, _p], _i),
     "dwb_conv2d_nhwc_bwd_data_noalloc": ([_p, _p, _p, _i64, _i64, _i64, _i64, _i, _p], _i),
 }
 

@@ -1,0 +1,199 @@
+"""8-bit activation checkpoints: the codec, and the weight gradient that reads them.
+
+A training step keeps the input of every depthwise convolution for the weight
+gradient (and the input of every norm, ``norm_ops``).  Kept as a checkpoint it
+takes 1 + 1/32 bytes a value instead of 2: for every pixel and block of 32
+channels one exponent byte E, and a signed code q of 8 bits a channel; the value
+is ``q * 2^(E - 127)``.  The exponent is the smallest one with which 127 steps
+reach the block's largest magnitude, so a value is off by at most half a step,
+``amax / 127`` or less; what a checkpoint stands for is exact in the 16-bit type
+it came from.  A block that holds an infinity or a NaN reads back as NaN.
+
+``codes``: int8, the activation's shape, channels_last.  ``scales``: uint8
+[B, H, W, ceil(C / 32)], contiguous.
+
+Everything here validates tensors and calls the C ABI on the current stream;
+there is no CPU or PyTorch fallback.  The reference's ops are inference-only
+(convmixer/kernels/depthwise_torch_ops.py:157-159) and keep nothing.
+
+Torch ops:
+
+* ``depthwise::act8_encode(Tensor input) -> (Tensor codes, Tensor scales)``
+* ``depthwise::act8_decode(Tensor codes, Tensor scales, ScalarType dtype) -> Tensor``
+* ``depthwise::conv2d_nhwc_act8(Tensor input, Tensor weight, Tensor? bias=None)
+  -> (Tensor output, Tensor codes, Tensor scales)``: ``depthwise::conv2d_nhwc``
+  whose backward pass takes the weight gradient from the checkpoint, so that the
+  graph does not keep the input.  The input gradient does not read the input and
+  is the same as the other op's.
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+
+import torch
+
+from . import _lib, dw_ops
+from .dw_ops import _DeviceGuard, _stream_of
+
+BLOCK = 32
+DTYPE_CODES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+
+
+def check_nhwc(x: torch.Tensor, name: str = "input") -> int:
+    """A channels_last float16 or bfloat16 CUDA tensor [B, C, H, W] with C % 8 == 0; returns its dwb_dtype."""
+    if not x.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor (the engine has no CPU path)")
+    code = DTYPE_CODES.get(x.dtype)
+    if code is None:
+        raise RuntimeError(f"{name} must be float16 or bfloat16, got {x.dtype}")
+    if x.dim() != 4:
+        raise RuntimeError(f"{name} must be 4-D [B, C, H, W], got {tuple(x.shape)}")
+    if not x.is_contiguous(memory_format=torch.channels_last):
+        raise RuntimeError(f"{name} must be channels_last")
+    return code
+
+
+def check_checkpoint(codes: torch.Tensor, scales: torch.Tensor) -> None:
+    if not codes.is_cuda or codes.dtype != torch.int8 or codes.dim() != 4:
+        raise RuntimeError(f"codes must be a 4-D int8 CUDA tensor, got {codes.dtype} {tuple(codes.shape)} on {codes.device}")
+    if not codes.is_contiguous(memory_format=torch.channels_last):
+        raise RuntimeError("codes must be channels_last")
+    B, C, H, W = codes.shape
+    want = (B, H, W, -(-C // BLOCK))
+    if scales.dtype != torch.uint8 or tuple(scales.shape) != want or not scales.is_contiguous():
+        raise RuntimeError(f"scales must be contiguous uint8 {want}, got {scales.dtype} {tuple(scales.shape)}")
+    if scales.device != codes.device:
+        raise RuntimeError(f"scales is on {scales.device}, codes on {codes.device}")
+
+
+def empty_checkpoint(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Unwritten codes and scales for an activation like ``x``."""
+    B, C, H, W = x.shape
+    codes = torch.empty_like(x, dtype=torch.int8, memory_format=torch.channels_last)
+    return codes, torch.empty((B, H, W, -(-C // BLOCK)), dtype=torch.uint8, device=x.device)
+
+
+def act8_encode(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of a channels_last float16 or bfloat16 activation."""
+    dtype = check_nhwc(x)
+    B, C, H, W = x.shape
+    codes, scales = empty_checkpoint(x)
+    with _DeviceGuard(x.device):
+        stream = _stream_of(x)
+        _lib.call("dwb_act8_encode_nhwc", x.data_ptr(), codes.data_ptr(), scales.data_ptr(), B * H * W, C, dtype, stream)
+        _lib.after_launch(stream, "depthwise act8_encode")
+    return codes, scales
+
+
+def act8_decode(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """The activation a checkpoint stands for, channels_last; ``dtype``: the type it was made from."""
+    check_checkpoint(codes, scales)
+    if dtype not in DTYPE_CODES:
+        raise RuntimeError(f"dtype must be float16 or bfloat16, got {dtype}")
+    B, C, H, W = codes.shape
+    x = torch.empty_like(codes, dtype=dtype, memory_format=torch.channels_last)
+    with _DeviceGuard(codes.device):
+        stream = _stream_of(codes)
+        _lib.call("dwb_act8_decode_nhwc", codes.data_ptr(), scales.data_ptr(), x.data_ptr(), B * H * W, C,
+                  DTYPE_CODES[dtype], stream)
+        _lib.after_launch(stream, "depthwise act8_decode")
+    return x
+
+
+@functools.lru_cache(maxsize=1024)
+def _wgrad_workspace_bytes(B: int, H: int, W: int, C: int, K: int) -> int:
+    n = ctypes.c_int64(0)
+    _lib.call("dwb_conv2d_nhwc_bwd_weight_act8_workspace", B, H, W, C, K, ctypes.byref(n))
+    return n.value
+
+
+def conv2d_nhwc_backward_weight_act8(codes: torch.Tensor, scales: torch.Tensor, dy: torch.Tensor, K: int) -> torch.Tensor:
+    """dw of y = conv(x, w) as [K, K, C] float32 from the checkpoint of x (a float16 activation).
+
+    The sums have a fixed order: the same bits on every call.  An infinity or a NaN
+    in ``dy`` or the checkpoint may spread to every tap of its channel."""
+    check_checkpoint(codes, scales)
+    dw_ops.check_input(dy, "grad_output")
+    if dy.shape != codes.shape:
+        raise RuntimeError(f"grad_output shape {tuple(dy.shape)} != checkpoint shape {tuple(codes.shape)}")
+    if dy.device != codes.device:
+        raise RuntimeError(f"grad_output is on {dy.device}, checkpoint on {codes.device}")
+    B, C, H, W = dy.shape
+    K = int(K)
+    nbytes = _wgrad_workspace_bytes(B, H, W, C, K)
+    dw = torch.empty((K, K, C), dtype=torch.float32, device=dy.device)
+    ws = torch.empty(max(16, nbytes), dtype=torch.uint8, device=dy.device)
+    with _DeviceGuard(dy.device):
+        stream = _stream_of(dy)
+        _lib.call("dwb_conv2d_nhwc_bwd_weight_act8", codes.data_ptr(), scales.data_ptr(), dy.data_ptr(), dw.data_ptr(),
+                  ws.data_ptr(), ws.numel(), B, H, W, C, K, stream)
+        _lib.after_launch(stream, "depthwise conv2d_nhwc weight gradient from a checkpoint")
+    return dw
+
+
+def conv2d_nhwc_act8(x: torch.Tensor, w: torch.Tensor, bias=None) -> torch.Tensor:
+    """y = conv(x, w) (+ bias), differentiable; keeps the 8-bit checkpoint of x for the weight gradient."""
+    return torch.ops.depthwise.conv2d_nhwc_act8(x, w, bias)[0]
+
+
+torch.library.define("depthwise::act8_encode", "(Tensor input) -> (Tensor codes, Tensor scales)")
+torch.library.define("depthwise::act8_decode", "(Tensor codes, Tensor scales, ScalarType dtype) -> Tensor")
+torch.library.define("depthwise::conv2d_nhwc_act8",
+                     "(Tensor input, Tensor weight, Tensor? bias=None) -> (Tensor output, Tensor codes, Tensor scales)")
+
+
+@torch.library.impl("depthwise::act8_encode", "default")
+def _act8_encode_impl(input):
+    return act8_encode(input)
+
+
+@torch.library.register_fake("depthwise::act8_encode")
+def _act8_encode_fake(input):
+    return empty_checkpoint(input)
+
+
+@torch.library.impl("depthwise::act8_decode", "default")
+def _act8_decode_impl(codes, scales, dtype):
+    return act8_decode(codes, scales, dtype)
+
+
+@torch.library.register_fake("depthwise::act8_decode")
+def _act8_decode_fake(codes, scales, dtype):
+    return torch.empty_like(codes, dtype=dtype)
+
+
+@torch.library.impl("depthwise::conv2d_nhwc_act8", "default")
+def _conv2d_nhwc_act8_impl(input, weight, bias=None):
+    y = dw_ops.conv2d_nhwc_fused(input, weight, bias=bias)
+    return y, *act8_encode(input)
+
+
+@torch.library.register_fake("depthwise::conv2d_nhwc_act8")
+def _conv2d_nhwc_act8_fake(input, weight, bias=None):
+    return torch.empty_like(input), *empty_checkpoint(input)
+
+
+def _conv2d_nhwc_act8_setup(ctx, inputs, output):
+    _, w, bias = inputs
+    _, codes, scales = output
+    ctx.save_for_backward(w, codes, scales)
+    ctx.has_bias = bias is not None
+    ctx.mark_non_differentiable(codes, scales)
+    ctx.set_materialize_grads(False)
+
+
+def _conv2d_nhwc_act8_backward(ctx, grad, _codes, _scales):
+    if grad is None:
+        return None, None, None
+    w, codes, scales = ctx.saved_tensors
+    g = grad if grad.is_contiguous(memory_format=torch.channels_last) else grad.contiguous(
+        memory_format=torch.channels_last)
+    dx = dw_ops.conv2d_nhwc_backward_input(g, w) if ctx.needs_input_grad[0] else None
+    dw = conv2d_nhwc_backward_weight_act8(codes, scales, g, w.shape[0]).to(w.dtype) if ctx.needs_input_grad[1] else None
+    db = g.float().sum(dim=(0, 2, 3)).to(g.dtype) if ctx.has_bias and ctx.needs_input_grad[2] else None
+    return dx, dw, db
+
+
+torch.library.register_autograd("depthwise::conv2d_nhwc_act8", _conv2d_nhwc_act8_backward,
+                                setup_context=_conv2d_nhwc_act8_setup)

@@ -1,0 +1,162 @@
+// dw_act8.cu -- the 8-bit activation checkpoint as two streaming kernels:
+// encode (16-bit activation -> codes and exponent bytes) and decode.  The
+// format is described in dw_act8.cuh.
+//
+// Both are bound by memory: encode moves 2 + 1 + 1/32 bytes a value, decode
+// the same the other way.  A lane holds one 16-byte vector (8 channels), four
+// neighbouring lanes a block, so the block's maximum is two shuffles; each
+// thread keeps kUnroll vectors in flight.
+#include <cuda_runtime.h>
+
+#include "../../include/dwconv_b200.h"
+#include "dw_act8.cuh"
+#include "dw_host.h"
+#include "dw_launch.h"
+
+namespace dwb {
+
+constexpr int kActThreads = 256;
+constexpr int kUnroll = 4;
+
+// Vectors are numbered over pixels x quads of lanes.  WHOLE (C % 32 == 0): every quad is full and
+// the numbering is the memory order; else the last quad of a pixel has idle lanes.
+struct Act8Shape {
+  long long units;  // pixels * lanes_per_pixel
+  int vecs;         // C / 8
+  int lanes;        // lanes per pixel, 4 * ceil(C / 32)
+};
+
+template <bool WHOLE>
+struct Act8Place {
+  long long vec;    // vector index in memory order (C / 8 per pixel)
+  long long block;  // exponent byte index
+  bool active;
+  __device__ __forceinline__ Act8Place(long long u, const Act8Shape& s) {
+    active = u < s.units;
+    block = u >> 2;
+    if constexpr (WHOLE) {
+      vec = u;
+    } else {
+      const long long pixel = s.units <= 0x7fffffffLL ? static_cast<long long>(static_cast<unsigned>(u) / static_cast<unsigned>(s.lanes))
+                                                      : u / s.lanes;
+      const int v = static_cast<int>(u - pixel * s.lanes);
+      active = active && v < s.vecs;
+      vec = pixel * s.vecs + v;
+    }
+  }
+};
+
+template <typename T, bool WHOLE>
+__global__ void __launch_bounds__(kActThreads) act8_encode_kernel(const uint4* __restrict__ x, uint2* __restrict__ codes,
+                                                                  uint8_t* __restrict__ scales, const Act8Shape s) {
+  griddep_wait();
+  griddep_launch_dependents();
+  // block-uniform trip count: every lane takes part in the shuffles
+  for (long long base = static_cast<long long>(blockIdx.x) * (kActThreads * kUnroll); base < s.units;
+       base += static_cast<long long>(gridDim.x) * (kActThreads * kUnroll)) {
+    uint4 v[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const Act8Place<WHOLE> p(base + i * kActThreads + threadIdx.x, s);
+      v[i] = p.active ? __ldcs(x + p.vec) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const Act8Place<WHOLE> p(base + i * kActThreads + threadIdx.x, s);
+      const uint32_t E = act8_exponent<T>(act8_block_amax(v[i]));
+      if (p.active) {
+        codes[p.vec] = act8_codes<T>(v[i], E);
+        if ((threadIdx.x & 3) == 0) scales[p.block] = static_cast<uint8_t>(E);
+      }
+    }
+  }
+}
+
+template <typename T, bool WHOLE>
+__global__ void __launch_bounds__(kActThreads) act8_decode_kernel(const uint2* __restrict__ codes,
+                                                                  const uint8_t* __restrict__ scales,
+                                                                  uint4* __restrict__ x, const Act8Shape s) {
+  griddep_wait();
+  griddep_launch_dependents();
+  for (long long base = static_cast<long long>(blockIdx.x) * (kActThreads * kUnroll); base < s.units;
+       base += static_cast<long long>(gridDim.x) * (kActThreads * kUnroll)) {
+    uint2 q[kUnroll];
+    uint32_t E[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const Act8Place<WHOLE> p(base + i * kActThreads + threadIdx.x, s);
+      q[i] = p.active ? __ldcs(codes + p.vec) : make_uint2(0u, 0u);
+      E[i] = p.active ? scales[p.block] : 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const Act8Place<WHOLE> p(base + i * kActThreads + threadIdx.x, s);
+      f32x2 f[4];
+      act8_values(q[i], act8_step(E[i]), f);
+      if (p.active)
+        x[p.vec] = make_uint4(Type16<T>::from_f32x2(f[0]), Type16<T>::from_f32x2(f[1]), Type16<T>::from_f32x2(f[2]),
+                              Type16<T>::from_f32x2(f[3]));
+    }
+  }
+}
+
+static int act8_check(const void* x, const void* codes, const void* scales, int64_t pixels, int64_t C, int dtype) {
+  if (dtype != DWB_F16 && dtype != DWB_BF16) return DWB_ERR_BAD_ARG;
+  if (pixels < 0 || pixels > (1LL << 40) || C < 8 || C > (1 << 20) || (C % 8) != 0) return DWB_ERR_BAD_SHAPE;
+  if (pixels == 0) return DWB_OK;
+  if (!x || !codes || !scales) return DWB_ERR_NULL_POINTER;
+  if (!is_aligned(x, 16) || !is_aligned(codes, 8)) return DWB_ERR_BAD_ALIGN;
+  return DWB_OK;
+}
+
+static int act8_launch(const void* fn, const char* what, const void* in0, const void* in1, const void* in2, int64_t pixels,
+                       int64_t C, void* stream) {
+  const int rc = require_device();
+  if (rc != DWB_OK) return rc;
+  Act8Shape s;
+  s.vecs = static_cast<int>(C / 8);
+  s.lanes = static_cast<int>((C + kAct8Block - 1) / kAct8Block) * 4;
+  s.units = pixels * s.lanes;
+  const long long want = (s.units + kActThreads * kUnroll - 1) / (kActThreads * kUnroll);
+  const unsigned blocks = static_cast<unsigned>(want < 0x7fffffffLL ? want : 0x7fffffffLL);
+  void* args[4] = {&in0, &in1, &in2, &s};
+  const cudaError_t e = launch_kernel(fn, dim3(blocks), dim3(kActThreads), args, 0, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return record_cuda_failure(what, e);
+  }
+  return DWB_OK;
+}
+
+template <typename T>
+static const void* encode_fn(bool whole) {
+  return whole ? reinterpret_cast<const void*>(&act8_encode_kernel<T, true>)
+               : reinterpret_cast<const void*>(&act8_encode_kernel<T, false>);
+}
+template <typename T>
+static const void* decode_fn(bool whole) {
+  return whole ? reinterpret_cast<const void*>(&act8_decode_kernel<T, true>)
+               : reinterpret_cast<const void*>(&act8_decode_kernel<T, false>);
+}
+
+}  // namespace dwb
+
+extern "C" int dwb_act8_encode_nhwc(const void* x, void* codes, void* scales, int64_t pixels, int64_t C, int dtype,
+                                    void* stream) {
+  using namespace dwb;
+  const int rc = act8_check(x, codes, scales, pixels, C, dtype);
+  if (rc != DWB_OK || pixels == 0) return rc;
+  const bool whole = (C % kAct8Block) == 0;
+  return act8_launch(dtype == DWB_F16 ? encode_fn<__half>(whole) : encode_fn<__nv_bfloat16>(whole), "act8_encode_kernel", x,
+                     codes, scales, pixels, C, stream);
+}
+
+extern "C" int dwb_act8_decode_nhwc(const void* codes, const void* scales, void* x, int64_t pixels, int64_t C, int dtype,
+                                    void* stream) {
+  using namespace dwb;
+  const int rc = act8_check(x, codes, scales, pixels, C, dtype);
+  if (rc != DWB_OK || pixels == 0) return rc;
+  const bool whole = (C % kAct8Block) == 0;
+  return act8_launch(dtype == DWB_F16 ? decode_fn<__half>(whole) : decode_fn<__nv_bfloat16>(whole), "act8_decode_kernel",
+                     codes, scales, x, pixels, C, stream);
+}

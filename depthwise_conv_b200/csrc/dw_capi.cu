@@ -17,6 +17,7 @@
 
 #include "../../include/dwconv_b200.h"
 #include "dw_backward.h"
+#include "dw_host.h"
 #include "dw_kernel.cuh"
 #include "dw_launch.h"
 #include "dw_planner.h"
@@ -175,6 +176,13 @@ static int get_device_state(DeviceState** out) {
   std::call_once(st->once, init_device, dev, st);
   *out = st;
   return st->status;
+}
+
+int record_cuda_failure(const char* what, cudaError_t e) { return cuda_fail(what, e); }
+
+int require_device() {
+  DeviceState* st = nullptr;
+  return get_device_state(&st);
 }
 
 static int regs_of_variant(int K, int R, int M, int acc, int pre, void* ctx) {

@@ -1,0 +1,175 @@
+// dw_groupnorm.cuh -- group normalisation with an activation on channels-last
+// 16-bit tensors: the arithmetic that its kernels share.
+//
+//   x [B, P, C] (P = H * W pixels), G groups of Cg = C / G channels, n = P Cg:
+//   mean = sum x / n,  var = sum (x - mean)^2 / n,  rstd = 1 / sqrt(var + eps)
+//   xh = (x - mean) rstd,  u = xh weight + bias,  y = act(u)
+//
+//   backward, from dy and the saved x (16 bits, or its 8-bit checkpoint), mean
+//   and rstd:  g = dy act'(u),  dbias = sum g,  dweight = sum g xh,
+//   m1 = sum_group(g weight) / n,  m2 = sum_group(g weight xh) / n,
+//   dx = rstd ((g weight - m1) - xh m2).
+//
+// Layout of the work in every kernel: a thread owns one 16-byte vector of 8
+// channels and walks over pixels, so that its parameters and its sums stay in
+// registers and every group structure (groups of 1, 3, 9 channels, groups that
+// end inside a vector) is a matter of how the per-channel sums are added up.
+// Statistics: a thread sums (x - k) and (x - k)^2 with k its own first value,
+// which takes out the offset of the data, and the (count, mean, sum of squared
+// deviations) triples of threads, CTAs and channels are merged by
+// M2 = sum M2_i + sum n_i (mean_i - mean)^2.  All in fp32.
+#pragma once
+
+#include "dw_act8.cuh"
+
+namespace dwb {
+
+enum : int { kActSilu = 3 };  // after kActNone, kActRelu, kActGelu
+
+template <int ACT>
+__device__ __forceinline__ f32x2 act_value2(f32x2 u) {
+  if constexpr (ACT == kActRelu) {
+    const float2 f = bits_f2(u);  // a comparison, not fmaxf: NaN stays NaN
+    return f2_bits(make_float2(f.x < 0.0f ? 0.0f : f.x, f.y < 0.0f ? 0.0f : f.y));
+  } else if constexpr (ACT == kActGelu) {
+    return gelu_erf2(u);
+  } else if constexpr (ACT == kActSilu) {
+    const float2 e = bits_f2(fmul2(u, splat2(-1.4426950408889634f)));
+    const f32x2 d = fma2(f2_bits(make_float2(ex2_approx(e.x), ex2_approx(e.y))), splat2(1.0f), splat2(1.0f));
+    const float2 df = bits_f2(d);
+    return fmul2(u, f2_bits(make_float2(rcp_approx(df.x), rcp_approx(df.y))));
+  } else {
+    return u;
+  }
+}
+
+// act'(u).  GELU: Phi(u) + u phi(u), Phi from the erfc approximation of gelu_erf2 (Abramowitz & Stegun
+// 7.1.26), whose exponential phi shares: two special-function operations a value.  ReLU: 0 at 0.
+template <int ACT>
+__device__ __forceinline__ f32x2 act_slope2(f32x2 u) {
+  if constexpr (ACT == kActRelu) {
+    const float2 f = bits_f2(u);
+    return f2_bits(make_float2(f.x > 0.0f ? 1.0f : 0.0f, f.y > 0.0f ? 1.0f : 0.0f));
+  } else if constexpr (ACT == kActGelu) {
+    const f32x2 au = u & 0x7fffffff7fffffffull;
+    const float2 d = bits_f2(fma2(au, splat2(0.3275911f * 0.70710678118654752f), splat2(1.0f)));
+    const f32x2 t = f2_bits(make_float2(rcp_approx(d.x), rcp_approx(d.y)));
+    f32x2 poly = fma2(splat2(0.5f * 1.061405429f), t, splat2(0.5f * -1.453152027f));
+    poly = fma2(poly, t, splat2(0.5f * 1.421413741f));
+    poly = fma2(poly, t, splat2(0.5f * -0.284496736f));
+    poly = fma2(poly, t, splat2(0.5f * 0.254829592f));
+    poly = fmul2(poly, t);
+    const float2 ea = bits_f2(fmul2(fmul2(u, splat2(-0.5f * 1.4426950408889634f)), u));
+    const f32x2 e = f2_bits(make_float2(ex2_approx(ea.x), ex2_approx(ea.y)));  // exp(-u^2 / 2)
+    const float2 h = bits_f2(fmul2(poly, e));                                  // erfc(|u| / sqrt 2) / 2
+    const float2 uf = bits_f2(u);
+    const f32x2 cdf = f2_bits(make_float2(uf.x < 0.0f ? h.x : 1.0f - h.x, uf.y < 0.0f ? h.y : 1.0f - h.y));
+    return fma2(fmul2(u, splat2(0.3989422804014327f)), e, cdf);
+  } else if constexpr (ACT == kActSilu) {
+    const float2 e = bits_f2(fmul2(u, splat2(-1.4426950408889634f)));
+    const float2 s = make_float2(rcp_approx(1.0f + ex2_approx(e.x)), rcp_approx(1.0f + ex2_approx(e.y)));
+    const f32x2 sv = f2_bits(s);
+    const f32x2 rest = fma2(sv, splat2(-1.0f), splat2(1.0f));  // 1 - s
+    return fmul2(sv, fma2(u, rest, splat2(1.0f)));
+  } else {
+    return splat2(1.0f);
+  }
+}
+
+// Sizes of one call.
+struct GnShape {
+  long long P;     // pixels of a sample
+  int B, C, G, Cg;
+  float eps;
+  int param_f32;   // weight and bias: fp32 instead of the tensor's type
+};
+
+// Weight or bias of channel c (`otherwise` where the vector is absent).
+template <typename T>
+__device__ __forceinline__ float gn_param(const void* p, int c, int f32, float otherwise) {
+  if (!p) return otherwise;
+  return f32 ? static_cast<const float*>(p)[c] : Type16<T>::to_float(static_cast<const T*>(p)[c]);
+}
+
+template <typename T>
+__device__ __forceinline__ void gn_load_params(const void* weight, const void* bias, int c, int f32, f32x2 (&w)[4],
+                                               f32x2 (&b)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i] = f2_bits(make_float2(gn_param<T>(weight, c + 2 * i, f32, 1.0f), gn_param<T>(weight, c + 2 * i + 1, f32, 1.0f)));
+    b[i] = f2_bits(make_float2(gn_param<T>(bias, c + 2 * i, f32, 0.0f), gn_param<T>(bias, c + 2 * i + 1, f32, 0.0f)));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void gn_unpack(const uint4& v, f32x2 (&f)[4]) {
+  f[0] = Type16<T>::to_f32x2(v.x);
+  f[1] = Type16<T>::to_f32x2(v.y);
+  f[2] = Type16<T>::to_f32x2(v.z);
+  f[3] = Type16<T>::to_f32x2(v.w);
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 gn_pack(const f32x2 (&f)[4]) {
+  return make_uint4(Type16<T>::from_f32x2(f[0]), Type16<T>::from_f32x2(f[1]), Type16<T>::from_f32x2(f[2]),
+                    Type16<T>::from_f32x2(f[3]));
+}
+
+__device__ __forceinline__ f32x2 fsub2(f32x2 a, f32x2 b) { return fma2(b, splat2(-1.0f), a); }
+
+// Sums of one thread about its own first values.
+struct GnSums {
+  f32x2 k[4], s1[4], s2[4];
+  int n = 0;
+  __device__ __forceinline__ void add(const f32x2 (&v)[4]) {
+    if (n == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        k[i] = v[i];
+        s1[i] = s2[i] = f32x2_zero();
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x2 d = fsub2(v[i], k[i]);
+        fadd2(s1[i], d);
+        ffma2(s2[i], d, d);
+      }
+    }
+    ++n;
+  }
+  // per-channel mean and sum of squared deviations (n >= 1)
+  __device__ __forceinline__ void moments(float (&mean)[8], float (&m2)[8]) const {
+    const float inv = 1.0f / static_cast<float>(n);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 kf = bits_f2(k[i]), a = bits_f2(s1[i]), q = bits_f2(s2[i]);
+      const float dx = a.x * inv, dy = a.y * inv;
+      mean[2 * i] = kf.x + dx;
+      mean[2 * i + 1] = kf.y + dy;
+      // a difference that rounding may leave below zero; NaN stays NaN
+      const float qx = q.x - a.x * dx, qy = q.y - a.y * dy;
+      m2[2 * i] = qx < 0.0f ? 0.0f : qx;
+      m2[2 * i + 1] = qy < 0.0f ? 0.0f : qy;
+    }
+  }
+};
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Sum over the CTA (blockDim.x a multiple of 32, at most 1024); `scratch` holds 33 floats.
+__device__ __forceinline__ float block_sum(float v, float* scratch) {
+  v = warp_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float s = 0.0f;
+  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) s += scratch[w];
+  return s;
+}
+
+}  // namespace dwb

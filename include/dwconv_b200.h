@@ -55,8 +55,16 @@ typedef enum dwb_status {
 typedef enum dwb_act {
     DWB_ACT_NONE = 0,
     DWB_ACT_RELU = 1,
-    DWB_ACT_GELU = 2            /* exact erf GELU, as nn.GELU() default          */
+    DWB_ACT_GELU = 2,           /* exact erf GELU, as nn.GELU() default          */
+    DWB_ACT_SILU = 3            /* x sigmoid(x): group norm entry points only    */
 } dwb_act;
+
+/* Element types, where an entry point takes more than fp16. */
+typedef enum dwb_dtype {
+    DWB_F16 = 0,
+    DWB_BF16 = 1,
+    DWB_F32 = 2                 /* parameter vectors only                        */
+} dwb_dtype;
 
 typedef enum dwb_accum {
     DWB_ACCUM_F32 = 0,          /* every tap accumulated in fp32 (FFMA2)          */
@@ -285,6 +293,68 @@ DWB_API int dwb_conv2d_nhwc_bwd_weight_det(const void* x, const void* dy, float*
  * GPU race on it. */
 DWB_API int dwb_conv2d_nhwc_bwd_data_noalloc(const void* dy, const void* w, void* dx, int64_t B, int64_t H,
                                              int64_t W, int64_t C, int K, void* stream);
+
+/* ---- 8-bit activation checkpoints ------------------------------------------------
+ * What a training step keeps of an activation for its backward pass, in 1 + 1/32
+ * bytes a value instead of 2.  No counterpart in the reference (inference only).
+ *
+ * For every pixel and block of 32 channels (the last block of a pixel may be
+ * shorter): one exponent byte E and a signed code q of 8 bits a channel; the
+ * value is q * 2^(E - 127).  E - 127 is the smallest exponent e with
+ * amax <= 127 * 2^e, within -24..9 for fp16 and -127..121 for bf16 (a larger
+ * amax saturates at 127 * 2^9 and 127 * 2^121); q = rint(x * 2^-e), ties to even,
+ * -127..127.  q * 2^e is exact in the type it came from.  E = 255: the block held
+ * an infinity or a NaN, and all of it reads back as NaN.
+ *   codes:  int8 [pixels][C], 8-byte aligned;  scales: uint8 [pixels][ceil(C / 32)].
+ * x: [pixels][C] fp16 or bf16 (dtype), 16-byte aligned, C % 8 == 0, C <= 2^20. */
+DWB_API int dwb_act8_encode_nhwc(const void* x, void* codes, void* scales, int64_t pixels, int64_t C,
+                                 int dtype, void* stream);
+DWB_API int dwb_act8_decode_nhwc(const void* codes, const void* scales, void* x, int64_t pixels, int64_t C,
+                                 int dtype, void* stream);
+
+/* The depthwise weight gradient from the checkpoint of the convolution's fp16
+ * input: dw[kh][kw][c] = sum over b, h, w of dy[b][h][w][c] * x[b][h+kh-K/2][w+kw-K/2][c]
+ * with x the checkpoint's values.  dy: NHWC fp16; dw: [K][K][C] fp32, written (not
+ * added to), 16-byte aligned.  Sums in fp32 in a fixed order: the same bits on
+ * every run.  An infinity or a NaN in x or dy may spread to every tap of its
+ * channel.  workspace: 16-byte aligned, at least the size that
+ * dwb_conv2d_nhwc_bwd_weight_act8_workspace reports; no two calls that may overlap
+ * share one.  K odd, 1..31, C % 8 == 0. */
+DWB_API int dwb_conv2d_nhwc_bwd_weight_act8_workspace(int64_t B, int64_t H, int64_t W, int64_t C, int K,
+                                                      int64_t* bytes);
+DWB_API int dwb_conv2d_nhwc_bwd_weight_act8(const void* codes, const void* scales, const void* dy, float* dw,
+                                            void* workspace, int64_t workspace_bytes, int64_t B, int64_t H,
+                                            int64_t W, int64_t C, int K, void* stream);
+
+/* ---- group normalisation with an activation ----------------------------------------
+ * y = act((x - mean) * rstd * weight + bias), mean and variance (biased) over the H * W
+ * pixels and C / G channels of each group of each sample; x, y NHWC fp16 or bf16 (dtype),
+ * weight, bias [C] or NULL (1 / 0) of dtype or fp32 (param_dtype), mean, rstd [B][G] fp32
+ * outputs (rstd = 1 / sqrt(var + eps)).  act: any dwb_act.  C % 8 == 0, C <= 65536,
+ * C % G == 0, eps >= 0; every sum in fp32, the same bits on every run.  No counterpart in
+ * the reference, whose networks normalise with an inference BatchNorm.
+ *
+ * codes, scales: NULL, or the buffers of an 8-bit checkpoint of x, written in the same pass.
+ *
+ * The backward pass takes dy, mean, rstd and either x or its checkpoint (codes, scales), the
+ * other NULL, and writes dx (dtype) and dweight, dbias ([C], param_dtype, either may be NULL);
+ * dx may be the buffer of dy.  ReLU's slope at 0 is 0.  With B == 0 dweight and dbias are zero.
+ *
+ * workspace: 16-byte aligned, at least the size dwb_group_norm_act_workspace reports for the
+ * shape (backward: 0 or 1); no two calls that may overlap share one.  0 bytes may be NULL. */
+DWB_API int dwb_group_norm_act_workspace(int64_t B, int64_t H, int64_t W, int64_t C, int G, int backward,
+                                         int64_t* bytes);
+DWB_API int dwb_group_norm_act_nhwc_fwd(const void* x, const void* weight, const void* bias, void* y,
+                                        float* mean, float* rstd, void* codes, void* scales,
+                                        void* workspace, int64_t workspace_bytes,
+                                        int64_t B, int64_t H, int64_t W, int64_t C, int G, double eps,
+                                        int act, int dtype, int param_dtype, void* stream);
+DWB_API int dwb_group_norm_act_nhwc_bwd(const void* dy, const void* x, const void* codes, const void* scales,
+                                        const float* mean, const float* rstd, const void* weight,
+                                        const void* bias, void* dx, void* dweight, void* dbias,
+                                        void* workspace, int64_t workspace_bytes,
+                                        int64_t B, int64_t H, int64_t W, int64_t C, int G,
+                                        int act, int dtype, int param_dtype, void* stream);
 
 /* ---- diagnostics ----------------------------------------------------------- */
 
