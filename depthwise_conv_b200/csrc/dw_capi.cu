@@ -185,6 +185,30 @@ int require_device() {
   return get_device_state(&st);
 }
 
+cudaError_t allow_large_cta(const void* fn) {
+  // the kernels that asked, and on which devices (a bit each) it has been done
+  static struct {
+    const void* fn;
+    uint64_t devices;
+  } known[128];
+  static std::mutex mu;
+  int dev = -1;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  std::lock_guard<std::mutex> lk(mu);
+  int i = 0;
+  while (i < 128 && known[i].fn && known[i].fn != fn) ++i;
+  if (i < 128 && known[i].fn == fn && (known[i].devices >> dev & 1)) return cudaSuccess;
+  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, g_devices[dev].hw.smem_optin);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess && i < 128) {  // a full table only means that the attributes are set again
+    known[i].fn = fn;
+    known[i].devices |= uint64_t{1} << dev;
+  }
+  return e;
+}
+
 static int regs_of_variant(int K, int R, int M, int acc, int pre, void* ctx) {
   DeviceState* st = static_cast<DeviceState*>(ctx);
   const KernelEntry* e = find_variant(K, R, M, acc, pre);

@@ -1,12 +1,14 @@
 // dw_groupnorm.cu -- group normalisation with an activation, channels last:
-// the split kernels (statistics, combination, application as separate
-// launches over row chunks) and the C entry points.  The formulas stand in
-// dw_groupnorm.cuh.
+// the C entry points, and the split kernels (statistics, combination,
+// application as separate launches over row chunks) for groups that are too
+// large for the shared memory of a cluster (dw_groupnorm_cluster.cu takes all
+// others).  The formulas stand in dw_groupnorm.cuh.
 #include <cuda_runtime.h>
 #include <math.h>
 
 #include "../../include/dwconv_b200.h"
 #include "dw_groupnorm.cuh"
+#include "dw_groupnorm_cluster.h"
 #include "dw_host.h"
 #include "dw_launch.h"
 
@@ -392,7 +394,12 @@ static int gn_shape(int64_t B, int64_t H, int64_t W, int64_t C, int G, double ep
 }
 
 // Workspace: the chunks' partial sums; for the backward pass also the samples' sums and the groups' means.
+// Resident kernels need the samples' sums only.
 static int64_t gn_workspace(const GnShape& s, bool backward) {
+  GnResident r;
+  if (backward ? gn_resident_plan(s, GnPass::kBackward16, &r) && gn_resident_plan(s, GnPass::kBackward8, &r)
+               : gn_resident_plan(s, GnPass::kForward, &r))
+    return backward ? static_cast<int64_t>(s.B) * s.C * static_cast<int64_t>(sizeof(float2)) : 0;
   const GnSplit p = gn_split(s);
   int64_t n = static_cast<int64_t>(s.B) * p.chunks * s.C;
   if (backward) n += static_cast<int64_t>(s.B) * s.C + static_cast<int64_t>(s.B) * s.G;
@@ -439,6 +446,9 @@ static const void* grad_apply_fn(int act) {
 template <typename T>
 static int gn_forward(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd, void* codes,
                       void* scales, void* workspace, GnShape s, int act, cudaStream_t stream) {
+  GnResident res;
+  if (gn_resident_plan(s, GnPass::kForward, &res))
+    return gn_resident_forward<T>(x, weight, bias, y, mean, rstd, codes, scales, s, res, act, stream);
   GnSplit p = gn_split(s);
   const dim3 grid(s.B, p.chunks, p.tiles);
   void* part = workspace;
@@ -456,23 +466,29 @@ template <typename T>
 static int gn_backward(const void* dy, const void* x, const void* codes, const void* scales, const float* mean,
                        const float* rstd, const void* weight, const void* bias, void* dx, void* dweight, void* dbias,
                        void* workspace, GnShape s, int act, cudaStream_t stream) {
-  GnSplit p = gn_split(s);
-  const dim3 grid(s.B, p.chunks, p.tiles);
-  float2* part = static_cast<float2*>(workspace);
-  float2* sums = part + static_cast<int64_t>(s.B) * p.chunks * s.C;
-  float2* m12 = sums + static_cast<int64_t>(s.B) * s.C;
-  const void* src = codes ? codes : x;
-  void* a1[] = {&dy, &src, &scales, &weight, &bias, &mean, &rstd, &part, &s, &p};
-  int rc = gn_launch(codes ? grad_sums_fn<T, true>(act) : grad_sums_fn<T, false>(act), "gn_grad_sums_kernel", grid, kGnThreads,
-                     a1, stream);
-  if (rc != DWB_OK) return rc;
-  void* a2[] = {&part, &weight, &sums, &m12, &s, &p};
-  rc = gn_launch(reinterpret_cast<const void*>(&gn_grad_combine_kernel<T>), "gn_grad_combine_kernel", dim3(s.B, s.G), 128, a2,
-                 stream);
-  if (rc != DWB_OK) return rc;
-  void* a3[] = {&dy, &src, &scales, &weight, &bias, &mean, &rstd, &m12, &dx, &s, &p};
-  rc = gn_launch(codes ? grad_apply_fn<T, true>(act) : grad_apply_fn<T, false>(act), "gn_grad_apply_kernel", grid, kGnThreads,
-                 a3, stream);
+  float2* sums = static_cast<float2*>(workspace);
+  int rc;
+  GnResident res;
+  if (gn_resident_plan(s, codes ? GnPass::kBackward8 : GnPass::kBackward16, &res)) {
+    rc = gn_resident_backward<T>(dy, x, codes, scales, mean, rstd, weight, bias, dx, sums, s, res, act, stream);
+  } else {
+    GnSplit p = gn_split(s);
+    const dim3 grid(s.B, p.chunks, p.tiles);
+    float2* m12 = sums + static_cast<int64_t>(s.B) * s.C;
+    float2* part = m12 + static_cast<int64_t>(s.B) * s.G;
+    const void* src = codes ? codes : x;
+    void* a1[] = {&dy, &src, &scales, &weight, &bias, &mean, &rstd, &part, &s, &p};
+    rc = gn_launch(codes ? grad_sums_fn<T, true>(act) : grad_sums_fn<T, false>(act), "gn_grad_sums_kernel", grid, kGnThreads,
+                   a1, stream);
+    if (rc != DWB_OK) return rc;
+    void* a2[] = {&part, &weight, &sums, &m12, &s, &p};
+    rc = gn_launch(reinterpret_cast<const void*>(&gn_grad_combine_kernel<T>), "gn_grad_combine_kernel", dim3(s.B, s.G), 128,
+                   a2, stream);
+    if (rc != DWB_OK) return rc;
+    void* a3[] = {&dy, &src, &scales, &weight, &bias, &mean, &rstd, &m12, &dx, &s, &p};
+    rc = gn_launch(codes ? grad_apply_fn<T, true>(act) : grad_apply_fn<T, false>(act), "gn_grad_apply_kernel", grid,
+                   kGnThreads, a3, stream);
+  }
   if (rc != DWB_OK || (!dweight && !dbias)) return rc;
   void* a4[] = {&sums, &dweight, &dbias, &s};
   return gn_launch(reinterpret_cast<const void*>(&gn_grad_params_kernel<T>), "gn_grad_params_kernel", dim3((s.C + 31) / 32), 256,

@@ -13,6 +13,10 @@ int record_cuda_failure(const char* what, cudaError_t e);
 // DWB_OK when the current device is an sm_100 part this library has kernels for.
 int require_device();
 
+// Let a kernel take all of an SM's shared memory and clusters of up to 16 CTAs
+// (set once per kernel and device).
+cudaError_t allow_large_cta(const void* fn);
+
 inline bool is_aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 // B200: the persistent and split grids of the host planners are sized for it.

@@ -424,7 +424,7 @@ extern "C" int dwb_conv2d_nhwc_bwd_weight_act8(const void* codes, const void* sc
   void* a1[] = {&codes, &scales, &dy, &part, &p};
   const void* fn = wgrad8_fn(K);
   const int smem = wgrad8_smem(p);
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_large_cta(fn);
   if (e == cudaSuccess)
     e = launch_kernel(fn, dim3(static_cast<unsigned>((C + kWgChannels - 1) / kWgChannels), p.chunks, p.col_tiles),
                       dim3(kWgThreads), a1, smem, st);
