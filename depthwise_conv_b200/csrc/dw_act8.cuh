@@ -42,6 +42,12 @@ struct Type16<__half> {
     const __half2 h = __floats2half2_rn(f.x, f.y);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
+  // min(max(v, -limit), limit) with limit = 127 * 2^9, the largest value a code stands for
+  static __device__ __forceinline__ uint32_t clamp_pair(uint32_t u) {
+    const __half2 lim = __half2half2(__ushort_as_half(0x7bf0));
+    const __half2 h = __hmax2(__hmin2(*reinterpret_cast<__half2*>(&u), lim), __hneg2(lim));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
   static __device__ __forceinline__ float to_float(__half h) { return __half2float(h); }
   static __device__ __forceinline__ uint32_t abs_to_f32_bits(uint32_t a) {
     return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(a))));
@@ -58,6 +64,12 @@ struct Type16<__nv_bfloat16> {
   static __device__ __forceinline__ uint32_t from_f32x2(f32x2 v) {
     const float2 f = bits_f2(v);
     const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  // limit = 127 * 2^121
+  static __device__ __forceinline__ uint32_t clamp_pair(uint32_t u) {
+    const __nv_bfloat162 lim = __bfloat162bfloat162(__ushort_as_bfloat16(0x7f7e));
+    const __nv_bfloat162 h = __hmax2(__hmin2(*reinterpret_cast<__nv_bfloat162*>(&u), lim), __hneg2(lim));
     return *reinterpret_cast<const uint32_t*>(&h);
   }
   static __device__ __forceinline__ float to_float(__nv_bfloat16 h) { return __bfloat162float(h); }
@@ -90,16 +102,9 @@ __device__ __forceinline__ uint32_t act8_block_amax(const uint4& v) {
   return max(a & 0xffffu, a >> 16);
 }
 
-// One value pair's codes in the low bytes of the two floats' bits: rint through the magic number
-// 1.5 * 2^23, whose unit is 1 (ties to even, as rint).
-__device__ __forceinline__ float2 act8_code_pair(f32x2 v, f32x2 inv) {
-  const float2 s = bits_f2(fmul2(v, inv));
-  const f32x2 c = f2_bits(make_float2(fminf(fmaxf(s.x, -127.0f), 127.0f), fminf(fmaxf(s.y, -127.0f), 127.0f)));
-  f32x2 r = splat2(12582912.0f);
-  fadd2(r, c);
-  return bits_f2(r);
-}
-
+// rint(x * 2^(127 - E)) through the magic number 1.5 * 2^23, whose unit is 1 (ties to even, as rint): the
+// code stands in the low byte.  The values are clamped in their own type first, two at a time; below that
+// limit every amax has an exponent that 127 steps reach.
 template <typename T>
 __device__ __forceinline__ uint2 act8_codes(const uint4& v, uint32_t E) {
   if (E == 255u) return make_uint2(0u, 0u);
@@ -108,7 +113,8 @@ __device__ __forceinline__ uint2 act8_codes(const uint4& v, uint32_t E) {
   uint32_t b[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 r = act8_code_pair(Type16<T>::to_f32x2(w[i]), inv);
+    // the product is exact (or so small that it rounds to 0), so one fma rounds as a product and a sum do
+    const float2 r = bits_f2(fma2(Type16<T>::to_f32x2(Type16<T>::clamp_pair(w[i])), inv, splat2(12582912.0f)));
     b[i] = __byte_perm(__float_as_uint(r.x), __float_as_uint(r.y), 0x0040);
   }
   return make_uint2(__byte_perm(b[0], b[1], 0x5410), __byte_perm(b[2], b[3], 0x5410));

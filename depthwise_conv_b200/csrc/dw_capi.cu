@@ -190,7 +190,7 @@ cudaError_t allow_large_cta(const void* fn) {
   static struct {
     const void* fn;
     uint64_t devices;
-  } known[128];
+  } known[256];
   static std::mutex mu;
   int dev = -1;
   cudaError_t e = cudaGetDevice(&dev);
@@ -198,11 +198,11 @@ cudaError_t allow_large_cta(const void* fn) {
   if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
   std::lock_guard<std::mutex> lk(mu);
   int i = 0;
-  while (i < 128 && known[i].fn && known[i].fn != fn) ++i;
-  if (i < 128 && known[i].fn == fn && (known[i].devices >> dev & 1)) return cudaSuccess;
+  while (i < 256 && known[i].fn && known[i].fn != fn) ++i;
+  if (i < 256 && known[i].fn == fn && (known[i].devices >> dev & 1)) return cudaSuccess;
   e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, g_devices[dev].hw.smem_optin);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e == cudaSuccess && i < 128) {  // a full table only means that the attributes are set again
+  if (e == cudaSuccess && i < 256) {  // a full table only means that the attributes are set again
     known[i].fn = fn;
     known[i].devices |= uint64_t{1} << dev;
   }

@@ -54,25 +54,29 @@ __global__ void __launch_bounds__(kGnThreads) gn_stats_kernel(const uint4* __res
   const GnThread th(s, p);
   const int width = p.lanes * 8;
   if (th.active) {
-    GnSums sums;
     const uint4* base = x + (th.sample * s.P * s.C + th.c) / 8;
     const long long step = s.C / 8;
-    for (long long r = th.r0 + th.lane_row; r < th.r1; r += 4LL * p.rl) {
-      uint4 v[4];
+    const long long r = th.r0 + th.lane_row;
+    if (r < th.r1) {
+      GnSums sums;
+      f32x2 f[4];
+      gn_unpack<T>(base[r * step], f);
+      sums.start(f);
+      const int n = static_cast<int>((th.r1 - r + p.rl - 1) / p.rl);
+      for (int i = 1; i < n; i += 4) {
+        uint4 v[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (r + i * p.rl < th.r1) v[i] = base[(r + static_cast<long long>(i) * p.rl) * step];
+        for (int j = 0; j < 4; ++j)
+          if (i + j < n) v[j] = base[(r + static_cast<long long>(i + j) * p.rl) * step];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (r + i * p.rl < th.r1) {
-          f32x2 f[4];
-          gn_unpack<T>(v[i], f);
-          sums.add(f);
-        }
-    }
-    if (sums.n) {
+        for (int j = 0; j < 4; ++j)
+          if (i + j < n) {
+            gn_unpack<T>(v[j], f);
+            sums.add(f);
+          }
+      }
       float mean[8], m2[8];
-      sums.moments(mean, m2);
+      sums.moments(n, mean, m2);
 #pragma unroll
       for (int i = 0; i < 8; ++i) ent[threadIdx.x * 8 + i] = make_float2(mean[i], m2[i]);
     }

@@ -26,13 +26,36 @@ namespace dwb {
 
 enum : int { kActSilu = 3 };  // after kActNone, kActRelu, kActGelu
 
+// erfc(a / sqrt 2) / 2 = exp(-a^2 / 2) * poly(t) t for a = |u|, t = 1 / (1 + p a): Abramowitz & Stegun
+// 7.1.26 (|error| <= 1.5e-7), as gelu_erf2 uses it.  Returns poly(t), t and the exponential.
+struct HalfErfc {
+  f32x2 a, poly, t, e;
+};
+__device__ __forceinline__ HalfErfc half_erfc2(f32x2 u) {
+  HalfErfc r;
+  r.a = u & 0x7fffffff7fffffffull;
+  const float2 d = bits_f2(fma2(r.a, splat2(0.3275911f * 0.70710678118654752f), splat2(1.0f)));
+  r.t = f2_bits(make_float2(rcp_approx(d.x), rcp_approx(d.y)));
+  f32x2 q = fma2(splat2(0.5f * 1.061405429f), r.t, splat2(0.5f * -1.453152027f));
+  q = fma2(q, r.t, splat2(0.5f * 1.421413741f));
+  q = fma2(q, r.t, splat2(0.5f * -0.284496736f));
+  r.poly = fma2(q, r.t, splat2(0.5f * 0.254829592f));
+  const float2 x = bits_f2(fmul2(fmul2(u, splat2(-0.5f * 1.4426950408889634f)), u));
+  r.e = f2_bits(make_float2(ex2_approx(x.x), ex2_approx(x.y)));
+  return r;
+}
+
 template <int ACT>
 __device__ __forceinline__ f32x2 act_value2(f32x2 u) {
   if constexpr (ACT == kActRelu) {
     const float2 f = bits_f2(u);  // a comparison, not fmaxf: NaN stays NaN
     return f2_bits(make_float2(f.x < 0.0f ? 0.0f : f.x, f.y < 0.0f ? 0.0f : f.y));
   } else if constexpr (ACT == kActGelu) {
-    return gelu_erf2(u);
+    // u Phi(u) = max(u, 0) - |u| erfc(|u| / sqrt 2) / 2, on both sides of 0: no selection
+    const HalfErfc h = half_erfc2(u);
+    const float2 f = bits_f2(u);
+    const f32x2 lost = fmul2(fmul2(h.poly, h.t), h.e);
+    return fma2(fmul2(h.a, splat2(-1.0f)), lost, f2_bits(make_float2(fmaxf(f.x, 0.0f), fmaxf(f.y, 0.0f))));
   } else if constexpr (ACT == kActSilu) {
     const float2 e = bits_f2(fmul2(u, splat2(-1.4426950408889634f)));
     const f32x2 d = fma2(f2_bits(make_float2(ex2_approx(e.x), ex2_approx(e.y))), splat2(1.0f), splat2(1.0f));
@@ -43,32 +66,27 @@ __device__ __forceinline__ f32x2 act_value2(f32x2 u) {
   }
 }
 
-// act'(u).  GELU: Phi(u) + u phi(u), Phi from the erfc approximation of gelu_erf2 (Abramowitz & Stegun
-// 7.1.26), whose exponential phi shares: two special-function operations a value.  ReLU: 0 at 0.
+// act'(u).  ReLU: 0 at 0.
 template <int ACT>
 __device__ __forceinline__ f32x2 act_slope2(f32x2 u) {
   if constexpr (ACT == kActRelu) {
     const float2 f = bits_f2(u);
     return f2_bits(make_float2(f.x > 0.0f ? 1.0f : 0.0f, f.y > 0.0f ? 1.0f : 0.0f));
   } else if constexpr (ACT == kActGelu) {
-    const f32x2 au = u & 0x7fffffff7fffffffull;
-    const float2 d = bits_f2(fma2(au, splat2(0.3275911f * 0.70710678118654752f), splat2(1.0f)));
-    const f32x2 t = f2_bits(make_float2(rcp_approx(d.x), rcp_approx(d.y)));
-    f32x2 poly = fma2(splat2(0.5f * 1.061405429f), t, splat2(0.5f * -1.453152027f));
-    poly = fma2(poly, t, splat2(0.5f * 1.421413741f));
-    poly = fma2(poly, t, splat2(0.5f * -0.284496736f));
-    poly = fma2(poly, t, splat2(0.5f * 0.254829592f));
-    poly = fmul2(poly, t);
-    const float2 ea = bits_f2(fmul2(fmul2(u, splat2(-0.5f * 1.4426950408889634f)), u));
-    const f32x2 e = f2_bits(make_float2(ex2_approx(ea.x), ex2_approx(ea.y)));  // exp(-u^2 / 2)
-    const float2 h = bits_f2(fmul2(poly, e));                                  // erfc(|u| / sqrt 2) / 2
-    const float2 uf = bits_f2(u);
-    const f32x2 cdf = f2_bits(make_float2(uf.x < 0.0f ? h.x : 1.0f - h.x, uf.y < 0.0f ? h.y : 1.0f - h.y));
-    return fma2(fmul2(u, splat2(0.3989422804014327f)), e, cdf);
+    // Phi(u) + u phi(u) with k = erfc(|u| / sqrt 2) / 2 - |u| phi(u) is k below 0 and 1 - k above:
+    // 1/2 + (1/2 - k) with the sign of u.  phi has the exponential that erfc has.
+    const HalfErfc h = half_erfc2(u);
+    const f32x2 k = fma2(h.poly, h.t, fmul2(h.a, splat2(-0.3989422804014327f)));
+    const f32x2 d = fma2(fmul2(k, splat2(-1.0f)), h.e, splat2(0.5f));
+    f32x2 r = splat2(0.5f);
+    fadd2(r, d ^ (u & 0x8000000080000000ull));
+    return r;
   } else if constexpr (ACT == kActSilu) {
     const float2 e = bits_f2(fmul2(u, splat2(-1.4426950408889634f)));
-    const float2 s = make_float2(rcp_approx(1.0f + ex2_approx(e.x)), rcp_approx(1.0f + ex2_approx(e.y)));
-    const f32x2 sv = f2_bits(s);
+    f32x2 d = splat2(1.0f);
+    fadd2(d, f2_bits(make_float2(ex2_approx(e.x), ex2_approx(e.y))));
+    const float2 df = bits_f2(d);
+    const f32x2 sv = f2_bits(make_float2(rcp_approx(df.x), rcp_approx(df.y)));
     const f32x2 rest = fma2(sv, splat2(-1.0f), splat2(1.0f));  // 1 - s
     return fmul2(sv, fma2(u, rest, splat2(1.0f)));
   } else {
@@ -120,26 +138,23 @@ __device__ __forceinline__ f32x2 fsub2(f32x2 a, f32x2 b) { return fma2(b, splat2
 // Sums of one thread about its own first values.
 struct GnSums {
   f32x2 k[4], s1[4], s2[4];
-  int n = 0;
-  __device__ __forceinline__ void add(const f32x2 (&v)[4]) {
-    if (n == 0) {
+  __device__ __forceinline__ void start(const f32x2 (&v)[4]) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        k[i] = v[i];
-        s1[i] = s2[i] = f32x2_zero();
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x2 d = fsub2(v[i], k[i]);
-        fadd2(s1[i], d);
-        ffma2(s2[i], d, d);
-      }
+    for (int i = 0; i < 4; ++i) {
+      k[i] = v[i];
+      s1[i] = s2[i] = f32x2_zero();
     }
-    ++n;
   }
-  // per-channel mean and sum of squared deviations (n >= 1)
-  __device__ __forceinline__ void moments(float (&mean)[8], float (&m2)[8]) const {
+  __device__ __forceinline__ void add(const f32x2 (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x2 d = fsub2(v[i], k[i]);
+      fadd2(s1[i], d);
+      ffma2(s2[i], d, d);
+    }
+  }
+  // per-channel mean and sum of squared deviations of the n >= 1 values seen
+  __device__ __forceinline__ void moments(int n, float (&mean)[8], float (&m2)[8]) const {
     const float inv = 1.0f / static_cast<float>(n);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

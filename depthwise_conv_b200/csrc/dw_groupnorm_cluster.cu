@@ -22,8 +22,8 @@
 
 namespace dwb {
 
-constexpr int kGnForwardThreads = 512;
-constexpr int kGnBackwardThreads = 256;
+constexpr int kGnThreads = 256;
+constexpr int kGnForwardCtas = 4, kGnBackwardCtas = 2;  // CTAs an SM that the registers have to allow
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
@@ -87,84 +87,118 @@ struct GnPlace {
 // Pixels of a CTA that lane row `lr` handles.
 __device__ __forceinline__ int gn_lane_rows(int rows, int lr, int rl) { return rows > lr ? (rows - lr + rl - 1) / rl : 0; }
 
-// ONE: C / G is a multiple of 8, so that a thread's vector lies in one group.
-template <typename T, int ACT, bool CKPT, bool ONE>
-__global__ void __launch_bounds__(kGnForwardThreads, 2)
+// SUB: channels of a vector that surely share a group (8, 4 or 1: C / G is a multiple of it).
+template <int SUB>
+__device__ __forceinline__ f32x2 gn_of(const f32x2 (&v)[SUB == 8 ? 1 : SUB == 4 ? 2 : 4], int pair) {
+  return v[SUB == 8 ? 0 : SUB == 4 ? pair / 2 : pair];
+}
+
+// The two halves of what the groups of a thread's channels hold in `fin`.
+template <int SUB>
+__device__ __forceinline__ void gn_read_groups(const float2* fin, int first, int Cg, f32x2 (&x)[SUB == 8 ? 1 : SUB == 4 ? 2 : 4],
+                                               f32x2 (&y)[SUB == 8 ? 1 : SUB == 4 ? 2 : 4]) {
+#pragma unroll
+  for (int i = 0; i < (SUB == 8 ? 1 : SUB == 4 ? 2 : 4); ++i) {
+    const int c = first + i * (SUB == 1 ? 2 : SUB);
+    const float2 lo = fin[c / Cg], hi = SUB == 1 ? fin[(c + 1) / Cg] : lo;
+    x[i] = f2_bits(make_float2(lo.x, hi.x));
+    y[i] = f2_bits(make_float2(lo.y, hi.y));
+  }
+}
+
+template <typename T, int ACT, bool CKPT, int SUB>
+__global__ void __launch_bounds__(kGnThreads, kGnForwardCtas)
     gn_resident_kernel(const T* __restrict__ x, const void* __restrict__ weight, const void* __restrict__ bias,
                        T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
                        int8_t* __restrict__ codes, uint8_t* __restrict__ scales, const GnShape s, const GnResident p) {
   extern __shared__ __align__(16) unsigned char smem[];
+  constexpr int kEnt = 8 / SUB;                   // moments a thread hands over
+  constexpr int kParts = SUB == 8 ? 1 : SUB == 4 ? 2 : 4;
   uint4* stage = reinterpret_cast<uint4*>(smem);  // [iters][threads]: a thread's own vectors
   float2* ent = reinterpret_cast<float2*>(stage + p.iters * p.threads);
-  float2* grp = ent + p.threads * (ONE ? 1 : 8);
-  const int groups = p.slab / s.Cg;
-  float2* fin = grp + groups;
+  float2* grp = ent + p.threads * kEnt;
+  float2* fin = grp + p.slab / s.Cg;
   griddep_wait();
   griddep_launch_dependents();
   const GnPlace at(s, p);
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, nt = p.threads;
   const long long first = (at.sample * s.P + at.r0 + at.lane_row) * s.C + at.c;  // this thread's first value
   const long long step = static_cast<long long>(p.rl) * s.C;
   const int mine = at.active ? gn_lane_rows(at.rows, at.lane_row, p.rl) : 0;
   const int quarter = (p.iters + 3) / 4;
-  for (int part = 0; part < 4; ++part) {
-    const int end = min(mine, (part + 1) * quarter);
-    for (int i = part * quarter; i < end; ++i) cp_async16(stage + i * p.threads + tid, x + first + i * step);
-    cp_async_commit();
-  }
-  GnSums sums;
-  for (int part = 0; part < 4; ++part) {
-    cp_async_wait_part(part);
-    const int end = min(mine, (part + 1) * quarter);
-    for (int i = part * quarter; i < end; ++i) {
-      f32x2 f[4];
-      gn_unpack<T>(stage[i * p.threads + tid], f);
-      sums.add(f);
+  {
+    const T* src = x + first;
+    uint4* dst = stage + tid;
+    for (int part = 0; part < 4; ++part) {
+      const int end = min(mine, (part + 1) * quarter);
+#pragma unroll 4
+      for (int i = part * quarter; i < end; ++i, src += step, dst += nt) cp_async16(dst, src);
+      cp_async_commit();
     }
   }
-  if (sums.n) {
+  if (mine) {
+    GnSums sums;
+    f32x2 f[4];
+    const uint4* v = stage + tid;
+    cp_async_wait_part(0);
+    gn_unpack<T>(*v, f);
+    sums.start(f);
+    v += nt;
+    int i = 1;
+    for (int part = 0; part < 4; ++part) {
+      cp_async_wait_part(part);
+      const int end = min(mine, (part + 1) * quarter);
+#pragma unroll 4
+      for (; i < end; ++i, v += nt) {
+        gn_unpack<T>(*v, f);
+        sums.add(f);
+      }
+    }
     float mean[8], m2[8];
-    sums.moments(mean, m2);
-    if constexpr (ONE) {
+    sums.moments(mine, mean, m2);
+#pragma unroll
+    for (int e = 0; e < kEnt; ++e) {
       float m = 0.0f, q = 0.0f, d2 = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m += mean[i];
-      m *= 0.125f;
+      for (int k = 0; k < SUB; ++k) m += mean[e * SUB + k];
+      m *= 1.0f / SUB;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        q += m2[i];
-        d2 += (mean[i] - m) * (mean[i] - m);
+      for (int k = 0; k < SUB; ++k) {
+        q += m2[e * SUB + k];
+        d2 += (mean[e * SUB + k] - m) * (mean[e * SUB + k] - m);
       }
-      ent[tid] = make_float2(m, q + static_cast<float>(sums.n) * d2);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ent[tid * 8 + i] = make_float2(mean[i], m2[i]);
+      ent[tid * kEnt + e] = make_float2(m, q + static_cast<float>(mine) * d2);
     }
   }
   __syncthreads();
-  // one warp a group: the moments of this CTA's pixels
-  const int lane = tid & 31, warps = blockDim.x >> 5, here = at.width / s.Cg;
-  for (int g = tid >> 5; g < here; g += warps) {
-    const int per_row = ONE ? s.Cg / 8 : s.Cg;
-    const int live = min(at.rows, p.rl), entries = per_row * live;
-    auto entry = [&](int e, float& n) {
-      const int lr = e / per_row, k = g * per_row + (e - lr * per_row);
-      n = static_cast<float>(gn_lane_rows(at.rows, lr, p.rl) * (ONE ? 8 : 1));
-      return ONE ? ent[lr * p.lanes + k] : ent[lr * p.lanes * 8 + k];
-    };
-    float sum = 0.0f, m2 = 0.0f, n;
-    for (int e = lane; e < entries; e += 32) {
-      const float2 v = entry(e, n);
-      sum += n * v.x;
+  // one warp a group: the moments of this CTA's pixels.  Lanes go along the group's entries of a pixel first.
+  const int lane = tid & 31, warps = nt >> 5, here = at.width / s.Cg;
+  {
+    const int per_row = s.Cg / SUB, live = min(at.rows, p.rl);
+    const int turns = at.rows / p.rl, rest = at.rows - turns * p.rl;  // lane rows below `rest` have a pixel more
+    const bool fits = per_row <= 32;
+    const int k0 = fits ? lane % per_row : lane, k_step = fits ? per_row : 32;
+    const int r_step = fits ? 32 / per_row : 1, r0 = fits ? lane / per_row : 0;
+    for (int g = tid >> 5; g < here; g += warps) {
+      const float2* of_group = ent + g * per_row;
+      float sum = 0.0f, m2 = 0.0f;
+      if (r0 < r_step)
+        for (int r = r0; r < live; r += r_step) {
+          const float n = static_cast<float>((turns + (r < rest)) * SUB);
+          for (int k = k0; k < per_row; k += k_step) sum += n * of_group[r * p.lanes * kEnt + k].x;
+        }
+      const float mean = at.rows ? warp_sum(sum) / (static_cast<float>(at.rows) * static_cast<float>(s.Cg)) : 0.0f;
+      if (r0 < r_step)
+        for (int r = r0; r < live; r += r_step) {
+          const float n = static_cast<float>((turns + (r < rest)) * SUB);
+          for (int k = k0; k < per_row; k += k_step) {
+            const float2 v = of_group[r * p.lanes * kEnt + k];
+            m2 += v.y + n * (v.x - mean) * (v.x - mean);
+          }
+        }
+      m2 = warp_sum(m2);
+      if (lane == 0) grp[g] = make_float2(mean, m2);
     }
-    const float total = static_cast<float>(at.rows) * static_cast<float>(s.Cg);
-    const float mean = at.rows ? warp_sum(sum) / total : 0.0f;
-    for (int e = lane; e < entries; e += 32) {
-      const float2 v = entry(e, n);
-      m2 += v.y + n * (v.x - mean) * (v.x - mean);
-    }
-    m2 = warp_sum(m2);
-    if (lane == 0) grp[g] = make_float2(mean, m2);
   }
   if (p.cluster > 1) {
     cluster_arrive();
@@ -172,13 +206,9 @@ __global__ void __launch_bounds__(kGnForwardThreads, 2)
   } else {
     __syncthreads();
   }
-  for (int g = tid; g < here; g += blockDim.x) {
-    const float n = static_cast<float>(s.P) * static_cast<float>(s.Cg);
-    float mean, m2;
-    if (p.cluster == 1) {
-      mean = grp[g].x;
-      m2 = grp[g].y;
-    } else {
+  for (int g = tid; g < here; g += nt) {
+    float mean = grp[g].x, m2 = grp[g].y;
+    if (p.cluster > 1) {
       float sum = 0.0f;
       for (int r = 0; r < p.cluster; ++r)
         sum += static_cast<float>(GnPlace::rows_of(s, p, r)) * cluster_load(grp + g, r).x;
@@ -189,7 +219,7 @@ __global__ void __launch_bounds__(kGnForwardThreads, 2)
         m2 += v.y + static_cast<float>(GnPlace::rows_of(s, p, r)) * static_cast<float>(s.Cg) * (v.x - mean) * (v.x - mean);
       }
     }
-    const float rstd = 1.0f / sqrtf(m2 / n + s.eps);
+    const float rstd = 1.0f / sqrtf(m2 / (static_cast<float>(s.P) * static_cast<float>(s.Cg)) + s.eps);
     fin[g] = make_float2(mean, rstd);
     if (at.rank == 0) {
       const long long o = at.sample * s.G + at.c_base / s.Cg + g;
@@ -199,145 +229,152 @@ __global__ void __launch_bounds__(kGnForwardThreads, 2)
   }
   if (p.cluster > 1) cluster_arrive();  // this CTA has read the others' moments
   __syncthreads();
-  f32x2 w[4], b[4], m[4], rs[4];
+  f32x2 w[4], b[4], m[kParts];
   if (at.active) {
+    f32x2 rs[kParts];
     gn_load_params<T>(weight, bias, at.c, s.param_f32, w, b);
-    if constexpr (ONE) {
-      const float2 f = fin[at.vec * 8 / s.Cg];
+    gn_read_groups<SUB>(fin, at.vec * 8, s.Cg, m, rs);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        m[i] = splat2(f.x);
-        rs[i] = splat2(f.y);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 lo = fin[(at.vec * 8 + 2 * i) / s.Cg], hi = fin[(at.vec * 8 + 2 * i + 1) / s.Cg];
-        m[i] = f2_bits(make_float2(lo.x, hi.x));
-        rs[i] = f2_bits(make_float2(lo.y, hi.y));
-      }
-    }
+    for (int j = 0; j < 4; ++j) w[j] = fmul2(w[j], gn_of<SUB>(rs, j));
   }
-  const long long sblocks = (s.C + kAct8Block - 1) / kAct8Block;
-  // a checkpoint's block maximum is a warp shuffle: every lane goes through every turn
-  const int turns = CKPT ? gn_lane_rows(at.rows, 0, p.rl) : mine;
-  for (int i = 0; i < turns; ++i) {
-    const bool on = i < mine;
-    const uint4 v = on ? stage[i * p.threads + tid] : make_uint4(0u, 0u, 0u, 0u);
-    if constexpr (CKPT) {
-      const uint32_t E = act8_exponent<T>(act8_block_amax(v));
+  const uint4* v = stage + tid;
+  T* yp = y + first;
+  if constexpr (CKPT) {
+    const long long sblocks = (s.C + kAct8Block - 1) / kAct8Block;
+    int8_t* qp = codes + first;
+    uint8_t* sp = scales + (at.sample * s.P + at.r0 + at.lane_row) * sblocks + at.c / kAct8Block;
+    const long long sstep = p.rl * sblocks;
+    // a block's maximum is a warp shuffle: every lane goes through every turn
+    const int turns = gn_lane_rows(at.rows, 0, p.rl);
+#pragma unroll 2
+    for (int i = 0; i < turns; ++i, v += nt, yp += step, qp += step, sp += sstep) {
+      const bool on = i < mine;
+      const uint4 u = on ? *v : make_uint4(0u, 0u, 0u, 0u);
+      const uint32_t E = act8_exponent<T>(act8_block_amax(u));
       if (on) {
-        *reinterpret_cast<uint2*>(codes + first + i * step) = act8_codes<T>(v, E);
-        if ((at.vec & 3) == 0)
-          scales[(at.sample * s.P + at.r0 + at.lane_row + static_cast<long long>(i) * p.rl) * sblocks + at.c / kAct8Block] =
-              static_cast<uint8_t>(E);
+        *reinterpret_cast<uint2*>(qp) = act8_codes<T>(u, E);
+        if ((at.vec & 3) == 0) *sp = static_cast<uint8_t>(E);
+        f32x2 f[4];
+        gn_unpack<T>(u, f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = act_value2<ACT>(fma2(fsub2(f[j], gn_of<SUB>(m, j)), w[j], b[j]));
+        *reinterpret_cast<uint4*>(yp) = gn_pack<T>(f);
       }
     }
-    if (on) {
+  } else {
+#pragma unroll 2
+    for (int i = 0; i < mine; ++i, v += nt, yp += step) {
       f32x2 f[4];
-      gn_unpack<T>(v, f);
+      gn_unpack<T>(*v, f);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) f[j] = act_value2<ACT>(fma2(fmul2(fsub2(f[j], m[j]), rs[j]), w[j], b[j]));
-      *reinterpret_cast<uint4*>(y + first + i * step) = gn_pack<T>(f);
+      for (int j = 0; j < 4; ++j) f[j] = act_value2<ACT>(fma2(fsub2(f[j], gn_of<SUB>(m, j)), w[j], b[j]));
+      *reinterpret_cast<uint4*>(yp) = gn_pack<T>(f);
     }
   }
   if (p.cluster > 1) cluster_wait();  // nobody reads this CTA's shared memory any more
 }
 
-template <typename T, int ACT, bool SRC8, bool ONE>
-__global__ void __launch_bounds__(kGnBackwardThreads, 2)
+// The slope of the activation costs most of the arithmetic, so g = dy act'(u) is computed once and kept in fp32
+// where dy lay (dy lands in the second half of g's place) for the second use.
+template <typename T, int ACT, bool SRC8, int SUB>
+__global__ void __launch_bounds__(kGnThreads, kGnBackwardCtas)
     gn_resident_grad_kernel(const T* __restrict__ dy, const void* __restrict__ src, const uint8_t* __restrict__ scales,
                             const void* __restrict__ weight, const void* __restrict__ bias, const float* __restrict__ mean,
                             const float* __restrict__ rstd, T* __restrict__ dx, float2* __restrict__ sums_out,
                             const GnShape s, const GnResident p) {
   extern __shared__ __align__(16) unsigned char smem[];
-  uint4* stage = reinterpret_cast<uint4*>(smem);  // dy
-  unsigned char* saved = reinterpret_cast<unsigned char*>(stage + p.iters * p.threads);
+  constexpr int kParts = SUB == 8 ? 1 : SUB == 4 ? 2 : 4;
   constexpr int kSaved = SRC8 ? 8 : 16;
-  float2* ent = reinterpret_cast<float2*>(saved + p.iters * p.threads * kSaved);
-  float2* chan = ent + p.threads * 8;
+  const int nt = p.threads, tid = threadIdx.x;
+  uint4* g_lo = reinterpret_cast<uint4*>(smem);   // [iters][threads] g of channels 0..3
+  uint4* g_hi = g_lo + p.iters * nt;              // [iters][threads] dy, then g of channels 4..7
+  unsigned char* saved = reinterpret_cast<unsigned char*>(g_hi + p.iters * nt);
+  float2* ent = reinterpret_cast<float2*>(saved + p.iters * nt * kSaved);
+  float2* chan = ent + nt * 8;
   float2* total = chan + p.slab;
   float2* fin = total + p.slab;
   griddep_wait();
   griddep_launch_dependents();
   const GnPlace at(s, p);
-  const int tid = threadIdx.x;
   const long long pixel0 = at.sample * s.P + at.r0 + at.lane_row;
   const long long first = pixel0 * s.C + at.c;
   const long long step = static_cast<long long>(p.rl) * s.C;
   const long long sblocks = (s.C + kAct8Block - 1) / kAct8Block;
   const int mine = at.active ? gn_lane_rows(at.rows, at.lane_row, p.rl) : 0;
   const int quarter = (p.iters + 3) / 4;
-  for (int part = 0; part < 4; ++part) {
-    const int end = min(mine, (part + 1) * quarter);
-    for (int i = part * quarter; i < end; ++i) {
-      cp_async16(stage + i * p.threads + tid, dy + first + i * step);
-      if constexpr (SRC8)
-        cp_async8(saved + (i * p.threads + tid) * kSaved, static_cast<const int8_t*>(src) + first + i * step);
-      else
-        cp_async16(saved + (i * p.threads + tid) * kSaved, static_cast<const T*>(src) + first + i * step);
+  {
+    const T* a = dy + first;
+    const unsigned char* q = static_cast<const unsigned char*>(src) + first * (SRC8 ? 1 : 2);
+    uint4* da = g_hi + tid;
+    unsigned char* dq = saved + tid * kSaved;
+    for (int part = 0; part < 4; ++part) {
+      const int end = min(mine, (part + 1) * quarter);
+#pragma unroll 2
+      for (int i = part * quarter; i < end; ++i, a += step, q += step * (SRC8 ? 1 : 2), da += nt, dq += nt * kSaved) {
+        cp_async16(da, a);
+        if constexpr (SRC8) cp_async8(dq, q);
+        else cp_async16(dq, q);
+      }
+      cp_async_commit();
     }
-    cp_async_commit();
   }
-  f32x2 w[4], b[4], m[4], rs[4];
+  f32x2 w[4], b[4], m[kParts], rs[kParts];
   if (at.active) {
     gn_load_params<T>(weight, bias, at.c, s.param_f32, w, b);
-    if constexpr (ONE) {
-      const long long o = at.sample * s.G + at.c / s.Cg;
-      const f32x2 mv = splat2(mean[o]), rv = splat2(rstd[o]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        m[i] = mv;
-        rs[i] = rv;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const long long lo = at.sample * s.G + (at.c + 2 * i) / s.Cg, hi = at.sample * s.G + (at.c + 2 * i + 1) / s.Cg;
-        m[i] = f2_bits(make_float2(mean[lo], mean[hi]));
-        rs[i] = f2_bits(make_float2(rstd[lo], rstd[hi]));
-      }
+    for (int i = 0; i < kParts; ++i) {
+      const int c = at.c + i * (SUB == 1 ? 2 : SUB);
+      const long long lo = at.sample * s.G + c / s.Cg, hi = SUB == 1 ? at.sample * s.G + (c + 1) / s.Cg : lo;
+      m[i] = f2_bits(make_float2(mean[lo], mean[hi]));
+      rs[i] = f2_bits(make_float2(rstd[lo], rstd[hi]));
     }
   }
-  // x_hat and g = dy act'(u) of this thread's vector i
-  auto normalised = [&](int i, uint32_t E, f32x2(&xh)[4], f32x2(&g)[4]) {
-    f32x2 d[4];
-    gn_unpack<T>(stage[i * p.threads + tid], d);
-    if constexpr (SRC8)
-      act8_values(*reinterpret_cast<const uint2*>(saved + (i * p.threads + tid) * kSaved), act8_step(E), xh);
-    else
-      gn_unpack<T>(*reinterpret_cast<const uint4*>(saved + (i * p.threads + tid) * kSaved), xh);
+  const uint8_t* const sp0 = SRC8 ? scales + pixel0 * sblocks + at.c / kAct8Block : nullptr;
+  const long long sstep = p.rl * sblocks;
+  auto x_hat = [&](const unsigned char* at_saved, uint32_t E, f32x2(&xh)[4]) {
+    if constexpr (SRC8) act8_values(*reinterpret_cast<const uint2*>(at_saved), act8_step(E), xh);
+    else gn_unpack<T>(*reinterpret_cast<const uint4*>(at_saved), xh);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) xh[j] = fmul2(fsub2(xh[j], gn_of<SUB>(m, j)), gn_of<SUB>(rs, j));
+  };
+  {
+    f32x2 sg[4], sx[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sg[j] = sx[j] = f32x2_zero();
+    const unsigned char* q = saved + tid * kSaved;
+    uint4 *lo = g_lo + tid, *hi = g_hi + tid;
+    const uint8_t* sp = sp0;
+    for (int part = 0; part < 4; ++part) {
+      cp_async_wait_part(part);
+      const int end = min(mine, (part + 1) * quarter);
+#pragma unroll 2
+      for (int i = part * quarter; i < end; ++i, q += nt * kSaved, lo += nt, hi += nt) {
+        uint32_t E = 0;
+        if constexpr (SRC8) {
+          E = *sp;
+          sp += sstep;
+        }
+        f32x2 xh[4], g[4];
+        x_hat(q, E, xh);
+        gn_unpack<T>(*hi, g);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          g[j] = fmul2(g[j], act_slope2<ACT>(fma2(xh[j], w[j], b[j])));
+          fadd2(sg[j], g[j]);
+          ffma2(sx[j], g[j], xh[j]);
+        }
+        *reinterpret_cast<ulonglong2*>(lo) = make_ulonglong2(g[0], g[1]);
+        *reinterpret_cast<ulonglong2*>(hi) = make_ulonglong2(g[2], g[3]);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      xh[j] = fmul2(fsub2(xh[j], m[j]), rs[j]);
-      g[j] = fmul2(d[j], act_slope2<ACT>(fma2(xh[j], w[j], b[j])));
+      const float2 a = bits_f2(sg[j]), c = bits_f2(sx[j]);
+      *reinterpret_cast<float4*>(ent + tid * 8 + 2 * j) = make_float4(a.x, c.x, a.y, c.y);
     }
-  };
-  const uint8_t* sc = SRC8 ? scales + pixel0 * sblocks + at.c / kAct8Block : nullptr;
-  f32x2 sg[4], sx[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) sg[j] = sx[j] = f32x2_zero();
-  for (int part = 0; part < 4; ++part) {
-    cp_async_wait_part(part);
-    const int end = min(mine, (part + 1) * quarter);
-    for (int i = part * quarter; i < end; ++i) {
-      f32x2 xh[4], g[4];
-      normalised(i, SRC8 ? sc[static_cast<long long>(i) * p.rl * sblocks] : 0u, xh, g);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        fadd2(sg[j], g[j]);
-        ffma2(sx[j], g[j], xh[j]);
-      }
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 a = bits_f2(sg[j]), q = bits_f2(sx[j]);
-    ent[tid * 8 + 2 * j] = make_float2(a.x, q.x);
-    ent[tid * 8 + 2 * j + 1] = make_float2(a.y, q.y);
   }
   __syncthreads();
-  for (int j = tid; j < at.width; j += blockDim.x) {
+  for (int j = tid; j < at.width; j += nt) {
     float2 a = make_float2(0.0f, 0.0f);
 #pragma unroll 4
     for (int r = 0; r < p.rl; ++r) {
@@ -353,7 +390,7 @@ __global__ void __launch_bounds__(kGnBackwardThreads, 2)
   } else {
     __syncthreads();
   }
-  for (int j = tid; j < at.width; j += blockDim.x) {
+  for (int j = tid; j < at.width; j += nt) {
     float2 a = chan[j];
     if (p.cluster > 1) {
       a = make_float2(0.0f, 0.0f);
@@ -370,7 +407,7 @@ __global__ void __launch_bounds__(kGnBackwardThreads, 2)
   if (p.cluster > 1) cluster_arrive();
   __syncthreads();
   const float inv = 1.0f / (static_cast<float>(s.P) * static_cast<float>(s.Cg));
-  const int lane = tid & 31, warps = blockDim.x >> 5, here = at.width / s.Cg;
+  const int lane = tid & 31, warps = nt >> 5, here = at.width / s.Cg;
   for (int g = tid >> 5; g < here; g += warps) {
     float m1 = 0.0f, m2 = 0.0f;
     for (int j = lane; j < s.Cg; j += 32) {
@@ -382,31 +419,29 @@ __global__ void __launch_bounds__(kGnBackwardThreads, 2)
     if (lane == 0) fin[g] = make_float2(m1 * inv, -m2 * inv);
   }
   __syncthreads();
-  f32x2 m1[4], m2[4];
-  if (at.active) {
-    if constexpr (ONE) {
-      const float2 f = fin[at.vec * 8 / s.Cg];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        m1[i] = splat2(f.x);
-        m2[i] = splat2(f.y);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 lo = fin[(at.vec * 8 + 2 * i) / s.Cg], hi = fin[(at.vec * 8 + 2 * i + 1) / s.Cg];
-        m1[i] = f2_bits(make_float2(lo.x, hi.x));
-        m2[i] = f2_bits(make_float2(lo.y, hi.y));
-      }
+  f32x2 m1[kParts], m2[kParts];
+  if (at.active) gn_read_groups<SUB>(fin, at.vec * 8, s.Cg, m1, m2);
+  const unsigned char* q = saved + tid * kSaved;
+  const uint4 *lo = g_lo + tid, *hi = g_hi + tid;
+  const uint8_t* sp = sp0;
+  T* out = dx + first;
+#pragma unroll 2
+  for (int i = 0; i < mine; ++i, q += nt * kSaved, lo += nt, hi += nt, out += step) {
+    uint32_t E = 0;
+    if constexpr (SRC8) {
+      E = *sp;
+      sp += sstep;
     }
-  }
-  for (int i = 0; i < mine; ++i) {
-    f32x2 xh[4], g[4];
-    normalised(i, SRC8 ? sc[static_cast<long long>(i) * p.rl * sblocks] : 0u, xh, g);
+    f32x2 xh[4];
+    x_hat(q, E, xh);
+    const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(lo), c = *reinterpret_cast<const ulonglong2*>(hi);
+    const f32x2 g[4] = {a.x, a.y, c.x, c.y};
     // the product rounded by itself, so that a group whose m1 is that product leaves exactly nothing
 #pragma unroll
-    for (int j = 0; j < 4; ++j) xh[j] = fmul2(rs[j], fma2(xh[j], m2[j], fsub2(fmul2(g[j], w[j]), m1[j])));
-    *reinterpret_cast<uint4*>(dx + first + i * step) = gn_pack<T>(xh);
+    for (int j = 0; j < 4; ++j)
+      xh[j] = fmul2(gn_of<SUB>(rs, j),
+                    fma2(xh[j], gn_of<SUB>(m2, j), fsub2(fmul2(g[j], w[j]), gn_of<SUB>(m1, j))));
+    *reinterpret_cast<uint4*>(out) = gn_pack<T>(xh);
   }
   if (p.cluster > 1) cluster_wait();
 }
@@ -415,9 +450,11 @@ __global__ void __launch_bounds__(kGnBackwardThreads, 2)
 
 static int gcd_int(int a, int b) { return b == 0 ? a : gcd_int(b, a % b); }
 
+static int gn_sub(const GnShape& s) { return s.Cg % 8 == 0 ? 8 : s.Cg % 4 == 0 ? 4 : 1; }
+
 static bool gn_resident_fill(const GnShape& s, GnPass pass, int slab, int cluster, int limit, GnResident* p) {
-  const int most = pass == GnPass::kForward ? kGnForwardThreads : kGnBackwardThreads;
-  const int bytes = pass == GnPass::kForward ? 16 : pass == GnPass::kBackward16 ? 32 : 24;
+  const int most = kGnThreads;
+  const int bytes = pass == GnPass::kForward ? 16 : pass == GnPass::kBackward16 ? 48 : 40;
   p->slab = slab;
   p->slabs = (s.C + slab - 1) / slab;
   p->lanes = (slab / 8 + 3) / 4 * 4;
@@ -430,9 +467,8 @@ static bool gn_resident_fill(const GnShape& s, GnPass pass, int slab, int cluste
   if (p->rl > p->rows_per_cta) p->rl = p->rows_per_cta;
   p->threads = (p->lanes * p->rl + 31) / 32 * 32;
   p->iters = (p->rows_per_cta + p->rl - 1) / p->rl;
-  const bool one = s.Cg % 8 == 0;
   const long long extra = pass == GnPass::kForward
-                              ? 8LL * (p->threads * (one ? 1 : 8) + 2 * (slab / s.Cg))
+                              ? 8LL * (p->threads * (8 / gn_sub(s)) + 2 * (slab / s.Cg))
                               : 8LL * (p->threads * 8 + 2 * slab + slab / s.Cg);
   const long long need = static_cast<long long>(p->iters) * p->threads * bytes + extra;
   if (need > limit) return false;
@@ -441,14 +477,14 @@ static bool gn_resident_fill(const GnShape& s, GnPass pass, int slab, int cluste
 }
 
 bool gn_resident_plan(const GnShape& s, GnPass pass, GnResident* p) {
-  constexpr int kTwo = 113 * 1024;  // two CTAs an SM: (228 KB - 2 x 1 KB) / 2
-  constexpr int kOne = 227 * 1024;
+  // shared memory of four, two and one CTAs an SM: 228 KB less 1 KB each
+  constexpr int kFour = 56 * 1024, kTwo = 113 * 1024, kOne = 227 * 1024;
   const long long unit_ll = static_cast<long long>(s.Cg) / gcd_int(s.Cg, kAct8Block) * kAct8Block;
   const int unit = unit_ll < s.C ? static_cast<int>(unit_ll) : s.C;
   // whole 128-byte lines of a pixel where that costs no occupancy
   int slab = unit;
   while (slab < 64 && slab < s.C) slab = slab + unit < s.C ? slab + unit : s.C;
-  for (int limit : {kTwo, kOne})
+  for (int limit : {kFour, kTwo, kOne})
     for (int width : {slab, unit})
       for (int cluster = 1; cluster <= 16; cluster *= 2)
         if (gn_resident_fill(s, pass, width, cluster, limit, p)) {
@@ -475,31 +511,39 @@ static int gn_resident_launch(const void* fn, const char* what, const GnShape& s
   return DWB_OK;
 }
 
-template <typename T, bool CKPT, bool ONE>
+template <typename T, bool CKPT, int SUB>
 static const void* resident_fn(int act) {
   switch (act) {
-    case kActRelu: return reinterpret_cast<const void*>(&gn_resident_kernel<T, kActRelu, CKPT, ONE>);
-    case kActGelu: return reinterpret_cast<const void*>(&gn_resident_kernel<T, kActGelu, CKPT, ONE>);
-    case kActSilu: return reinterpret_cast<const void*>(&gn_resident_kernel<T, kActSilu, CKPT, ONE>);
-    default: return reinterpret_cast<const void*>(&gn_resident_kernel<T, kActNone, CKPT, ONE>);
+    case kActRelu: return reinterpret_cast<const void*>(&gn_resident_kernel<T, kActRelu, CKPT, SUB>);
+    case kActGelu: return reinterpret_cast<const void*>(&gn_resident_kernel<T, kActGelu, CKPT, SUB>);
+    case kActSilu: return reinterpret_cast<const void*>(&gn_resident_kernel<T, kActSilu, CKPT, SUB>);
+    default: return reinterpret_cast<const void*>(&gn_resident_kernel<T, kActNone, CKPT, SUB>);
   }
 }
-template <typename T, bool SRC8, bool ONE>
+template <typename T, bool SRC8, int SUB>
 static const void* resident_grad_fn(int act) {
   switch (act) {
-    case kActRelu: return reinterpret_cast<const void*>(&gn_resident_grad_kernel<T, kActRelu, SRC8, ONE>);
-    case kActGelu: return reinterpret_cast<const void*>(&gn_resident_grad_kernel<T, kActGelu, SRC8, ONE>);
-    case kActSilu: return reinterpret_cast<const void*>(&gn_resident_grad_kernel<T, kActSilu, SRC8, ONE>);
-    default: return reinterpret_cast<const void*>(&gn_resident_grad_kernel<T, kActNone, SRC8, ONE>);
+    case kActRelu: return reinterpret_cast<const void*>(&gn_resident_grad_kernel<T, kActRelu, SRC8, SUB>);
+    case kActGelu: return reinterpret_cast<const void*>(&gn_resident_grad_kernel<T, kActGelu, SRC8, SUB>);
+    case kActSilu: return reinterpret_cast<const void*>(&gn_resident_grad_kernel<T, kActSilu, SRC8, SUB>);
+    default: return reinterpret_cast<const void*>(&gn_resident_grad_kernel<T, kActNone, SRC8, SUB>);
   }
+}
+template <typename T, bool CKPT>
+static const void* resident_fn(int sub, int act) {
+  return sub == 8 ? resident_fn<T, CKPT, 8>(act) : sub == 4 ? resident_fn<T, CKPT, 4>(act) : resident_fn<T, CKPT, 1>(act);
+}
+template <typename T, bool SRC8>
+static const void* resident_grad_fn(int sub, int act) {
+  return sub == 8   ? resident_grad_fn<T, SRC8, 8>(act)
+         : sub == 4 ? resident_grad_fn<T, SRC8, 4>(act)
+                    : resident_grad_fn<T, SRC8, 1>(act);
 }
 
 template <typename T>
 int gn_resident_forward(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd, void* codes,
                         void* scales, const GnShape& s, const GnResident& p, int act, cudaStream_t stream) {
-  const bool one = s.Cg % 8 == 0;
-  const void* fn = codes ? (one ? resident_fn<T, true, true>(act) : resident_fn<T, true, false>(act))
-                         : (one ? resident_fn<T, false, true>(act) : resident_fn<T, false, false>(act));
+  const void* fn = codes ? resident_fn<T, true>(gn_sub(s), act) : resident_fn<T, false>(gn_sub(s), act);
   GnShape sv = s;
   GnResident pv = p;
   void* args[] = {&x, &weight, &bias, &y, &mean, &rstd, &codes, &scales, &sv, &pv};
@@ -510,9 +554,7 @@ template <typename T>
 int gn_resident_backward(const void* dy, const void* x, const void* codes, const void* scales, const float* mean,
                          const float* rstd, const void* weight, const void* bias, void* dx, float2* sums, const GnShape& s,
                          const GnResident& p, int act, cudaStream_t stream) {
-  const bool one = s.Cg % 8 == 0;
-  const void* fn = codes ? (one ? resident_grad_fn<T, true, true>(act) : resident_grad_fn<T, true, false>(act))
-                         : (one ? resident_grad_fn<T, false, true>(act) : resident_grad_fn<T, false, false>(act));
+  const void* fn = codes ? resident_grad_fn<T, true>(gn_sub(s), act) : resident_grad_fn<T, false>(gn_sub(s), act);
   const void* src = codes ? codes : x;
   GnShape sv = s;
   GnResident pv = p;
