@@ -75,10 +75,14 @@ __global__ void __launch_bounds__(kGnThreads) gn_stats_kernel(const uint4* __res
             sums.add(f);
           }
       }
-      float mean[8], m2[8];
+      f32x2 mean[4], m2[4];
       sums.moments(n, mean, m2);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ent[threadIdx.x * 8 + i] = make_float2(mean[i], m2[i]);
+      for (int i = 0; i < 4; ++i) {
+        const float2 a = bits_f2(mean[i]), q = bits_f2(m2[i]);
+        ent[threadIdx.x * 8 + 2 * i] = make_float2(a.x, q.x);
+        ent[threadIdx.x * 8 + 2 * i + 1] = make_float2(a.y, q.y);
+      }
     }
   }
   __syncthreads();
@@ -152,7 +156,7 @@ __global__ void __launch_bounds__(kGnThreads) gn_apply_kernel(const uint4* __res
   const long long step = s.C / 8, sblocks = (s.C + kAct8Block - 1) / kAct8Block;
   f32x2 w[4], b[4], m[4], rs[4];
   if (th.active) {
-    gn_load_params<T>(weight, bias, th.c, s.param_f32, w, b);
+    gn_load_params<T>(weight, bias, th.c, s, w, b);
     gn_load_stats(mean, rstd, th.sample, th.c, s, m, rs);
   }
   // the trip count is the same for the whole CTA: the block maxima are warp shuffles
@@ -216,7 +220,7 @@ __global__ void __launch_bounds__(kGnThreads) gn_grad_sums_kernel(const uint4* _
   const int width = p.lanes * 8;
   if (th.active) {
     f32x2 w[4], b[4], m[4], rs[4], sg[4], sx[4];
-    gn_load_params<T>(weight, bias, th.c, s.param_f32, w, b);
+    gn_load_params<T>(weight, bias, th.c, s, w, b);
     gn_load_stats(mean, rstd, th.sample, th.c, s, m, rs);
 #pragma unroll
     for (int i = 0; i < 4; ++i) sg[i] = sx[i] = f32x2_zero();
@@ -296,7 +300,7 @@ __global__ void __launch_bounds__(kGnThreads) gn_grad_apply_kernel(const uint4* 
   const GnThread th(s, p);
   if (!th.active) return;
   f32x2 w[4], b[4], m[4], rs[4], m1[4], m2[4];
-  gn_load_params<T>(weight, bias, th.c, s.param_f32, w, b);
+  gn_load_params<T>(weight, bias, th.c, s, w, b);
   gn_load_stats(mean, rstd, th.sample, th.c, s, m, rs);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -394,6 +398,7 @@ static int gn_shape(int64_t B, int64_t H, int64_t W, int64_t C, int G, double ep
   s->Cg = static_cast<int>(C / G);
   s->eps = static_cast<float>(eps);
   s->param_f32 = param_dtype == DWB_F32;
+  s->param_vec = 0;
   return DWB_OK;
 }
 
@@ -529,6 +534,7 @@ extern "C" int dwb_group_norm_act_nhwc_fwd(const void* x, const void* weight, co
     return DWB_ERR_BAD_ALIGN;
   rc = require_device();
   if (rc != DWB_OK) return rc;
+  s.param_vec = is_aligned(weight, 16) && is_aligned(bias, 16);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == DWB_F16 ? gn_forward<__half>(x, weight, bias, y, mean, rstd, codes, scales, workspace, s, act, st)
                           : gn_forward<__nv_bfloat16>(x, weight, bias, y, mean, rstd, codes, scales, workspace, s, act, st);
@@ -566,6 +572,7 @@ extern "C" int dwb_group_norm_act_nhwc_bwd(const void* dy, const void* x, const 
     if (e == cudaSuccess && dbias) e = cudaMemsetAsync(dbias, 0, n, st);
     return e == cudaSuccess ? DWB_OK : record_cuda_failure("cudaMemsetAsync(dweight, dbias)", e);
   }
+  s.param_vec = is_aligned(weight, 16) && is_aligned(bias, 16);
   return dtype == DWB_F16 ? gn_backward<__half>(dy, x, codes, scales, mean, rstd, weight, bias, dx, dweight, dbias, workspace,
                                                 s, act, st)
                           : gn_backward<__nv_bfloat16>(dy, x, codes, scales, mean, rstd, weight, bias, dx, dweight, dbias,

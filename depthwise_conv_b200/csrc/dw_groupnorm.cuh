@@ -27,14 +27,14 @@ namespace dwb {
 enum : int { kActSilu = 3 };  // after kActNone, kActRelu, kActGelu
 
 // erfc(a / sqrt 2) / 2 = exp(-a^2 / 2) * poly(t) t for a = |u|, t = 1 / (1 + p a): Abramowitz & Stegun
-// 7.1.26 (|error| <= 1.5e-7), as gelu_erf2 uses it.  Returns poly(t), t and the exponential.
+// 7.1.26 (|error| <= 1.5e-7), as gelu_erf2 uses it.  Returns -a, poly(t), t and the exponential.
 struct HalfErfc {
-  f32x2 a, poly, t, e;
+  f32x2 na, poly, t, e;
 };
 __device__ __forceinline__ HalfErfc half_erfc2(f32x2 u) {
   HalfErfc r;
-  r.a = u & 0x7fffffff7fffffffull;
-  const float2 d = bits_f2(fma2(r.a, splat2(0.3275911f * 0.70710678118654752f), splat2(1.0f)));
+  r.na = u | 0x8000000080000000ull;
+  const float2 d = bits_f2(fma2(r.na, splat2(-0.3275911f * 0.70710678118654752f), splat2(1.0f)));
   r.t = f2_bits(make_float2(rcp_approx(d.x), rcp_approx(d.y)));
   f32x2 q = fma2(splat2(0.5f * 1.061405429f), r.t, splat2(0.5f * -1.453152027f));
   q = fma2(q, r.t, splat2(0.5f * 1.421413741f));
@@ -55,7 +55,7 @@ __device__ __forceinline__ f32x2 act_value2(f32x2 u) {
     const HalfErfc h = half_erfc2(u);
     const float2 f = bits_f2(u);
     const f32x2 lost = fmul2(fmul2(h.poly, h.t), h.e);
-    return fma2(fmul2(h.a, splat2(-1.0f)), lost, f2_bits(make_float2(fmaxf(f.x, 0.0f), fmaxf(f.y, 0.0f))));
+    return fma2(h.na, lost, f2_bits(make_float2(fmaxf(f.x, 0.0f), fmaxf(f.y, 0.0f))));
   } else if constexpr (ACT == kActSilu) {
     const float2 e = bits_f2(fmul2(u, splat2(-1.4426950408889634f)));
     const f32x2 d = fma2(f2_bits(make_float2(ex2_approx(e.x), ex2_approx(e.y))), splat2(1.0f), splat2(1.0f));
@@ -74,12 +74,11 @@ __device__ __forceinline__ f32x2 act_slope2(f32x2 u) {
     return f2_bits(make_float2(f.x > 0.0f ? 1.0f : 0.0f, f.y > 0.0f ? 1.0f : 0.0f));
   } else if constexpr (ACT == kActGelu) {
     // Phi(u) + u phi(u) with k = erfc(|u| / sqrt 2) / 2 - |u| phi(u) is k below 0 and 1 - k above:
-    // 1/2 + (1/2 - k) with the sign of u.  phi has the exponential that erfc has.
+    // 1/2 plus k - 1/2 with its sign turned where u is positive.  phi has the exponential that erfc has.
     const HalfErfc h = half_erfc2(u);
-    const f32x2 k = fma2(h.poly, h.t, fmul2(h.a, splat2(-0.3989422804014327f)));
-    const f32x2 d = fma2(fmul2(k, splat2(-1.0f)), h.e, splat2(0.5f));
+    const f32x2 k = fma2(h.poly, h.t, fmul2(h.na, splat2(0.3989422804014327f)));
     f32x2 r = splat2(0.5f);
-    fadd2(r, d ^ (u & 0x8000000080000000ull));
+    fadd2(r, fma2(k, h.e, splat2(-0.5f)) ^ (~u & 0x8000000080000000ull));
     return r;
   } else if constexpr (ACT == kActSilu) {
     const float2 e = bits_f2(fmul2(u, splat2(-1.4426950408889634f)));
@@ -100,6 +99,7 @@ struct GnShape {
   int B, C, G, Cg;
   float eps;
   int param_f32;   // weight and bias: fp32 instead of the tensor's type
+  int param_vec;   // both on 16-byte boundaries (or absent)
 };
 
 // Weight or bias of channel c (`otherwise` where the vector is absent).
@@ -110,21 +110,41 @@ __device__ __forceinline__ float gn_param(const void* p, int c, int f32, float o
 }
 
 template <typename T>
-__device__ __forceinline__ void gn_load_params(const void* weight, const void* bias, int c, int f32, f32x2 (&w)[4],
-                                               f32x2 (&b)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    w[i] = f2_bits(make_float2(gn_param<T>(weight, c + 2 * i, f32, 1.0f), gn_param<T>(weight, c + 2 * i + 1, f32, 1.0f)));
-    b[i] = f2_bits(make_float2(gn_param<T>(bias, c + 2 * i, f32, 0.0f), gn_param<T>(bias, c + 2 * i + 1, f32, 0.0f)));
-  }
-}
-
-template <typename T>
 __device__ __forceinline__ void gn_unpack(const uint4& v, f32x2 (&f)[4]) {
   f[0] = Type16<T>::to_f32x2(v.x);
   f[1] = Type16<T>::to_f32x2(v.y);
   f[2] = Type16<T>::to_f32x2(v.z);
   f[3] = Type16<T>::to_f32x2(v.w);
+}
+
+// 8 channels of a parameter vector.
+template <typename T>
+__device__ __forceinline__ void gn_load_param8(const void* p, int c, const GnShape& s, float otherwise, f32x2 (&v)[4]) {
+  if (!p) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = splat2(otherwise);
+  } else if (s.param_vec && s.param_f32) {
+    const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(static_cast<const float*>(p) + c);
+    const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(static_cast<const float*>(p) + c + 4);
+    v[0] = a.x;
+    v[1] = a.y;
+    v[2] = b.x;
+    v[3] = b.y;
+  } else if (s.param_vec) {
+    gn_unpack<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(p) + c), v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = f2_bits(make_float2(gn_param<T>(p, c + 2 * i, s.param_f32, otherwise),
+                                 gn_param<T>(p, c + 2 * i + 1, s.param_f32, otherwise)));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void gn_load_params(const void* weight, const void* bias, int c, const GnShape& s, f32x2 (&w)[4],
+                                               f32x2 (&b)[4]) {
+  gn_load_param8<T>(weight, c, s, 1.0f, w);
+  gn_load_param8<T>(bias, c, s, 0.0f, b);
 }
 
 template <typename T>
@@ -154,18 +174,16 @@ struct GnSums {
     }
   }
   // per-channel mean and sum of squared deviations of the n >= 1 values seen
-  __device__ __forceinline__ void moments(int n, float (&mean)[8], float (&m2)[8]) const {
-    const float inv = 1.0f / static_cast<float>(n);
+  __device__ __forceinline__ void moments(int n, f32x2 (&mean)[4], f32x2 (&m2)[4]) const {
+    const f32x2 inv = splat2(rcp_approx(static_cast<float>(n)));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 kf = bits_f2(k[i]), a = bits_f2(s1[i]), q = bits_f2(s2[i]);
-      const float dx = a.x * inv, dy = a.y * inv;
-      mean[2 * i] = kf.x + dx;
-      mean[2 * i + 1] = kf.y + dy;
-      // a difference that rounding may leave below zero; NaN stays NaN
-      const float qx = q.x - a.x * dx, qy = q.y - a.y * dy;
-      m2[2 * i] = qx < 0.0f ? 0.0f : qx;
-      m2[2 * i + 1] = qy < 0.0f ? 0.0f : qy;
+      const f32x2 d = fmul2(s1[i], inv);
+      mean[i] = k[i];
+      fadd2(mean[i], d);
+      // a difference that rounding may leave below zero; a NaN or an infinity is in the mean as well
+      const float2 q = bits_f2(fsub2(s2[i], fmul2(s1[i], d)));
+      m2[i] = f2_bits(make_float2(fmaxf(q.x, 0.0f), fmaxf(q.y, 0.0f)));
     }
   }
 };

@@ -45,6 +45,11 @@ __device__ __forceinline__ void cluster_arrive() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
+// For a barrier that orders nothing but the end of this CTA's reads.
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_wait() {
   __syncwarp();
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -63,24 +68,22 @@ struct GnPlace {
   int rank, c_base, width;   // rank in the cluster; first channel; channels of this slab
   int lane_row, vec, c;
   bool active;
-  long long sample, r0;
-  int rows;                  // pixels of this CTA
+  int r0, rows;              // pixels of this CTA
+  long long sample;
   __device__ __forceinline__ GnPlace(const GnShape& s, const GnResident& p) {
-    const int cl = blockIdx.x / p.cluster;
-    rank = blockIdx.x - cl * p.cluster;
-    sample = cl / p.slabs;
-    c_base = (cl - static_cast<int>(sample) * p.slabs) * p.slab;
-    width = s.C - c_base < p.slab ? s.C - c_base : p.slab;
-    lane_row = threadIdx.x / p.lanes;
+    rank = blockIdx.x & (p.cluster - 1);
+    sample = blockIdx.y;
+    c_base = (blockIdx.x >> p.cluster_log) * p.slab;
+    width = min(s.C - c_base, p.slab);
+    lane_row = threadIdx.x * p.lane_mul >> 16;
     vec = threadIdx.x - lane_row * p.lanes;
     c = c_base + vec * 8;
     active = lane_row < p.rl && vec * 8 < width;
-    r0 = static_cast<long long>(rank) * p.rows_per_cta;
+    r0 = rank * p.rows_per_cta;
     rows = rows_of(s, p, rank);
   }
   static __device__ __forceinline__ int rows_of(const GnShape& s, const GnResident& p, int rank) {
-    const long long first = static_cast<long long>(rank) * p.rows_per_cta, left = s.P - first;
-    return left <= 0 ? 0 : left < p.rows_per_cta ? static_cast<int>(left) : p.rows_per_cta;
+    return max(0, min(p.rows_per_cta, static_cast<int>(s.P) - rank * p.rows_per_cta));
   }
 };
 
@@ -154,20 +157,34 @@ __global__ void __launch_bounds__(kGnThreads, kGnForwardCtas)
         sums.add(f);
       }
     }
-    float mean[8], m2[8];
+    f32x2 mean[4], m2[4];
     sums.moments(mine, mean, m2);
+    const float n = static_cast<float>(mine);
+    if constexpr (SUB == 1) {
 #pragma unroll
-    for (int e = 0; e < kEnt; ++e) {
-      float m = 0.0f, q = 0.0f, d2 = 0.0f;
-#pragma unroll
-      for (int k = 0; k < SUB; ++k) m += mean[e * SUB + k];
-      m *= 1.0f / SUB;
-#pragma unroll
-      for (int k = 0; k < SUB; ++k) {
-        q += m2[e * SUB + k];
-        d2 += (mean[e * SUB + k] - m) * (mean[e * SUB + k] - m);
+      for (int j = 0; j < 4; ++j) {
+        const float2 a = bits_f2(mean[j]), q = bits_f2(m2[j]);
+        *reinterpret_cast<float4*>(ent + tid * 8 + 2 * j) = make_float4(a.x, q.x, a.y, q.y);
       }
-      ent[tid * kEnt + e] = make_float2(m, q + static_cast<float>(mine) * d2);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kEnt; ++e) {
+        f32x2 sum = mean[e * SUB / 2], q = m2[e * SUB / 2], d2 = f32x2_zero();
+#pragma unroll
+        for (int j = 1; j < SUB / 2; ++j) {
+          fadd2(sum, mean[e * SUB / 2 + j]);
+          fadd2(q, m2[e * SUB / 2 + j]);
+        }
+        const float2 sf = bits_f2(sum), qf = bits_f2(q);
+        const float mid = (sf.x + sf.y) * (1.0f / SUB);
+#pragma unroll
+        for (int j = 0; j < SUB / 2; ++j) {
+          const f32x2 d = fsub2(mean[e * SUB / 2 + j], splat2(mid));
+          ffma2(d2, d, d);
+        }
+        const float2 df = bits_f2(d2);
+        ent[tid * kEnt + e] = make_float2(mid, qf.x + qf.y + n * (df.x + df.y));
+      }
     }
   }
   __syncthreads();
@@ -206,33 +223,32 @@ __global__ void __launch_bounds__(kGnThreads, kGnForwardCtas)
   } else {
     __syncthreads();
   }
-  for (int g = tid; g < here; g += nt) {
+  // a lane a rank: all of the cluster's moments of a group at once, added up the same way in every CTA
+  for (int g = tid >> 5; g < here; g += warps) {
     float mean = grp[g].x, m2 = grp[g].y;
     if (p.cluster > 1) {
-      float sum = 0.0f;
-      for (int r = 0; r < p.cluster; ++r)
-        sum += static_cast<float>(GnPlace::rows_of(s, p, r)) * cluster_load(grp + g, r).x;
-      mean = sum / static_cast<float>(s.P);
-      m2 = 0.0f;
-      for (int r = 0; r < p.cluster; ++r) {
-        const float2 v = cluster_load(grp + g, r);
-        m2 += v.y + static_cast<float>(GnPlace::rows_of(s, p, r)) * static_cast<float>(s.Cg) * (v.x - mean) * (v.x - mean);
-      }
+      const float n = lane < p.cluster ? static_cast<float>(GnPlace::rows_of(s, p, lane)) : 0.0f;
+      const float2 v = lane < p.cluster ? cluster_load(grp + g, lane) : make_float2(0.0f, 0.0f);
+      mean = warp_sum(n * v.x) / static_cast<float>(s.P);
+      // a CTA without pixels has a mean of 0 and a weight of 0
+      m2 = warp_sum(lane < p.cluster ? v.y + n * static_cast<float>(s.Cg) * (v.x - mean) * (v.x - mean) : 0.0f);
     }
     const float rstd = 1.0f / sqrtf(m2 / (static_cast<float>(s.P) * static_cast<float>(s.Cg)) + s.eps);
-    fin[g] = make_float2(mean, rstd);
-    if (at.rank == 0) {
-      const long long o = at.sample * s.G + at.c_base / s.Cg + g;
-      mean_out[o] = mean;
-      rstd_out[o] = rstd;
+    if (lane == 0) {
+      fin[g] = make_float2(mean, rstd);
+      if (at.rank == 0) {
+        const long long o = at.sample * s.G + at.c_base / s.Cg + g;
+        mean_out[o] = mean;
+        rstd_out[o] = rstd;
+      }
     }
   }
-  if (p.cluster > 1) cluster_arrive();  // this CTA has read the others' moments
+  if (p.cluster > 1) cluster_arrive_relaxed();  // this CTA has read the others' moments
   __syncthreads();
   f32x2 w[4], b[4], m[kParts];
   if (at.active) {
     f32x2 rs[kParts];
-    gn_load_params<T>(weight, bias, at.c, s.param_f32, w, b);
+    gn_load_params<T>(weight, bias, at.c, s, w, b);
     gn_read_groups<SUB>(fin, at.vec * 8, s.Cg, m, rs);
 #pragma unroll
     for (int j = 0; j < 4; ++j) w[j] = fmul2(w[j], gn_of<SUB>(rs, j));
@@ -320,7 +336,7 @@ __global__ void __launch_bounds__(kGnThreads, kGnBackwardCtas)
   }
   f32x2 w[4], b[4], m[kParts], rs[kParts];
   if (at.active) {
-    gn_load_params<T>(weight, bias, at.c, s.param_f32, w, b);
+    gn_load_params<T>(weight, bias, at.c, s, w, b);
 #pragma unroll
     for (int i = 0; i < kParts; ++i) {
       const int c = at.c + i * (SUB == 1 ? 2 : SUB);
@@ -394,6 +410,7 @@ __global__ void __launch_bounds__(kGnThreads, kGnBackwardCtas)
     float2 a = chan[j];
     if (p.cluster > 1) {
       a = make_float2(0.0f, 0.0f);
+#pragma unroll 4
       for (int r = 0; r < p.cluster; ++r) {
         const float2 e = cluster_load(chan + j, r);
         a.x += e.x;
@@ -404,7 +421,7 @@ __global__ void __launch_bounds__(kGnThreads, kGnBackwardCtas)
     const float wj = gn_param<T>(weight, at.c_base + j, s.param_f32, 1.0f);
     total[j] = make_float2(a.x * wj, a.y * wj);
   }
-  if (p.cluster > 1) cluster_arrive();
+  if (p.cluster > 1) cluster_arrive_relaxed();
   __syncthreads();
   const float inv = 1.0f / (static_cast<float>(s.P) * static_cast<float>(s.Cg));
   const int lane = tid & 31, warps = nt >> 5, here = at.width / s.Cg;
@@ -462,6 +479,9 @@ static bool gn_resident_fill(const GnShape& s, GnPass pass, int slab, int cluste
   const long long rows = (s.P + cluster - 1) / cluster;
   if (rows > (1 << 20)) return false;
   p->cluster = cluster;
+  p->cluster_log = 0;
+  while ((1 << p->cluster_log) < cluster) ++p->cluster_log;
+  p->lane_mul = 65536u / p->lanes + 1;  // exact for thread < 1024: the error of thread / lanes stays below 1 / 64
   p->rows_per_cta = static_cast<int>(rows);
   p->rl = most / p->lanes;
   if (p->rl > p->rows_per_cta) p->rl = p->rows_per_cta;
@@ -473,7 +493,7 @@ static bool gn_resident_fill(const GnShape& s, GnPass pass, int slab, int cluste
   const long long need = static_cast<long long>(p->iters) * p->threads * bytes + extra;
   if (need > limit) return false;
   p->smem = static_cast<int>(need);
-  return static_cast<long long>(s.B) * p->slabs * cluster <= 0x7fffffffLL;
+  return s.B <= 65535;  // grid y
 }
 
 bool gn_resident_plan(const GnShape& s, GnPass pass, GnResident* p) {
@@ -502,7 +522,7 @@ static int gn_resident_launch(const void* fn, const char* what, const GnShape& s
                               cudaStream_t stream) {
   cudaError_t e = allow_large_cta(fn);
   if (e == cudaSuccess)
-    e = launch_kernel(fn, dim3(static_cast<unsigned>(static_cast<long long>(s.B) * p.slabs * p.cluster)), dim3(p.threads), args,
+    e = launch_kernel(fn, dim3(static_cast<unsigned>(p.slabs * p.cluster), static_cast<unsigned>(s.B)), dim3(p.threads), args,
                       p.smem, stream, p.cluster);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();

@@ -16,7 +16,9 @@ struct GnResident {
   int lanes;         // threads along a pixel (a multiple of 4)
   int rl;            // pixels a CTA handles at once
   int threads;       // lanes * rl, rounded up to a warp
-  int cluster;       // CTAs that share the sample's pixels
+  unsigned lane_mul; // thread / lanes = thread * lane_mul >> 16
+  int cluster;       // CTAs that share the sample's pixels: 1 << cluster_log
+  int cluster_log;
   int rows_per_cta;
   int iters;         // pixels a thread handles
   int smem;
