@@ -120,19 +120,29 @@ __device__ __forceinline__ uint2 act8_codes(const uint4& v, uint32_t E) {
   return make_uint2(__byte_perm(b[0], b[1], 0x5410), __byte_perm(b[2], b[3], 0x5410));
 }
 
-// 8 codes as fp32 pairs times `step`.  Byte u = q + 128 under 0x4b000000 is the float 2^23 + u.
-__device__ __forceinline__ void act8_values(const uint2& q, float step, f32x2 (&out)[4]) {
+// 4 codes as fp32 pairs times `step`.  Byte u = q + 128 under 0x4b000000 is the float 2^23 + u.
+__device__ __forceinline__ void act8_values4(uint32_t q, float step, f32x2 (&out)[2]) {
   const f32x2 off = splat2(-8388736.0f);  // -(2^23 + 128)
   const f32x2 s = splat2(step);
+  const uint32_t w = q ^ 0x80808080u;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t w = (i < 2 ? q.x : q.y) ^ 0x80808080u;
-    const uint32_t lo = __byte_perm(w, 0x4b000000u, (i & 1) ? 0x7442 : 0x7440);
-    const uint32_t hi = __byte_perm(w, 0x4b000000u, (i & 1) ? 0x7443 : 0x7441);
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t lo = __byte_perm(w, 0x4b000000u, i ? 0x7442 : 0x7440);
+    const uint32_t hi = __byte_perm(w, 0x4b000000u, i ? 0x7443 : 0x7441);
     f32x2 f = (static_cast<unsigned long long>(hi) << 32) | lo;
     fadd2(f, off);
     out[i] = fmul2(f, s);
   }
+}
+
+__device__ __forceinline__ void act8_values(const uint2& q, float step, f32x2 (&out)[4]) {
+  f32x2 a[2], b[2];
+  act8_values4(q.x, step, a);
+  act8_values4(q.y, step, b);
+  out[0] = a[0];
+  out[1] = a[1];
+  out[2] = b[0];
+  out[3] = b[1];
 }
 
 }  // namespace dwb

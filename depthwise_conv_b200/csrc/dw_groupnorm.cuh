@@ -10,7 +10,7 @@
 //   m1 = sum_group(g weight) / n,  m2 = sum_group(g weight xh) / n,
 //   dx = rstd ((g weight - m1) - xh m2).
 //
-// Layout of the work in every kernel: a thread owns one 16-byte vector of 8
+// Layout of the work in every kernel: a thread owns one vector of 8 (or 4)
 // channels and walks over pixels, so that its parameters and its sums stay in
 // registers and every group structure (groups of 1, 3, 9 channels, groups that
 // end inside a vector) is a matter of how the per-channel sums are added up.
@@ -140,6 +140,27 @@ __device__ __forceinline__ void gn_load_param8(const void* p, int c, const GnSha
   }
 }
 
+// 4 channels of a parameter vector.
+template <typename T>
+__device__ __forceinline__ void gn_load_param4(const void* p, int c, const GnShape& s, float otherwise, f32x2 (&v)[2]) {
+  if (!p) {
+    v[0] = v[1] = splat2(otherwise);
+  } else if (s.param_vec && s.param_f32) {
+    const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(static_cast<const float*>(p) + c);
+    v[0] = a.x;
+    v[1] = a.y;
+  } else if (s.param_vec) {
+    const uint2 a = *reinterpret_cast<const uint2*>(static_cast<const T*>(p) + c);
+    v[0] = Type16<T>::to_f32x2(a.x);
+    v[1] = Type16<T>::to_f32x2(a.y);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      v[i] = f2_bits(make_float2(gn_param<T>(p, c + 2 * i, s.param_f32, otherwise),
+                                 gn_param<T>(p, c + 2 * i + 1, s.param_f32, otherwise)));
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ void gn_load_params(const void* weight, const void* bias, int c, const GnShape& s, f32x2 (&w)[4],
                                                f32x2 (&b)[4]) {
@@ -154,6 +175,9 @@ __device__ __forceinline__ uint4 gn_pack(const f32x2 (&f)[4]) {
 }
 
 __device__ __forceinline__ f32x2 fsub2(f32x2 a, f32x2 b) { return fma2(b, splat2(-1.0f), a); }
+
+// A sum of squares that rounding may leave below zero (a comparison, not fmaxf: NaN stays NaN).
+__device__ __forceinline__ float not_negative(float v) { return v < 0.0f ? 0.0f : v; }
 
 // Sums of one thread about its own first values.
 struct GnSums {
@@ -181,9 +205,8 @@ struct GnSums {
       const f32x2 d = fmul2(s1[i], inv);
       mean[i] = k[i];
       fadd2(mean[i], d);
-      // a difference that rounding may leave below zero; a NaN or an infinity is in the mean as well
       const float2 q = bits_f2(fsub2(s2[i], fmul2(s1[i], d)));
-      m2[i] = f2_bits(make_float2(fmaxf(q.x, 0.0f), fmaxf(q.y, 0.0f)));
+      m2[i] = f2_bits(make_float2(not_negative(q.x), not_negative(q.y)));
     }
   }
 };
@@ -192,6 +215,15 @@ __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
+}
+
+// Two sums at once: the shuffles of one hide those of the other.
+__device__ __forceinline__ void warp_sum2(float& a, float& b) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+    b += __shfl_xor_sync(0xffffffffu, b, o);
+  }
 }
 
 // Sum over the CTA (blockDim.x a multiple of 32, at most 1024); `scratch` holds 33 floats.
@@ -204,5 +236,105 @@ __device__ __forceinline__ float block_sum(float v, float* scratch) {
   for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) s += scratch[w];
   return s;
 }
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async8(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// SUB: channels of a vector that surely share a group (8, 4 or 1: C / G is a multiple of it).
+template <int SUB>
+__device__ __forceinline__ f32x2 gn_of(const f32x2 (&v)[SUB == 8 ? 1 : SUB == 4 ? 2 : 4], int pair) {
+  return v[SUB == 8 ? 0 : SUB == 4 ? pair / 2 : pair];
+}
+
+// The two halves of what `fin` holds for the groups (from `first_group` on) of the 8 channels from c on.
+template <int SUB>
+__device__ __forceinline__ void gn_read_groups(const float2* fin, int c, int Cg, int first_group,
+                                               f32x2 (&x)[SUB == 8 ? 1 : SUB == 4 ? 2 : 4],
+                                               f32x2 (&y)[SUB == 8 ? 1 : SUB == 4 ? 2 : 4]) {
+#pragma unroll
+  for (int i = 0; i < (SUB == 8 ? 1 : SUB == 4 ? 2 : 4); ++i) {
+    const int at = c + i * (SUB == 1 ? 2 : SUB);
+    const float2 lo = fin[at / Cg - first_group], hi = SUB == 1 ? fin[(at + 1) / Cg - first_group] : lo;
+    x[i] = f2_bits(make_float2(lo.x, hi.x));
+    y[i] = f2_bits(make_float2(lo.y, hi.y));
+  }
+}
+
+// A thread's moments (n pixels a channel) for the merge of its CTA: one entry for every SUB channels.
+template <int SUB>
+__device__ __forceinline__ void gn_hand_over(const f32x2 (&mean)[4], const f32x2 (&m2)[4], float n, float2* ent) {
+  if constexpr (SUB == 1) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 a = bits_f2(mean[j]), q = bits_f2(m2[j]);
+      *reinterpret_cast<float4*>(ent + 2 * j) = make_float4(a.x, q.x, a.y, q.y);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8 / SUB; ++e) {
+      f32x2 sum = mean[e * SUB / 2], q = m2[e * SUB / 2], d2 = f32x2_zero();
+#pragma unroll
+      for (int j = 1; j < SUB / 2; ++j) {
+        fadd2(sum, mean[e * SUB / 2 + j]);
+        fadd2(q, m2[e * SUB / 2 + j]);
+      }
+      const float2 sf = bits_f2(sum), qf = bits_f2(q);
+      const float mid = (sf.x + sf.y) * (1.0f / SUB);
+#pragma unroll
+      for (int j = 0; j < SUB / 2; ++j) {
+        const f32x2 d = fsub2(mean[e * SUB / 2 + j], splat2(mid));
+        ffma2(d2, d, d);
+      }
+      const float2 df = bits_f2(d2);
+      ent[e] = make_float2(mid, qf.x + qf.y + n * (df.x + df.y));
+    }
+  }
+}
+
+// A warp's merge of a segment's entries [lane row][per_row] in shared memory.  Lanes go along a lane row first.
+struct GnMerge {
+  int per_row, live, full, rest, row_words, k0, k_step, r0, r_step;
+  __device__ __forceinline__ GnMerge(int lane, int entries_per_row, int rows, int rl, int words) {
+    per_row = entries_per_row;
+    live = min(rows, rl);
+    full = rows / rl;
+    rest = rows - full * rl;  // lane rows below `rest` have a pixel more
+    row_words = words;
+    const bool fits = per_row <= 32;
+    k0 = fits ? lane % per_row : lane;
+    k_step = fits ? per_row : 32;
+    r_step = fits ? 32 / per_row : 1;
+    r0 = fits ? lane / per_row : 0;
+  }
+  // (mean, M2) over `rows` pixels of `channels`; (0, 0) without pixels.
+  template <int SUB>
+  __device__ __forceinline__ float2 run(const float2* first, int rows, int channels) const {
+    // about one thread's mean, which is a mean of its values already: nothing cancels in the last step
+    const float pivot = live ? first[0].x : 0.0f;
+    float s1 = 0.0f, s2 = 0.0f;
+    if (r0 < r_step)
+#pragma unroll 4
+      for (int r = r0; r < live; r += r_step) {
+        const float n = static_cast<float>((full + (r < rest)) * SUB);
+        for (int k = k0; k < per_row; k += k_step) {
+          const float2 v = first[r * row_words + k];
+          const float d = v.x - pivot;
+          s1 += n * d;
+          s2 += v.y + n * d * d;
+        }
+      }
+    warp_sum2(s1, s2);
+    if (!rows) return make_float2(0.0f, 0.0f);
+    const float d = s1 / (static_cast<float>(rows) * static_cast<float>(channels));
+    return make_float2(pivot + d, not_negative(s2 - s1 * d));
+  }
+};
 
 }  // namespace dwb

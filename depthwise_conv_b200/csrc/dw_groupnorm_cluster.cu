@@ -5,10 +5,10 @@
 //
 // Bound by memory: forward 4 bytes a value (5.03 with a checkpoint), backward 6
 // (5.03 from a checkpoint).  Every thread copies its own vectors to shared
-// memory (cp.async, 16 bytes; 8 for codes) and is the only one that reads them,
-// so the copies need no barrier: all of a CTA's loads are in flight at once, and
-// the sums begin when the first quarter has landed.  Two CTAs an SM (110 KB
-// each) let one load while the other computes or stores.  The moments (forward)
+// memory (cp.async) and is the only one that reads them, so the copies need no
+// barrier: all of a CTA's loads are in flight at once, and the sums begin when
+// the first quarter has landed.  Four CTAs an SM let one load while another
+// computes or stores.  The moments (forward)
 // or the channel sums (backward) of the cluster's CTAs are exchanged through
 // distributed shared memory, and every CTA adds them up in rank order: the same
 // bits in every CTA and on every run.
@@ -23,15 +23,7 @@
 namespace dwb {
 
 constexpr int kGnThreads = 256;
-constexpr int kGnForwardCtas = 4, kGnBackwardCtas = 2;  // CTAs an SM that the registers have to allow
 
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async8(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Wait until all but the `3 - part` newest of four groups have landed.
 __device__ __forceinline__ void cp_async_wait_part(int part) {
   if (part == 0) asm volatile("cp.async.wait_group 3;" ::: "memory");
@@ -70,15 +62,15 @@ struct GnPlace {
   bool active;
   int r0, rows;              // pixels of this CTA
   long long sample;
-  __device__ __forceinline__ GnPlace(const GnShape& s, const GnResident& p) {
+  __device__ __forceinline__ GnPlace(const GnShape& s, const GnResident& p, int channels) {  // of a thread
     rank = blockIdx.x & (p.cluster - 1);
     sample = blockIdx.y;
     c_base = (blockIdx.x >> p.cluster_log) * p.slab;
     width = min(s.C - c_base, p.slab);
     lane_row = threadIdx.x * p.lane_mul >> 16;
     vec = threadIdx.x - lane_row * p.lanes;
-    c = c_base + vec * 8;
-    active = lane_row < p.rl && vec * 8 < width;
+    c = c_base + vec * channels;
+    active = lane_row < p.rl && vec * channels < width;
     r0 = rank * p.rows_per_cta;
     rows = rows_of(s, p, rank);
   }
@@ -90,27 +82,8 @@ struct GnPlace {
 // Pixels of a CTA that lane row `lr` handles.
 __device__ __forceinline__ int gn_lane_rows(int rows, int lr, int rl) { return rows > lr ? (rows - lr + rl - 1) / rl : 0; }
 
-// SUB: channels of a vector that surely share a group (8, 4 or 1: C / G is a multiple of it).
-template <int SUB>
-__device__ __forceinline__ f32x2 gn_of(const f32x2 (&v)[SUB == 8 ? 1 : SUB == 4 ? 2 : 4], int pair) {
-  return v[SUB == 8 ? 0 : SUB == 4 ? pair / 2 : pair];
-}
-
-// The two halves of what the groups of a thread's channels hold in `fin`.
-template <int SUB>
-__device__ __forceinline__ void gn_read_groups(const float2* fin, int first, int Cg, f32x2 (&x)[SUB == 8 ? 1 : SUB == 4 ? 2 : 4],
-                                               f32x2 (&y)[SUB == 8 ? 1 : SUB == 4 ? 2 : 4]) {
-#pragma unroll
-  for (int i = 0; i < (SUB == 8 ? 1 : SUB == 4 ? 2 : 4); ++i) {
-    const int c = first + i * (SUB == 1 ? 2 : SUB);
-    const float2 lo = fin[c / Cg], hi = SUB == 1 ? fin[(c + 1) / Cg] : lo;
-    x[i] = f2_bits(make_float2(lo.x, hi.x));
-    y[i] = f2_bits(make_float2(lo.y, hi.y));
-  }
-}
-
 template <typename T, int ACT, bool CKPT, int SUB>
-__global__ void __launch_bounds__(kGnThreads, kGnForwardCtas)
+__global__ void __launch_bounds__(kGnThreads, 4)
     gn_resident_kernel(const T* __restrict__ x, const void* __restrict__ weight, const void* __restrict__ bias,
                        T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
                        int8_t* __restrict__ codes, uint8_t* __restrict__ scales, const GnShape s, const GnResident p) {
@@ -123,7 +96,7 @@ __global__ void __launch_bounds__(kGnThreads, kGnForwardCtas)
   float2* fin = grp + p.slab / s.Cg;
   griddep_wait();
   griddep_launch_dependents();
-  const GnPlace at(s, p);
+  const GnPlace at(s, p, 8);
   const int tid = threadIdx.x, nt = p.threads;
   const long long first = (at.sample * s.P + at.r0 + at.lane_row) * s.C + at.c;  // this thread's first value
   const long long step = static_cast<long long>(p.rl) * s.C;
@@ -139,6 +112,9 @@ __global__ void __launch_bounds__(kGnThreads, kGnForwardCtas)
       cp_async_commit();
     }
   }
+  // the parameters come in while the pixels do
+  f32x2 w[4], b[4];
+  if (at.active) gn_load_params<T>(weight, bias, at.c, s, w, b);
   if (mine) {
     GnSums sums;
     f32x2 f[4];
@@ -159,62 +135,16 @@ __global__ void __launch_bounds__(kGnThreads, kGnForwardCtas)
     }
     f32x2 mean[4], m2[4];
     sums.moments(mine, mean, m2);
-    const float n = static_cast<float>(mine);
-    if constexpr (SUB == 1) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 a = bits_f2(mean[j]), q = bits_f2(m2[j]);
-        *reinterpret_cast<float4*>(ent + tid * 8 + 2 * j) = make_float4(a.x, q.x, a.y, q.y);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < kEnt; ++e) {
-        f32x2 sum = mean[e * SUB / 2], q = m2[e * SUB / 2], d2 = f32x2_zero();
-#pragma unroll
-        for (int j = 1; j < SUB / 2; ++j) {
-          fadd2(sum, mean[e * SUB / 2 + j]);
-          fadd2(q, m2[e * SUB / 2 + j]);
-        }
-        const float2 sf = bits_f2(sum), qf = bits_f2(q);
-        const float mid = (sf.x + sf.y) * (1.0f / SUB);
-#pragma unroll
-        for (int j = 0; j < SUB / 2; ++j) {
-          const f32x2 d = fsub2(mean[e * SUB / 2 + j], splat2(mid));
-          ffma2(d2, d, d);
-        }
-        const float2 df = bits_f2(d2);
-        ent[tid * kEnt + e] = make_float2(mid, qf.x + qf.y + n * (df.x + df.y));
-      }
-    }
+    gn_hand_over<SUB>(mean, m2, static_cast<float>(mine), ent + tid * kEnt);
   }
   __syncthreads();
-  // one warp a group: the moments of this CTA's pixels.  Lanes go along the group's entries of a pixel first.
+  // one warp a group: the moments of this CTA's pixels
   const int lane = tid & 31, warps = nt >> 5, here = at.width / s.Cg;
   {
-    const int per_row = s.Cg / SUB, live = min(at.rows, p.rl);
-    const int turns = at.rows / p.rl, rest = at.rows - turns * p.rl;  // lane rows below `rest` have a pixel more
-    const bool fits = per_row <= 32;
-    const int k0 = fits ? lane % per_row : lane, k_step = fits ? per_row : 32;
-    const int r_step = fits ? 32 / per_row : 1, r0 = fits ? lane / per_row : 0;
+    const GnMerge merge(lane, s.Cg / SUB, at.rows, p.rl, p.lanes * kEnt);
     for (int g = tid >> 5; g < here; g += warps) {
-      const float2* of_group = ent + g * per_row;
-      float sum = 0.0f, m2 = 0.0f;
-      if (r0 < r_step)
-        for (int r = r0; r < live; r += r_step) {
-          const float n = static_cast<float>((turns + (r < rest)) * SUB);
-          for (int k = k0; k < per_row; k += k_step) sum += n * of_group[r * p.lanes * kEnt + k].x;
-        }
-      const float mean = at.rows ? warp_sum(sum) / (static_cast<float>(at.rows) * static_cast<float>(s.Cg)) : 0.0f;
-      if (r0 < r_step)
-        for (int r = r0; r < live; r += r_step) {
-          const float n = static_cast<float>((turns + (r < rest)) * SUB);
-          for (int k = k0; k < per_row; k += k_step) {
-            const float2 v = of_group[r * p.lanes * kEnt + k];
-            m2 += v.y + n * (v.x - mean) * (v.x - mean);
-          }
-        }
-      m2 = warp_sum(m2);
-      if (lane == 0) grp[g] = make_float2(mean, m2);
+      const float2 m = merge.run<SUB>(ent + g * (s.Cg / SUB), at.rows, s.Cg);
+      if (lane == 0) grp[g] = m;
     }
   }
   if (p.cluster > 1) {
@@ -227,11 +157,16 @@ __global__ void __launch_bounds__(kGnThreads, kGnForwardCtas)
   for (int g = tid >> 5; g < here; g += warps) {
     float mean = grp[g].x, m2 = grp[g].y;
     if (p.cluster > 1) {
-      const float n = lane < p.cluster ? static_cast<float>(GnPlace::rows_of(s, p, lane)) : 0.0f;
+      // about rank 0's mean (rank 0 always has pixels)
+      const float n = lane < p.cluster ? static_cast<float>(GnPlace::rows_of(s, p, lane)) * static_cast<float>(s.Cg) : 0.0f;
       const float2 v = lane < p.cluster ? cluster_load(grp + g, lane) : make_float2(0.0f, 0.0f);
-      mean = warp_sum(n * v.x) / static_cast<float>(s.P);
-      // a CTA without pixels has a mean of 0 and a weight of 0
-      m2 = warp_sum(lane < p.cluster ? v.y + n * static_cast<float>(s.Cg) * (v.x - mean) * (v.x - mean) : 0.0f);
+      const float pivot = __shfl_sync(0xffffffffu, v.x, 0), d = v.x - pivot;
+      // a CTA without pixels has no weight
+      float s1 = n > 0.0f ? n * d : 0.0f, s2 = n > 0.0f ? v.y + n * d * d : 0.0f;
+      warp_sum2(s1, s2);
+      const float off = s1 / (static_cast<float>(s.P) * static_cast<float>(s.Cg));
+      mean = pivot + off;
+      m2 = not_negative(s2 - s1 * off);
     }
     const float rstd = 1.0f / sqrtf(m2 / (static_cast<float>(s.P) * static_cast<float>(s.Cg)) + s.eps);
     if (lane == 0) {
@@ -245,11 +180,10 @@ __global__ void __launch_bounds__(kGnThreads, kGnForwardCtas)
   }
   if (p.cluster > 1) cluster_arrive_relaxed();  // this CTA has read the others' moments
   __syncthreads();
-  f32x2 w[4], b[4], m[kParts];
+  f32x2 m[kParts];
   if (at.active) {
     f32x2 rs[kParts];
-    gn_load_params<T>(weight, bias, at.c, s, w, b);
-    gn_read_groups<SUB>(fin, at.vec * 8, s.Cg, m, rs);
+    gn_read_groups<SUB>(fin, at.vec * 8, s.Cg, 0, m, rs);
 #pragma unroll
     for (int j = 0; j < 4; ++j) w[j] = fmul2(w[j], gn_of<SUB>(rs, j));
   }
@@ -290,28 +224,29 @@ __global__ void __launch_bounds__(kGnThreads, kGnForwardCtas)
   if (p.cluster > 1) cluster_wait();  // nobody reads this CTA's shared memory any more
 }
 
-// The slope of the activation costs most of the arithmetic, so g = dy act'(u) is computed once and kept in fp32
-// where dy lay (dy lands in the second half of g's place) for the second use.
+// A thread owns 4 channels here (8 bytes of dy): with its sums and parameters it stays within 64 registers, so that
+// four CTAs share an SM.  The slope of the activation costs most of the arithmetic, so g = dy act'(u) is computed
+// once and kept in fp32 where dy lay (dy lands in the second half of g's place) for the second use.
+// SUB: 4 where C / G is a multiple of 4 (a thread's channels share a group), else 1.
 template <typename T, int ACT, bool SRC8, int SUB>
-__global__ void __launch_bounds__(kGnThreads, kGnBackwardCtas)
+__global__ void __launch_bounds__(kGnThreads, 4)
     gn_resident_grad_kernel(const T* __restrict__ dy, const void* __restrict__ src, const uint8_t* __restrict__ scales,
                             const void* __restrict__ weight, const void* __restrict__ bias, const float* __restrict__ mean,
                             const float* __restrict__ rstd, T* __restrict__ dx, float2* __restrict__ sums_out,
                             const GnShape s, const GnResident p) {
   extern __shared__ __align__(16) unsigned char smem[];
-  constexpr int kParts = SUB == 8 ? 1 : SUB == 4 ? 2 : 4;
-  constexpr int kSaved = SRC8 ? 8 : 16;
+  constexpr int kParts = SUB == 4 ? 1 : 2;
+  constexpr int kSaved = SRC8 ? 4 : 8;
   const int nt = p.threads, tid = threadIdx.x;
-  uint4* g_lo = reinterpret_cast<uint4*>(smem);   // [iters][threads] g of channels 0..3
-  uint4* g_hi = g_lo + p.iters * nt;              // [iters][threads] dy, then g of channels 4..7
-  unsigned char* saved = reinterpret_cast<unsigned char*>(g_hi + p.iters * nt);
-  float2* ent = reinterpret_cast<float2*>(saved + p.iters * nt * kSaved);
-  float2* chan = ent + nt * 8;
-  float2* total = chan + p.slab;
-  float2* fin = total + p.slab;
+  uint4* const gs = reinterpret_cast<uint4*>(smem) + tid;  // [iters][threads] g of 4 channels; dy in the second half
+  unsigned char* const saved = smem + 16 * p.iters * nt + tid * kSaved;
+  float2* const ent = reinterpret_cast<float2*>(smem + (16 + kSaved) * p.iters * nt);
+  float2* const chan = ent + nt * 4;
+  float2* const total = chan + p.slab;
+  float2* const fin = total + p.slab;
   griddep_wait();
   griddep_launch_dependents();
-  const GnPlace at(s, p);
+  const GnPlace at(s, p, 4);
   const long long pixel0 = at.sample * s.P + at.r0 + at.lane_row;
   const long long first = pixel0 * s.C + at.c;
   const long long step = static_cast<long long>(p.rl) * s.C;
@@ -321,80 +256,87 @@ __global__ void __launch_bounds__(kGnThreads, kGnBackwardCtas)
   {
     const T* a = dy + first;
     const unsigned char* q = static_cast<const unsigned char*>(src) + first * (SRC8 ? 1 : 2);
-    uint4* da = g_hi + tid;
-    unsigned char* dq = saved + tid * kSaved;
+    unsigned char* da = reinterpret_cast<unsigned char*>(gs) + 8;
+    unsigned char* dq = saved;
     for (int part = 0; part < 4; ++part) {
       const int end = min(mine, (part + 1) * quarter);
-#pragma unroll 2
-      for (int i = part * quarter; i < end; ++i, a += step, q += step * (SRC8 ? 1 : 2), da += nt, dq += nt * kSaved) {
-        cp_async16(da, a);
-        if constexpr (SRC8) cp_async8(dq, q);
-        else cp_async16(dq, q);
+#pragma unroll 4
+      for (int i = part * quarter; i < end; ++i, a += step, q += step * (SRC8 ? 1 : 2), da += nt * 16, dq += nt * kSaved) {
+        cp_async8(da, a);
+        if constexpr (SRC8) cp_async4(dq, q);
+        else cp_async8(dq, q);
       }
       cp_async_commit();
     }
   }
-  f32x2 w[4], b[4], m[kParts], rs[kParts];
-  if (at.active) {
-    gn_load_params<T>(weight, bias, at.c, s, w, b);
-#pragma unroll
-    for (int i = 0; i < kParts; ++i) {
-      const int c = at.c + i * (SUB == 1 ? 2 : SUB);
-      const long long lo = at.sample * s.G + c / s.Cg, hi = SUB == 1 ? at.sample * s.G + (c + 1) / s.Cg : lo;
-      m[i] = f2_bits(make_float2(mean[lo], mean[hi]));
-      rs[i] = f2_bits(make_float2(rstd[lo], rstd[hi]));
-    }
-  }
+  f32x2 w[2], m[kParts], rs[kParts];
   const uint8_t* const sp0 = SRC8 ? scales + pixel0 * sblocks + at.c / kAct8Block : nullptr;
   const long long sstep = p.rl * sblocks;
-  auto x_hat = [&](const unsigned char* at_saved, uint32_t E, f32x2(&xh)[4]) {
-    if constexpr (SRC8) act8_values(*reinterpret_cast<const uint2*>(at_saved), act8_step(E), xh);
-    else gn_unpack<T>(*reinterpret_cast<const uint4*>(at_saved), xh);
+  auto x_hat = [&](const unsigned char* place, uint32_t E, f32x2(&xh)[2]) {
+    if constexpr (SRC8) {
+      act8_values4(*reinterpret_cast<const uint32_t*>(place), act8_step(E), xh);
+    } else {
+      const uint2 v = *reinterpret_cast<const uint2*>(place);
+      xh[0] = Type16<T>::to_f32x2(v.x);
+      xh[1] = Type16<T>::to_f32x2(v.y);
+    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) xh[j] = fmul2(fsub2(xh[j], gn_of<SUB>(m, j)), gn_of<SUB>(rs, j));
+    for (int j = 0; j < 2; ++j) xh[j] = fmul2(fsub2(xh[j], m[SUB == 4 ? 0 : j]), rs[SUB == 4 ? 0 : j]);
   };
   {
-    f32x2 sg[4], sx[4];
+    f32x2 b[2], sg[2], sx[2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sg[j] = sx[j] = f32x2_zero();
-    const unsigned char* q = saved + tid * kSaved;
-    uint4 *lo = g_lo + tid, *hi = g_hi + tid;
+    for (int j = 0; j < 2; ++j) sg[j] = sx[j] = f32x2_zero();
+    if (at.active) {
+      gn_load_param4<T>(weight, at.c, s, 1.0f, w);
+      gn_load_param4<T>(bias, at.c, s, 0.0f, b);
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) {
+        const long long row = at.sample * s.G, lo = row + (at.c + 2 * i) / s.Cg;
+        const long long hi = SUB == 4 ? lo : row + (at.c + 2 * i + 1) / s.Cg;
+        m[i] = f2_bits(make_float2(mean[lo], mean[hi]));
+        rs[i] = f2_bits(make_float2(rstd[lo], rstd[hi]));
+      }
+    }
+    const unsigned char* q = saved;
+    uint4* g_at = gs;
     const uint8_t* sp = sp0;
     for (int part = 0; part < 4; ++part) {
       cp_async_wait_part(part);
       const int end = min(mine, (part + 1) * quarter);
 #pragma unroll 2
-      for (int i = part * quarter; i < end; ++i, q += nt * kSaved, lo += nt, hi += nt) {
+      for (int i = part * quarter; i < end; ++i, q += nt * kSaved, g_at += nt) {
         uint32_t E = 0;
         if constexpr (SRC8) {
           E = *sp;
           sp += sstep;
         }
-        f32x2 xh[4], g[4];
+        f32x2 xh[2], g[2];
         x_hat(q, E, xh);
-        gn_unpack<T>(*hi, g);
+        const uint2 v = reinterpret_cast<const uint2*>(g_at)[1];
+        g[0] = Type16<T>::to_f32x2(v.x);
+        g[1] = Type16<T>::to_f32x2(v.y);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 2; ++j) {
           g[j] = fmul2(g[j], act_slope2<ACT>(fma2(xh[j], w[j], b[j])));
           fadd2(sg[j], g[j]);
           ffma2(sx[j], g[j], xh[j]);
         }
-        *reinterpret_cast<ulonglong2*>(lo) = make_ulonglong2(g[0], g[1]);
-        *reinterpret_cast<ulonglong2*>(hi) = make_ulonglong2(g[2], g[3]);
+        *reinterpret_cast<ulonglong2*>(g_at) = make_ulonglong2(g[0], g[1]);
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 2; ++j) {
       const float2 a = bits_f2(sg[j]), c = bits_f2(sx[j]);
-      *reinterpret_cast<float4*>(ent + tid * 8 + 2 * j) = make_float4(a.x, c.x, a.y, c.y);
+      *reinterpret_cast<float4*>(ent + tid * 4 + 2 * j) = make_float4(a.x, c.x, a.y, c.y);
     }
   }
   __syncthreads();
   for (int j = tid; j < at.width; j += nt) {
     float2 a = make_float2(0.0f, 0.0f);
-#pragma unroll 4
+#pragma unroll 8
     for (int r = 0; r < p.rl; ++r) {
-      const float2 e = ent[r * p.lanes * 8 + j];
+      const float2 e = ent[r * p.lanes * 4 + j];
       a.x += e.x;
       a.y += e.y;
     }
@@ -410,7 +352,7 @@ __global__ void __launch_bounds__(kGnThreads, kGnBackwardCtas)
     float2 a = chan[j];
     if (p.cluster > 1) {
       a = make_float2(0.0f, 0.0f);
-#pragma unroll 4
+#pragma unroll 8
       for (int r = 0; r < p.cluster; ++r) {
         const float2 e = cluster_load(chan + j, r);
         a.x += e.x;
@@ -431,34 +373,42 @@ __global__ void __launch_bounds__(kGnThreads, kGnBackwardCtas)
       m1 += total[g * s.Cg + j].x;
       m2 += total[g * s.Cg + j].y;
     }
-    m1 = warp_sum(m1);
-    m2 = warp_sum(m2);
+    warp_sum2(m1, m2);
     if (lane == 0) fin[g] = make_float2(m1 * inv, -m2 * inv);
   }
   __syncthreads();
   f32x2 m1[kParts], m2[kParts];
-  if (at.active) gn_read_groups<SUB>(fin, at.vec * 8, s.Cg, m1, m2);
-  const unsigned char* q = saved + tid * kSaved;
-  const uint4 *lo = g_lo + tid, *hi = g_hi + tid;
+  if (at.active) {
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      const int c = at.vec * 4 + 2 * i;
+      const float2 lo = fin[c / s.Cg], hi = SUB == 4 ? lo : fin[(c + 1) / s.Cg];
+      m1[i] = f2_bits(make_float2(lo.x, hi.x));
+      m2[i] = f2_bits(make_float2(lo.y, hi.y));
+    }
+  }
+  const unsigned char* q = saved;
+  const uint4* g_at = gs;
   const uint8_t* sp = sp0;
   T* out = dx + first;
 #pragma unroll 2
-  for (int i = 0; i < mine; ++i, q += nt * kSaved, lo += nt, hi += nt, out += step) {
+  for (int i = 0; i < mine; ++i, q += nt * kSaved, g_at += nt, out += step) {
     uint32_t E = 0;
     if constexpr (SRC8) {
       E = *sp;
       sp += sstep;
     }
-    f32x2 xh[4];
+    f32x2 xh[2];
     x_hat(q, E, xh);
-    const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(lo), c = *reinterpret_cast<const ulonglong2*>(hi);
-    const f32x2 g[4] = {a.x, a.y, c.x, c.y};
+    const ulonglong2 gv = *reinterpret_cast<const ulonglong2*>(g_at);
+    const f32x2 g[2] = {gv.x, gv.y};
     // the product rounded by itself, so that a group whose m1 is that product leaves exactly nothing
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      xh[j] = fmul2(gn_of<SUB>(rs, j),
-                    fma2(xh[j], gn_of<SUB>(m2, j), fsub2(fmul2(g[j], w[j]), gn_of<SUB>(m1, j))));
-    *reinterpret_cast<uint4*>(out) = gn_pack<T>(xh);
+    for (int j = 0; j < 2; ++j) {
+      constexpr int kStep = SUB == 4 ? 0 : 1;
+      xh[j] = fmul2(rs[j * kStep], fma2(xh[j], m2[j * kStep], fsub2(fmul2(g[j], w[j]), m1[j * kStep])));
+    }
+    *reinterpret_cast<uint2*>(out) = make_uint2(Type16<T>::from_f32x2(xh[0]), Type16<T>::from_f32x2(xh[1]));
   }
   if (p.cluster > 1) cluster_wait();
 }
@@ -471,10 +421,11 @@ static int gn_sub(const GnShape& s) { return s.Cg % 8 == 0 ? 8 : s.Cg % 4 == 0 ?
 
 static bool gn_resident_fill(const GnShape& s, GnPass pass, int slab, int cluster, int limit, GnResident* p) {
   const int most = kGnThreads;
-  const int bytes = pass == GnPass::kForward ? 16 : pass == GnPass::kBackward16 ? 48 : 40;
+  // a thread's 8 (forward) or 4 channels of a pixel
+  const int bytes = pass == GnPass::kForward ? 16 : pass == GnPass::kBackward16 ? 24 : 20;
   p->slab = slab;
   p->slabs = (s.C + slab - 1) / slab;
-  p->lanes = (slab / 8 + 3) / 4 * 4;
+  p->lanes = pass == GnPass::kForward ? (slab / 8 + 3) / 4 * 4 : slab / 4;  // forward: the checkpoint's quads
   if (p->lanes > most) return false;
   const long long rows = (s.P + cluster - 1) / cluster;
   if (rows > (1 << 20)) return false;
@@ -489,32 +440,40 @@ static bool gn_resident_fill(const GnShape& s, GnPass pass, int slab, int cluste
   p->iters = (p->rows_per_cta + p->rl - 1) / p->rl;
   const long long extra = pass == GnPass::kForward
                               ? 8LL * (p->threads * (8 / gn_sub(s)) + 2 * (slab / s.Cg))
-                              : 8LL * (p->threads * 8 + 2 * slab + slab / s.Cg);
+                              : 8LL * (p->threads * 4 + 2 * slab + slab / s.Cg);
   const long long need = static_cast<long long>(p->iters) * p->threads * bytes + extra;
   if (need > limit) return false;
   p->smem = static_cast<int>(need);
   return s.B <= 65535;  // grid y
 }
 
+// The rule.  A unit's pixels are shared by the fewest CTAs (1 to 8) that hold them four to an SM, else two to an SM:
+// 32x32x1536, 32 groups, B = 16, forward: 33 us with 4 CTAs of 49 KB, 35 with 2 of 98 KB, 40 with 8 of 25 KB.  What
+// needs more goes to the streaming passes (one group over 32x32x768, B = 8: 8 CTAs of 196 KB 14.2 us, 16 of 98 KB
+// 11.4 us, streaming 11.2 us).
+// Backward, the streaming passes are faster from about 7 CTAs an SM on: 32x32x1536 with B = 2 / 4 / 8 / 16, resident
+// 12.5 / 24.3 / 44.1 / 81 us, streaming 17.9 / 25.9 / 41.2 / 67 us; a cluster's exchange (3.7 us) is too long for the
+// little that four CTAs an SM bring along.  Forward the resident kernels stay ahead at every size (56x56x1024,
+// B = 32: 97 against 119 us): they move two thirds of the data.
 bool gn_resident_plan(const GnShape& s, GnPass pass, GnResident* p) {
-  // shared memory of four, two and one CTAs an SM: 228 KB less 1 KB each
-  constexpr int kFour = 56 * 1024, kTwo = 113 * 1024, kOne = 227 * 1024;
-  const long long unit_ll = static_cast<long long>(s.Cg) / gcd_int(s.Cg, kAct8Block) * kAct8Block;
-  const int unit = unit_ll < s.C ? static_cast<int>(unit_ll) : s.C;
-  // whole 128-byte lines of a pixel where that costs no occupancy
-  int slab = unit;
-  while (slab < 64 && slab < s.C) slab = slab + unit < s.C ? slab + unit : s.C;
-  for (int limit : {kFour, kTwo, kOne})
-    for (int width : {slab, unit})
-      for (int cluster = 1; cluster <= 16; cluster *= 2)
-        if (gn_resident_fill(s, pass, width, cluster, limit, p)) {
-          // few clusters: more CTAs share a sample, as long as each thread keeps a few pixels
-          GnResident wider;
-          while (static_cast<long long>(s.B) * p->slabs * p->cluster < 2 * kSmCount && p->cluster < 8 && p->iters > 4 &&
-                 gn_resident_fill(s, pass, width, p->cluster * 2, limit, &wider))
-            *p = wider;
-          return true;
-        }
+  // shared memory of four and two CTAs an SM: 228 KB less 1 KB each
+  constexpr int kFour = 56 * 1024, kTwo = 113 * 1024;
+  // whole groups; forward: whole blocks of a checkpoint (with and without one: the same plan, the same bits), backward:
+  // whole vectors and, where it can be, 64 bytes of a pixel
+  const int align = pass == GnPass::kForward ? kAct8Block : 8;
+  const long long unit_ll = static_cast<long long>(s.Cg) / gcd_int(s.Cg, align) * align;
+  int unit = unit_ll < s.C ? static_cast<int>(unit_ll) : s.C;
+  for (int k = unit; unit < 32 && unit < s.C;) unit = unit + k < s.C ? unit + k : s.C;
+  for (int limit : {kFour, kTwo})
+    for (int cluster = 1; cluster <= 8; cluster *= 2)
+      if (gn_resident_fill(s, pass, unit, cluster, limit, p)) {
+        // few clusters: more CTAs share a sample, as long as each thread keeps a few pixels
+        GnResident wider;
+        while (static_cast<long long>(s.B) * p->slabs * p->cluster < 2 * kSmCount && p->cluster < 8 && p->iters > 4 &&
+               gn_resident_fill(s, pass, unit, p->cluster * 2, limit, &wider))
+          *p = wider;
+        return pass == GnPass::kForward || static_cast<long long>(s.B) * p->slabs * p->cluster <= 7 * kSmCount;
+      }
   return false;
 }
 
@@ -555,9 +514,7 @@ static const void* resident_fn(int sub, int act) {
 }
 template <typename T, bool SRC8>
 static const void* resident_grad_fn(int sub, int act) {
-  return sub == 8   ? resident_grad_fn<T, SRC8, 8>(act)
-         : sub == 4 ? resident_grad_fn<T, SRC8, 4>(act)
-                    : resident_grad_fn<T, SRC8, 1>(act);
+  return sub >= 4 ? resident_grad_fn<T, SRC8, 4>(act) : resident_grad_fn<T, SRC8, 1>(act);
 }
 
 template <typename T>

@@ -53,6 +53,10 @@ def rounded(ref, dtype):
 SHAPES = [(2, 7, 5, 64, 8), (1, 1, 1, 8, 1), (3, 1, 1, 24, 3), (2, 23, 17, 72, 8), (1, 9, 9, 40, 5), (2, 5, 6, 48, 16),
           (2, 3, 3, 8, 8), (2, 16, 16, 1536, 32), (1, 32, 32, 768, 1), (1, 130, 70, 64, 4), (5, 14, 14, 512, 32),
           (1, 3, 2, 4104, 3), (1, 200, 200, 64, 1), (70, 2, 3, 16, 2), (1, 7, 7, 1024, 32), (1, 57, 1, 200, 25)]
+# tensors that go through memory twice: groups larger than a tile, of 257 channels, of 9, of 4, of 3 in a ragged last
+# tile and of one channel; few long rows; a batch in several groups of samples
+LARGE = [(2, 61, 47, 1536, 2), (2, 31, 33, 2056, 8), (5, 120, 119, 72, 8), (8, 100, 90, 128, 32), (3, 128, 127, 264, 88),
+         (2, 180, 170, 104, 104), (1, 1, 40000, 40, 1), (6, 97, 96, 776, 97)]
 ACTS = ["gelu", "none", "silu", "relu"]
 
 
@@ -140,6 +144,29 @@ def test_backward(eng, i, shape, dtype, kept):
     assert all(torch.equal(p, q) for p, q in zip(got, again))
     got = eng.norm_ops.group_norm_act_backward(dy, saved, mean, rstd, G, None, None, "none")
     check_backward(got, dy, values, mean, rstd, G, None, None, "none")
+
+
+@pytest.mark.parametrize("i,shape", list(enumerate(LARGE)))
+def test_large_tensors(eng, i, shape):
+    """Forward with and without a checkpoint, backward from both."""
+    B, H, W, C, G = shape
+    dtype = [torch.float16, torch.bfloat16][i % 2]
+    act = ["gelu", "silu", "none"][i % 3]
+    x, dy = nhwc(B, C, H, W, i + 300, dtype), nhwc(B, C, H, W, i + 400, dtype, spread=0.3, offset=0.1)
+    w, b = params(C, i, torch.float32 if i % 2 else dtype)
+    got = eng.norm_ops.group_norm_act_forward(x, G, w, b, 1e-5, act, checkpoint=True)
+    check_forward(got, x, G, w, b, 1e-5, act)
+    plain = eng.norm_ops.group_norm_act_forward(x, G, w, b, 1e-5, act)
+    assert all(torch.equal(p, q) for p, q in zip(got, plain))
+    codes, scales = R.act8_encode(x)
+    assert torch.equal(got[3], codes) and torch.equal(got[4], scales)
+    del got, plain
+    mean, rstd = (t.float() for t in R.stats(x, G, 1e-5))
+    for saved, values in ((x, x), ((codes, scales), R.act8_decode(codes, scales))):
+        back = eng.norm_ops.group_norm_act_backward(dy, saved, mean, rstd, G, w, b, act)
+        check_backward(back, dy, values, mean, rstd, G, w, b, act)
+        again = eng.norm_ops.group_norm_act_backward(dy, saved, mean, rstd, G, w, b, act)
+        assert all(torch.equal(p, q) for p, q in zip(back, again))
 
 
 @pytest.mark.parametrize("offset,spread", [(1000.0, 1.0), (0.0, 1e-3), (0.0, 3000.0)])
