@@ -34,10 +34,24 @@ import functools
 import torch
 
 from . import _lib, dw_ops
-from .dw_ops import _DeviceGuard, _stream_of
+from .dw_ops import _DeviceGuard
 
 BLOCK = 32
 DTYPE_CODES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+
+
+def launch(name: str, where: str, device: torch.device, *args) -> None:
+    """Call an entry point with the device's current stream as its last argument, that device being current."""
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        _lib.call(name, *args, stream)
+    else:
+        with _DeviceGuard(device):
+            _lib.call(name, *args, stream)
+    if _lib.check_device_error_enabled():
+        with _DeviceGuard(device):
+            _lib.after_launch(stream, where)
 
 
 def check_nhwc(x: torch.Tensor, name: str = "input") -> int:
@@ -70,8 +84,8 @@ def check_checkpoint(codes: torch.Tensor, scales: torch.Tensor) -> None:
 def empty_checkpoint(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Unwritten codes and scales for an activation like ``x``."""
     B, C, H, W = x.shape
-    codes = torch.empty_like(x, dtype=torch.int8, memory_format=torch.channels_last)
-    return codes, torch.empty((B, H, W, -(-C // BLOCK)), dtype=torch.uint8, device=x.device)
+    codes = torch.empty_like(x, dtype=torch.int8)  # keeps the strides
+    return codes, x.new_empty((B, H, W, -(-C // BLOCK)), dtype=torch.uint8)
 
 
 def act8_encode(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -79,10 +93,8 @@ def act8_encode(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     dtype = check_nhwc(x)
     B, C, H, W = x.shape
     codes, scales = empty_checkpoint(x)
-    with _DeviceGuard(x.device):
-        stream = _stream_of(x)
-        _lib.call("dwb_act8_encode_nhwc", x.data_ptr(), codes.data_ptr(), scales.data_ptr(), B * H * W, C, dtype, stream)
-        _lib.after_launch(stream, "depthwise act8_encode")
+    launch("dwb_act8_encode_nhwc", "depthwise act8_encode", x.device, x.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+           B * H * W, C, dtype)
     return codes, scales
 
 
@@ -92,12 +104,9 @@ def act8_decode(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = 
     if dtype not in DTYPE_CODES:
         raise RuntimeError(f"dtype must be float16 or bfloat16, got {dtype}")
     B, C, H, W = codes.shape
-    x = torch.empty_like(codes, dtype=dtype, memory_format=torch.channels_last)
-    with _DeviceGuard(codes.device):
-        stream = _stream_of(codes)
-        _lib.call("dwb_act8_decode_nhwc", codes.data_ptr(), scales.data_ptr(), x.data_ptr(), B * H * W, C,
-                  DTYPE_CODES[dtype], stream)
-        _lib.after_launch(stream, "depthwise act8_decode")
+    x = torch.empty_like(codes, dtype=dtype)
+    launch("dwb_act8_decode_nhwc", "depthwise act8_decode", codes.device, codes.data_ptr(), scales.data_ptr(), x.data_ptr(),
+           B * H * W, C, DTYPE_CODES[dtype])
     return x
 
 
@@ -122,13 +131,10 @@ def conv2d_nhwc_backward_weight_act8(codes: torch.Tensor, scales: torch.Tensor, 
     B, C, H, W = dy.shape
     K = int(K)
     nbytes = _wgrad_workspace_bytes(B, H, W, C, K)
-    dw = torch.empty((K, K, C), dtype=torch.float32, device=dy.device)
-    ws = torch.empty(max(16, nbytes), dtype=torch.uint8, device=dy.device)
-    with _DeviceGuard(dy.device):
-        stream = _stream_of(dy)
-        _lib.call("dwb_conv2d_nhwc_bwd_weight_act8", codes.data_ptr(), scales.data_ptr(), dy.data_ptr(), dw.data_ptr(),
-                  ws.data_ptr(), ws.numel(), B, H, W, C, K, stream)
-        _lib.after_launch(stream, "depthwise conv2d_nhwc weight gradient from a checkpoint")
+    dw = dy.new_empty((K, K, C), dtype=torch.float32)
+    ws = dy.new_empty((max(16, nbytes),), dtype=torch.uint8)
+    launch("dwb_conv2d_nhwc_bwd_weight_act8", "depthwise conv2d_nhwc weight gradient from a checkpoint", dy.device,
+           codes.data_ptr(), scales.data_ptr(), dy.data_ptr(), dw.data_ptr(), ws.data_ptr(), nbytes, B, H, W, C, K)
     return dw
 
 

@@ -29,8 +29,7 @@ import functools
 import torch
 
 from . import _lib
-from .act8_ops import check_checkpoint, check_nhwc, empty_checkpoint
-from .dw_ops import _DeviceGuard, _stream_of
+from .act8_ops import check_checkpoint, check_nhwc, empty_checkpoint, launch
 
 ACT_CODES = _lib.NORM_ACT_CODES
 
@@ -43,22 +42,27 @@ def _act_code(act) -> int:
     return int(act)
 
 
+def _check_param(name: str, t, like: torch.Tensor) -> None:
+    if not t.is_cuda or t.dtype not in (like.dtype, torch.float32) or t.shape != like.shape[1:2] or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous {like.dtype} or float32 CUDA tensor with {like.shape[1]} elements, "
+                           f"got {t.dtype} {tuple(t.shape)}")
+    if t.device != like.device:
+        raise RuntimeError(f"{name} is on {t.device}, input on {like.device}")
+
+
 def _check_params(weight, bias, like: torch.Tensor, dtype_code: int):
     """Pointers of the parameter vectors and their dwb_dtype."""
-    C = like.shape[1]
-    given = [t for t in (weight, bias) if t is not None]
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is None:
-            continue
-        if not t.is_cuda or t.dtype not in (like.dtype, torch.float32) or t.shape != (C,) or not t.is_contiguous():
-            raise RuntimeError(f"{name} must be a contiguous {like.dtype} or float32 CUDA tensor with {C} elements, "
-                               f"got {t.dtype} {tuple(t.shape)}")
-        if t.device != like.device:
-            raise RuntimeError(f"{name} is on {t.device}, input on {like.device}")
-    if len(given) == 2 and given[0].dtype != given[1].dtype:
-        raise RuntimeError(f"weight and bias must have one type, got {given[0].dtype} and {given[1].dtype}")
-    code = _lib.F32 if given and given[0].dtype == torch.float32 else dtype_code
-    return (weight.data_ptr() if weight is not None else None, bias.data_ptr() if bias is not None else None, code)
+    wp = bp = None
+    if weight is not None:
+        _check_param("weight", weight, like)
+        wp = weight.data_ptr()
+    if bias is not None:
+        _check_param("bias", bias, like)
+        bp = bias.data_ptr()
+        if weight is not None and weight.dtype != bias.dtype:
+            raise RuntimeError(f"weight and bias must have one type, got {weight.dtype} and {bias.dtype}")
+    first = bias if weight is None else weight
+    return wp, bp, _lib.F32 if first is not None and first.dtype == torch.float32 else dtype_code
 
 
 @functools.lru_cache(maxsize=1024)
@@ -68,10 +72,9 @@ def _workspace_bytes(B: int, H: int, W: int, C: int, G: int, backward: int) -> i
     return n.value
 
 
-def _workspace(shape, G: int, backward: int, device):
-    B, C, H, W = shape
+def _workspace(x: torch.Tensor, B: int, H: int, W: int, C: int, G: int, backward: int):
     n = _workspace_bytes(B, H, W, C, G, backward)
-    return (torch.empty(n, dtype=torch.uint8, device=device) if n else None), n
+    return (x.new_empty((n,), dtype=torch.uint8) if n else None), n
 
 
 def group_norm_act_forward(x: torch.Tensor, num_groups: int, weight=None, bias=None, eps: float = 1e-5,
@@ -83,18 +86,15 @@ def group_norm_act_forward(x: torch.Tensor, num_groups: int, weight=None, bias=N
     B, C, H, W = x.shape
     G, act_code = int(num_groups), _act_code(act)
     wp, bp, param_dtype = _check_params(weight, bias, x, dtype)
-    ws, nbytes = _workspace(x.shape, G, 0, x.device)
-    y = torch.empty_like(x, memory_format=torch.channels_last)
-    mean = torch.empty((B, G), dtype=torch.float32, device=x.device)
+    ws, nbytes = _workspace(x, B, H, W, C, G, 0)
+    y = torch.empty_like(x)  # keeps the strides
+    mean = x.new_empty((B, G), dtype=torch.float32)
     rstd = torch.empty_like(mean)
     codes, scales = empty_checkpoint(x) if checkpoint else (None, None)
-    with _DeviceGuard(x.device):
-        stream = _stream_of(x)
-        _lib.call("dwb_group_norm_act_nhwc_fwd", x.data_ptr(), wp, bp, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
-                  codes.data_ptr() if checkpoint else None, scales.data_ptr() if checkpoint else None,
-                  ws.data_ptr() if nbytes else None, nbytes, B, H, W, C, G, float(eps), act_code, dtype, param_dtype,
-                  stream)
-        _lib.after_launch(stream, "depthwise group_norm_act")
+    launch("dwb_group_norm_act_nhwc_fwd", "depthwise group_norm_act", x.device, x.data_ptr(), wp, bp, y.data_ptr(),
+           mean.data_ptr(), rstd.data_ptr(), codes.data_ptr() if checkpoint else None,
+           scales.data_ptr() if checkpoint else None, ws.data_ptr() if nbytes else None, nbytes, B, H, W, C, G, float(eps),
+           act_code, dtype, param_dtype)
     return (y, mean, rstd, codes, scales) if checkpoint else (y, mean, rstd)
 
 
@@ -121,17 +121,14 @@ def group_norm_act_backward(dy: torch.Tensor, saved, mean: torch.Tensor, rstd: t
     for name, t in (("mean", mean), ("rstd", rstd)):
         if t.dtype != torch.float32 or t.shape != (B, G) or not t.is_contiguous() or t.device != dy.device:
             raise RuntimeError(f"{name} must be a contiguous float32 tensor [{B}, {G}] on {dy.device}")
-    ws, nbytes = _workspace(dy.shape, G, 1, dy.device)
-    dx = torch.empty_like(dy, memory_format=torch.channels_last)
+    ws, nbytes = _workspace(dy, B, H, W, C, G, 1)
+    dx = torch.empty_like(dy)
     dweight = torch.empty_like(weight) if weight is not None else None
     dbias = torch.empty_like(bias) if bias is not None else None
-    with _DeviceGuard(dy.device):
-        stream = _stream_of(dy)
-        _lib.call("dwb_group_norm_act_nhwc_bwd", dy.data_ptr(), xp, qp, sp, mean.data_ptr(), rstd.data_ptr(), wp, bp,
-                  dx.data_ptr(), dweight.data_ptr() if dweight is not None else None,
-                  dbias.data_ptr() if dbias is not None else None, ws.data_ptr() if nbytes else None, nbytes,
-                  B, H, W, C, G, act_code, dtype, param_dtype, stream)
-        _lib.after_launch(stream, "depthwise group_norm_act gradient")
+    launch("dwb_group_norm_act_nhwc_bwd", "depthwise group_norm_act gradient", dy.device, dy.data_ptr(), xp, qp, sp,
+           mean.data_ptr(), rstd.data_ptr(), wp, bp, dx.data_ptr(), dweight.data_ptr() if dweight is not None else None,
+           dbias.data_ptr() if dbias is not None else None, ws.data_ptr() if nbytes else None, nbytes, B, H, W, C, G,
+           act_code, dtype, param_dtype)
     return dx, dweight, dbias
 
 
