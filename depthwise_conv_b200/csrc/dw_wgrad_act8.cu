@@ -51,14 +51,12 @@ constexpr int kChain = 128;    // most products added up in one accumulator
 
 struct Wgrad8Params {
   int B, H, W, C, K;
-  int tw;           // columns of dy a tile holds (a multiple of 16)
+  int tw;           // columns of dy a tile holds (16, 32, 48 or 64)
   int col_tiles;
   int units;        // B * ceil(H / ROWS) steps of ROWS rows of x
   int unit_rows;    // ceil(H / ROWS)
   int per_chunk;    // units a CTA takes
   int chunks;
-  int xp, dp;       // words of a channel's row of x (one copy) and of dy, both odd
-  int ring;         // rows of dy kept
 };
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -82,112 +80,118 @@ __device__ __forceinline__ void codes_to_half(const uint2& q, uint32_t E, uint32
   }
 }
 
-// Five neighbouring pixels' codes: four columns of the tile and the one behind them.
-struct XItem {
-  uint2 q[5];
+constexpr int kAhead = 2;      // steps that global memory is read ahead
+
+// The exponent bytes of five neighbouring pixels: four columns of the tile and the one behind them.
+struct XScales {
   uint8_t e[5];
 };
 
-// MT x NT: 16-tap by 8-row products of one x row; ROWS: x rows a step; PACK: both rows in one product.
-template <int MT, int NT, int ROWS, bool PACK>
+// Asynchronous copies, of zeros where `on` is false (nothing is read then).
+__device__ __forceinline__ void copy8(void* dst, const void* src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(on ? 8 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copy16(void* dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+
+constexpr int up_to(int v, int to, int mod) { return v % mod == to % mod ? v : up_to(v + 1, to, mod); }
+constexpr int smaller(int a, int b) { return a < b ? a : b; }
+
+// MT x NT: 16-tap by 8-row products of one x row; ROWS: x rows a step; PACK: both rows in one product; TW: columns.
+//
+// Shared memory, in words of two columns: x [2 buffers][ROWS][2 copies][32 channels][XP], dy [ring][32 channels][DP].
+// In x, channel 8 v + k has place 4 k + v and XP is 8 or 24 modulo 32; in dy, places are channels and DP is odd: the
+// stores of a warp (4 vectors of 8 channels times 8 column pairs of x, or 8 words of dy) fall in 32 banks.  The copies
+// are 16 banks apart and the rows of dy 4, so that a fragment's 32 words do too.  Behind them, for each step read
+// ahead, the codes and values that a thread has under way: each in places of its own, which need no barrier.
+template <int MT, int NT, int ROWS, bool PACK, int TW>
 struct Wgrad8 {
-  const Wgrad8Params& p;
-  const int8_t* codes;
-  const uint8_t* scales;
-  const __half* dy;
-  uint32_t* xs;   // [2 buffers][ROWS][2 copies][32 channels][xp] (+16 words a copy: the copies' banks differ)
-  uint32_t* ds;   // [ring][32 channels][dp] (+4 words a row: 8 rows x 4 words fall in 32 banks)
-  int c0, w0, sblocks;
+  static constexpr int kXWords = (TW + (PACK ? 8 : 16 * MT)) / 2, kDWords = TW / 2;
+  static constexpr int XP = smaller(up_to(kXWords, 8, 32), up_to(kXWords, 24, 32));
+  static constexpr int DP = kDWords | 1;
+  static constexpr int kCopy = kWgChannels * XP + 16, kXRow = 2 * kCopy, kXBuffer = ROWS * kXRow;
+  static constexpr int kDRow = kWgChannels * DP + 4;
+  static constexpr int kDItems = TW * 2;  // of a row of dy: 2 columns x 8 channels
+  static constexpr int kBlocks = TW / 16;
+  static constexpr int kAcc = PACK ? 1 : ROWS;
+  typedef float Acc[4][kAcc][MT][NT][4];
 
-  __device__ __forceinline__ int copy_words() const { return kWgChannels * p.xp + 16; }
-  __device__ __forceinline__ int row_words() const { return kWgChannels * p.dp + 4; }
-  __device__ __forceinline__ int x_items() const { return ((p.tw + p.K - 1 + 3) / 4) * 4; }  // of one row
-  __device__ __forceinline__ int dy_items() const { return p.tw * 2; }                        // of one row
-
-  __device__ __forceinline__ void load_x(XItem& it, int b, int row, int item) const {
-    const int c = c0 + (item & 3) * 8, col = w0 - p.K / 2 + (item >> 2) * 4;
-    const bool on = row < p.H && c < p.C;
-    const long long line = (static_cast<long long>(b) * p.H + row) * p.W;
-#pragma unroll
-    for (int j = 0; j < 5; ++j) {
-      const bool in = on && col + j >= 0 && col + j < p.W;
-      it.q[j] = in ? *reinterpret_cast<const uint2*>(codes + (line + col + j) * p.C + c) : make_uint2(0u, 0u);
-      it.e[j] = in ? scales[(line + col + j) * sblocks + c / kAct8Block] : static_cast<uint8_t>(127);
-    }
+  static constexpr int ring(int K) { return K - 1 + 2 * ROWS; }
+  static constexpr int x_items(int K) { return (TW + K - 1 + 3) / 4 * 4; }  // of a row of x
+  static constexpr int fixed_words(int K) { return (2 * kXBuffer + ring(K) * kDRow + 3) / 4 * 4; }
+  static constexpr int smem(int K) {
+    return 4 * fixed_words(K) + kAhead * ROWS * (x_items(K) * 5 * 8 + kDItems * 2 * 16);
   }
-  // even copy: words (4i, 4i+1), (4i+2, 4i+3); odd copy: (4i+1, 4i+2), (4i+3, 4i+4)
-  __device__ __forceinline__ void store_x(const XItem& it, int buffer, int r, int item) const {
+
+  // even copy: words (4i, 4i + 1), (4i + 2, 4i + 3); odd copy: (4i + 1, 4i + 2), (4i + 3, 4i + 4)
+  static __device__ __forceinline__ void store_x(const uint2 (&q)[5], const XScales& s, uint32_t* row, int item) {
     uint32_t h[5][4];
 #pragma unroll
-    for (int j = 0; j < 5; ++j) codes_to_half(it.q[j], it.e[j], h[j]);
-    uint32_t* even = xs + (buffer * ROWS + r) * 2 * copy_words() + (item & 3) * 8 * p.xp + (item >> 2) * 2;
-    uint32_t* odd = even + copy_words();
+    for (int j = 0; j < 5; ++j) codes_to_half(q[j], s.e[j], h[j]);
+    uint32_t* even = row + (item & 3) * XP + (item >> 2) * 2;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const uint32_t sel = (k & 1) ? 0x7632 : 0x5410;
-      even[k * p.xp] = __byte_perm(h[0][k / 2], h[1][k / 2], sel);
-      even[k * p.xp + 1] = __byte_perm(h[2][k / 2], h[3][k / 2], sel);
-      odd[k * p.xp] = __byte_perm(h[1][k / 2], h[2][k / 2], sel);
-      odd[k * p.xp + 1] = __byte_perm(h[3][k / 2], h[4][k / 2], sel);
+      *reinterpret_cast<uint2*>(even + k * 4 * XP) =
+          make_uint2(__byte_perm(h[0][k / 2], h[1][k / 2], sel), __byte_perm(h[2][k / 2], h[3][k / 2], sel));
+      *reinterpret_cast<uint2*>(even + kCopy + k * 4 * XP) =
+          make_uint2(__byte_perm(h[1][k / 2], h[2][k / 2], sel), __byte_perm(h[3][k / 2], h[4][k / 2], sel));
     }
   }
-  __device__ __forceinline__ void load_dy(uint4 (&v)[2], int b, int row, int item) const {
-    const int c = c0 + (item & 3) * 8, col = w0 + (item >> 2) * 2;
-    const bool on = row >= 0 && row < p.H && c < p.C;
-    const long long line = (static_cast<long long>(b) * p.H + row) * p.W;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      v[j] = on && col + j < p.W ? *reinterpret_cast<const uint4*>(dy + (line + col + j) * p.C + c)
-                                 : make_uint4(0u, 0u, 0u, 0u);
-  }
-  __device__ __forceinline__ void store_dy(const uint4 (&v)[2], int slot, int item) const {
-    uint32_t* at = ds + slot * row_words() + (item & 3) * 8 * p.dp + (item >> 2);
+  static __device__ __forceinline__ void store_dy(const uint4 (&v)[2], uint32_t* row, int item) {
+    uint32_t* at = row + (item & 3) * 8 * DP + (item >> 2);
     const uint32_t a[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, b[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
 #pragma unroll
-    for (int k = 0; k < 8; ++k) at[k * p.dp] = __byte_perm(a[k / 2], b[k / 2], (k & 1) ? 0x7632 : 0x5410);
+    for (int k = 0; k < 8; ++k) at[k * DP] = __byte_perm(a[k / 2], b[k / 2], (k & 1) ? 0x7632 : 0x5410);
   }
 
-  // One step: ROWS rows of x in `buffer` against the ring rows first, first + 1, ...
-  __device__ __forceinline__ void multiply(float (&acc)[4][PACK ? 1 : ROWS][MT][NT][4], int buffer, int first) const {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const uint32_t* xa = xs + buffer * ROWS * 2 * copy_words() + (g & 1) * copy_words() + warp * 4 * p.xp + (g >> 1) + t;
-    const int used = p.K - 1 + ROWS;
+  // Place in x of this warp's first channel (4 * warp); its channels are 4 places apart.
+  static __device__ __forceinline__ int warp_place() {
+    const int warp = threadIdx.x >> 5;
+    return (warp & 1) * 16 + (warp >> 1);
+  }
+
+  // One step: ROWS rows of x at `xs` against the ring rows first, first + 1, ...
+  static __device__ __forceinline__ void multiply(Acc& acc, const uint32_t* xs, const uint32_t* ds, int first, int K) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t* xa = xs + (g & 1) * kCopy + warp_place() * XP + (g >> 1) + t;
+    const int used = K - 1 + ROWS;
     const uint32_t* db[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int j = n * 8 + g < used ? n * 8 + g : 0;  // rows past the last one feed columns that nothing reads
-      const int slot = first + j < p.ring ? first + j : first + j - p.ring;
-      db[n] = ds + slot * row_words() + warp * 4 * p.dp + t;
+      const int slot = first + j < ring(K) ? first + j : first + j - ring(K);
+      db[n] = ds + slot * kDRow + static_cast<int>(threadIdx.x >> 5) * 4 * DP + t;
     }
-    const int blocks = p.tw / 16;
 #pragma unroll
     for (int ch = 0; ch < 4; ++ch) {
-      const uint32_t* x0 = xa + ch * p.xp;
+      const uint32_t* x0 = xa + ch * 4 * XP;
       if constexpr (PACK) {
-        const uint32_t* x1 = x0 + 2 * copy_words();
-#pragma unroll 4
-        for (int w = 0; w < blocks; ++w)
-          mma_16816(acc[ch][0][0][0], x0[w * 8], x1[w * 8], x0[w * 8 + 4], x1[w * 8 + 4], db[0][ch * p.dp + w * 8],
-                    db[0][ch * p.dp + w * 8 + 4]);
+#pragma unroll
+        for (int w = 0; w < kBlocks; ++w)
+          mma_16816(acc[ch][0][0][0], x0[w * 8], x0[kXRow + w * 8], x0[w * 8 + 4], x0[kXRow + w * 8 + 4],
+                    db[0][ch * DP + w * 8], db[0][ch * DP + w * 8 + 4]);
       } else {
         // a row's words 8 columns apart: A tile m of a block needs words 2m, 2m + 1, 2m + 1, 2m + 2
         uint32_t a[ROWS][2 * MT + 1];
 #pragma unroll
         for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-          for (int i = 0; i < 2 * MT - 1; ++i) a[r][i + 2] = x0[r * 2 * copy_words() + i * 4];
-#pragma unroll 2
-        for (int w = 0; w < blocks; ++w) {
+          for (int i = 0; i < 2 * MT - 1; ++i) a[r][i + 2] = x0[r * kXRow + i * 4];
+#pragma unroll
+        for (int w = 0; w < kBlocks; ++w) {
 #pragma unroll
           for (int r = 0; r < ROWS; ++r) {  // 16 columns on: all words but two are the last block's
 #pragma unroll
             for (int i = 0; i < 2 * MT - 1; ++i) a[r][i] = a[r][i + 2];
-            a[r][2 * MT - 1] = x0[r * 2 * copy_words() + w * 8 + (2 * MT - 1) * 4];
-            a[r][2 * MT] = x0[r * 2 * copy_words() + w * 8 + 2 * MT * 4];
+            a[r][2 * MT - 1] = x0[r * kXRow + w * 8 + (2 * MT - 1) * 4];
+            a[r][2 * MT] = x0[r * kXRow + w * 8 + 2 * MT * 4];
           }
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const uint32_t b0 = db[n][ch * p.dp + w * 8], b1 = db[n][ch * p.dp + w * 8 + 4];
+            const uint32_t b0 = db[n][ch * DP + w * 8], b1 = db[n][ch * DP + w * 8 + 4];
 #pragma unroll
             for (int r = 0; r < ROWS; ++r)
 #pragma unroll
@@ -200,13 +204,12 @@ struct Wgrad8 {
   }
 
   // Row j of dy and row r of x belong to kh = K - 1 - j + r: the two rows' columns j and j + 1 are added.
-  __device__ __forceinline__ void write(float (&acc)[4][PACK ? 1 : ROWS][MT][NT][4], float* slice) const {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int c = c0 + warp * 4;
-    if (c >= p.C) return;
+  static __device__ __forceinline__ void write(Acc& acc, float* slice, int c, int C, int K) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    if (c >= C) return;
     auto put = [&](int kh, int kw, float v0, float v1, float v2, float v3) {
-      if (kh >= 0 && kh < p.K && kw < p.K)
-        *reinterpret_cast<float4*>(slice + (static_cast<long long>(kh) * p.K + kw) * p.C + c) = make_float4(v0, v1, v2, v3);
+      if (kh >= 0 && kh < K && kw < K)
+        *reinterpret_cast<float4*>(slice + (static_cast<long long>(kh) * K + kw) * C + c) = make_float4(v0, v1, v2, v3);
     };
     if constexpr (PACK) {
       float lo[4], hi[4];
@@ -216,8 +219,8 @@ struct Wgrad8 {
         lo[ch] = d[0] + d[3];
         hi[ch] = d[1] + __shfl_down_sync(0xffffffffu, d[2], 1);  // column 2t + 2; past the last one kh < 0
       }
-      put(p.K - 1 - 2 * t, g, lo[0], lo[1], lo[2], lo[3]);
-      put(p.K - 2 - 2 * t, g, hi[0], hi[1], hi[2], hi[3]);
+      put(K - 1 - 2 * t, g, lo[0], lo[1], lo[2], lo[3]);
+      put(K - 2 - 2 * t, g, hi[0], hi[1], hi[2], hi[3]);
     } else {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -240,32 +243,82 @@ struct Wgrad8 {
               }
             }
             const int j = n * 8 + 2 * t, kw = m * 16 + half * 8 + g;
-            put(p.K - 1 - j, kw, lo[0], lo[1], lo[2], lo[3]);
-            put(p.K - 2 - j, kw, hi[0], hi[1], hi[2], hi[3]);
+            put(K - 1 - j, kw, lo[0], lo[1], lo[2], lo[3]);
+            put(K - 2 - j, kw, hi[0], hi[1], hi[2], hi[3]);
           }
     }
   }
 };
 
-template <int MT, int NT, int ROWS, bool PACK>
-__global__ void __launch_bounds__(kWgThreads) wgrad8_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+template <int MT, bool PACK>
+constexpr int kWgCtas = PACK ? 3 : MT == 1 ? 2 : 1;
+
+template <int MT, int NT, int ROWS, bool PACK, int TW>
+__global__ void __launch_bounds__(kWgThreads, kWgCtas<MT, PACK>) wgrad8_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                             const __half* __restrict__ dy, float* __restrict__ part,
                                                             const Wgrad8Params p) {
+  using S = Wgrad8<MT, NT, ROWS, PACK, TW>;
   extern __shared__ __align__(16) uint32_t smem[];
+  uint32_t* const xs = smem;
+  uint32_t* const ds = smem + 2 * S::kXBuffer;
   griddep_wait();
   griddep_launch_dependents();
-  Wgrad8<MT, NT, ROWS, PACK> k{p, codes, scales, dy, smem, nullptr, 0, 0, 0};
-  k.ds = smem + 2 * ROWS * 2 * k.copy_words();
-  k.c0 = blockIdx.x * kWgChannels;
-  k.w0 = static_cast<int>(blockIdx.z) * p.tw;
-  k.sblocks = (p.C + kAct8Block - 1) / kAct8Block;
-  const int pad = p.K / 2, used = p.K - 1 + ROWS, tid = threadIdx.x;
-  const int xi = k.x_items(), di = k.dy_items();
-  float acc[4][PACK ? 1 : ROWS][MT][NT][4];
+  const int c0 = blockIdx.x * kWgChannels, w0 = static_cast<int>(blockIdx.z) * TW, tid = threadIdx.x;
+  const int sblocks = (p.C + kAct8Block - 1) / kAct8Block, pad = p.K / 2, used = p.K - 1 + ROWS, ring = S::ring(p.K);
+
+  // What this thread brings in at every step, a row further each time: one item of x (columns x_col .. x_col + 4, of
+  // row x_row of the step's ROWS) and one of dy (2 columns of row d_row).
+  const int x_items = S::x_items(p.K);
+  const int x_row = tid / x_items, x_item = tid - x_row * x_items;
+  const int x_c = c0 + (x_item & 3) * 8, x_col = w0 - pad + (x_item >> 2) * 4;
+  unsigned x_mask = 0;
+#pragma unroll
+  for (int j = 0; j < 5; ++j)
+    if (x_row < ROWS && x_c < p.C && x_col + j >= 0 && x_col + j < p.W) x_mask |= 1u << j;
+  // the last warps begin with dy, so that those that convert codes have none of it where the tile is narrow
+  const int d_tid = kWgThreads - 1 - tid, d_row = d_tid / S::kDItems, d_item = d_tid - d_row * S::kDItems;
+  const int d_c = c0 + (d_item & 3) * 8, d_col = w0 + (d_item >> 2) * 2;
+  unsigned d_mask = 0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    if (d_row < ROWS && d_c < p.C && d_col + j < p.W) d_mask |= 1u << j;
+  const long long line = static_cast<long long>(p.W) * p.C, s_line = static_cast<long long>(p.W) * sblocks;
+  unsigned char* const raw = reinterpret_cast<unsigned char*>(smem + S::fixed_words(p.K));
+  uint2* const x_raw = reinterpret_cast<uint2*>(raw) + tid;                                              // [kAhead][5][items]
+  uint4* const d_raw = reinterpret_cast<uint4*>(raw + kAhead * ROWS * x_items * 5 * 8) + d_tid;           // [kAhead][2][items]
+  const int x_many = ROWS * x_items, d_many = ROWS * S::kDItems;
+
+  // A row past the image: codes of 0, whatever the step.
+  auto load_scales = [&](XScales& s, const uint8_t* e, bool on) {
+#pragma unroll
+    for (int j = 0; j < 5; ++j) s.e[j] = on && (x_mask >> j & 1) ? e[j * sblocks] : static_cast<uint8_t>(127);
+  };
+  auto fetch = [&](int place, const int8_t* q, bool x_on, const __half* d, bool d_on) {
+    if (x_row < ROWS) {
+#pragma unroll
+      for (int j = 0; j < 5; ++j) {
+        const bool on = x_on && (x_mask >> j & 1);
+        copy8(x_raw + (place * 5 + j) * x_many, on ? q + j * p.C : codes, on);
+      }
+    }
+    if (d_row < ROWS) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const bool on = d_on && (d_mask >> j & 1);
+        copy16(d_raw + (place * 2 + j) * d_many, on ? d + j * p.C : dy, on);
+      }
+    }
+  };
+  auto fetched_x = [&](int place, uint2 (&q)[5]) {
+#pragma unroll
+    for (int j = 0; j < 5; ++j) q[j] = x_raw[(place * 5 + j) * x_many];
+  };
+
+  typename S::Acc acc;
 #pragma unroll
   for (int ch = 0; ch < 4; ++ch)
 #pragma unroll
-    for (int r = 0; r < (PACK ? 1 : ROWS); ++r)
+    for (int r = 0; r < S::kAcc; ++r)
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -279,82 +332,127 @@ __global__ void __launch_bounds__(kWgThreads) wgrad8_kernel(const int8_t* __rest
     const int b = u / p.unit_rows;
     const int s0 = u - b * p.unit_rows, steps = min(p.unit_rows - s0, u1 - u);
     const int top = s0 * ROWS + pad - (p.K - 1);  // first row of dy that the first row of x meets
-    __syncthreads();                              // the last image's rows have been read
-    for (int i = tid; i < used * di; i += kWgThreads) {
+    // of x and dy, this thread's next to fetch; of the exponent bytes, its next to load
+    int row = s0 * ROWS + x_row, drow = top + used + d_row;
+    const long long x_at = (static_cast<long long>(b) * p.H + row) * p.W + x_col;
+    const int8_t* q = codes + x_at * p.C + x_c;
+    const uint8_t* e = scales + x_at * sblocks + x_c / kAct8Block;
+    const __half* d = dy + ((static_cast<long long>(b) * p.H + drow) * p.W + d_col) * p.C + d_c;
+    // `step` of this image, at place step % kAhead; past the last one nothing is written there
+    auto next = [&](int step) {
+      if (step < steps) fetch(step & 1, q, row < p.H, d, drow >= 0 && drow < p.H);
+      cp_async_commit();
+      row += ROWS;
+      drow += ROWS;
+      q += ROWS * line;
+      d += ROWS * line;
+    };
+    __syncthreads();  // the last image's rows have been read
+    // the first step: its row of x, and all rows of dy that it meets
+    XScales sc[2];
+    load_scales(sc[0], e, s0 * ROWS + x_row < p.H);
+    fetch(0, q, row < p.H, d, false);
+    cp_async_commit();
+    row += ROWS;
+    q += ROWS * line;
+    for (int i = tid; i < used * S::kDItems; i += kWgThreads) {
+      const int r = i / S::kDItems, item = i - r * S::kDItems, at = top + r;
+      const int c = c0 + (item & 3) * 8, col = w0 + (item >> 2) * 2;
+      const __half* from = dy + ((static_cast<long long>(b) * p.H + at) * p.W + col) * p.C + c;
+      const bool on = at >= 0 && at < p.H && c < p.C;
       uint4 v[2];
-      const int r = i / di;
-      k.load_dy(v, b, top + r, i - r * di);
-      k.store_dy(v, r, i - r * di);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        v[j] = on && col + j < p.W ? *reinterpret_cast<const uint4*>(from + j * p.C) : make_uint4(0u, 0u, 0u, 0u);
+      S::store_dy(v, ds + r * S::kDRow, item);
     }
-    if (tid < ROWS * xi) {
-      XItem it;
-      const int r = tid / xi;
-      k.load_x(it, b, s0 * ROWS + r, tid - r * xi);
-      k.store_x(it, 0, r, tid - r * xi);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (x_row < ROWS) {
+      uint2 v[5];
+      fetched_x(0, v);
+      S::store_x(v, sc[0], xs + x_row * S::kXRow, x_item);
     }
+    e += ROWS * s_line;
+    load_scales(sc[0], e, steps > 1 && s0 * ROWS + ROWS + x_row < p.H);  // step 1
+    next(1);
     __syncthreads();
     int first = 0;  // ring slot of the row of dy with j = 0
     for (int s = 0; s < steps; ++s) {
       const bool more = s + 1 < steps;
-      XItem it;
-      uint4 v[2];
-      const int xr = tid / xi, dr = tid / di;
-      const bool get_x = more && xr < ROWS, get_dy = more && dr < ROWS;
-      if (get_x) k.load_x(it, b, (s0 + s + 1) * ROWS + xr, tid - xr * xi);
-      if (get_dy) k.load_dy(v, b, top + s * ROWS + used + dr, tid - dr * di);
-      k.multiply(acc, s & 1, first);
-      if (get_x) k.store_x(it, (s + 1) & 1, xr, tid - xr * xi);
-      if (get_dy) {
-        // the ring has ROWS rows more than a step reads: these slots belong to no row of this step
-        int slot = first + used + dr;
-        slot -= slot >= p.ring ? p.ring : 0;
-        k.store_dy(v, slot, tid - dr * di);
+      e += ROWS * s_line;
+      load_scales(sc[1], e, s + 2 < steps && (s0 + s + 2) * ROWS + x_row < p.H);
+      next(s + 2);
+      S::multiply(acc, xs + (s & 1) * S::kXBuffer, ds, first, p.K);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");  // step s + 1 is here
+      if (more && x_row < ROWS) {
+        uint2 v[5];
+        fetched_x((s + 1) & 1, v);
+        S::store_x(v, sc[0], xs + ((s + 1) & 1) * S::kXBuffer + x_row * S::kXRow, x_item);
       }
+      if (more && d_row < ROWS) {
+        // the ring has ROWS rows more than a step reads: these slots belong to no row of this step
+        int slot = first + used + d_row;
+        slot -= slot >= ring ? ring : 0;
+        const uint4 v[2] = {d_raw[((s + 1) & 1) * 2 * d_many], d_raw[(((s + 1) & 1) * 2 + 1) * d_many]};
+        S::store_dy(v, ds + slot * S::kDRow, d_item);
+      }
+      sc[0] = sc[1];
       first += ROWS;
-      first -= first >= p.ring ? p.ring : 0;
+      first -= first >= ring ? ring : 0;
       __syncthreads();
     }
     u += steps;
   }
   const long long slice = static_cast<long long>(blockIdx.z) * p.chunks + blockIdx.y;
-  k.write(acc, part + slice * p.K * p.K * p.C);
+  S::write(acc, part + slice * p.K * p.K * p.C, c0 + (tid >> 5) * 4, p.C, p.K);
 }
 
-// dw[i] = the slices' values added in slice order (n4 groups of 4).
-__global__ void __launch_bounds__(256) wgrad8_reduce_kernel(const float4* __restrict__ part, float4* __restrict__ dw,
-                                                            long long n4, int slices) {
+// dw[i] = the slices' values added in slice order (n2 pairs).
+__global__ void __launch_bounds__(256) wgrad8_reduce_kernel(const float2* __restrict__ part, float2* __restrict__ dw,
+                                                            long long n2, int slices) {
   griddep_wait();
   griddep_launch_dependents();
   const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= n4) return;
-  float4 a = part[i];
+  if (i >= n2) return;
+  float2 a = part[i];
+#pragma unroll 8
   for (int s = 1; s < slices; ++s) {
-    const float4 v = part[s * n4 + i];
+    const float2 v = part[s * n2 + i];
     a.x += v.x;
     a.y += v.y;
-    a.z += v.z;
-    a.w += v.w;
   }
   dw[i] = a;
 }
 
-// The kernel for K, with its rows a step.
-static const void* wgrad8_fn(int K) {
-  if (K <= 7) return reinterpret_cast<const void*>(&wgrad8_kernel<1, 1, 2, true>);
-  if (K <= 15) return reinterpret_cast<const void*>(&wgrad8_kernel<1, 2, 2, false>);
-  if (K <= 23) return reinterpret_cast<const void*>(&wgrad8_kernel<2, 3, 1, false>);
-  return reinterpret_cast<const void*>(&wgrad8_kernel<2, 4, 1, false>);
+// The kernel for K and a tile of columns, its rows a step and its shared memory.
+struct Wgrad8Kernel {
+  const void* fn;
+  int rows, ctas, smem;  // ctas: an SM, by registers
+};
+template <int MT, int NT, int ROWS, bool PACK, int TW>
+static Wgrad8Kernel wgrad8_kernel_of(int K) {
+  return {reinterpret_cast<const void*>(&wgrad8_kernel<MT, NT, ROWS, PACK, TW>), ROWS,
+          kWgCtas<MT, PACK>, Wgrad8<MT, NT, ROWS, PACK, TW>::smem(K)};
 }
-static int wgrad8_rows(int K) { return K <= 15 ? 2 : 1; }
-
-static int wgrad8_smem(const Wgrad8Params& p) {
-  return 4 * (2 * wgrad8_rows(p.K) * 2 * (kWgChannels * p.xp + 16) + p.ring * (kWgChannels * p.dp + 4));
+template <int TW>
+static Wgrad8Kernel wgrad8_kernel_for(int K) {
+  if (K <= 7) return wgrad8_kernel_of<1, 1, 2, true, TW>(K);
+  if (K <= 15) return wgrad8_kernel_of<1, 2, 2, false, TW>(K);
+  if (K <= 23) return wgrad8_kernel_of<2, 3, 1, false, TW>(K);
+  return wgrad8_kernel_of<2, 4, 1, false, TW>(K);
+}
+static Wgrad8Kernel wgrad8_kernel_for(int K, int tw) {
+  switch (tw) {
+    case 16: return wgrad8_kernel_for<16>(K);
+    case 32: return wgrad8_kernel_for<32>(K);
+    case 48: return wgrad8_kernel_for<48>(K);
+    default: return wgrad8_kernel_for<64>(K);
+  }
 }
 
 static int wgrad8_plan(int64_t B, int64_t H, int64_t W, int64_t C, int K, Wgrad8Params* p) {
   if (K < 1 || K > 31 || (K % 2) == 0 || B < 0 || H < 1 || W < 1 || C < 8 || (C % 8) != 0) return DWB_ERR_BAD_SHAPE;
   if (B > (1 << 30) || H > (1 << 24) || W > (1 << 21) || C > (1 << 20) || B * H > (1LL << 30)) return DWB_ERR_BAD_SHAPE;
-  const int rows = wgrad8_rows(K);
   p->B = static_cast<int>(B);
   p->H = static_cast<int>(H);
   p->W = static_cast<int>(W);
@@ -363,16 +461,17 @@ static int wgrad8_plan(int64_t B, int64_t H, int64_t W, int64_t C, int K, Wgrad8
   p->col_tiles = (p->W + kWgTile - 1) / kWgTile;
   p->tw = ((p->W + p->col_tiles - 1) / p->col_tiles + 15) / 16 * 16;  // even tiles: W = 65 is 48 + 17, not 64 + 1
   p->col_tiles = (p->W + p->tw - 1) / p->tw;
-  p->unit_rows = (p->H + rows - 1) / rows;
+  const Wgrad8Kernel k = wgrad8_kernel_for(K, p->tw);
+  p->unit_rows = (p->H + k.rows - 1) / k.rows;
   p->units = p->B * p->unit_rows;
-  p->xp = (p->tw + (K <= 7 ? 8 : K <= 15 ? 16 : 32)) / 2 | 1;
-  p->dp = (p->tw / 2) | 1;
-  p->ring = K - 1 + 2 * rows;
-  // a chain of at most kChain products, and CTAs for every SM, but not ranges shorter than the rows of dy
-  // that a range has to bring in before its first product
+  // As many ranges as CTAs run at once (a range more on some SMs would double the time), but none shorter than a
+  // third of the rows of dy that it has to bring in before its first product, and none whose chains get too long.
   const long long base = (C + kWgChannels - 1) / kWgChannels * p->col_tiles;
-  long long per = (static_cast<long long>(p->units) * base + 2LL * kSmCount - 1) / (2LL * kSmCount);
-  const long long least = (K - 1) / (2 * rows) > 1 ? (K - 1) / (2 * rows) : 1, most = kChain / (p->tw / 16);
+  const int room = 228 * 1024 / (k.smem + 1024);
+  const long long at_once = static_cast<long long>(room < k.ctas ? room : k.ctas) * kSmCount;
+  const long long ranges = at_once / base > 1 ? at_once / base : 1;
+  long long per = (p->units + ranges - 1) / ranges;
+  const long long least = (K - 1) / (3 * k.rows) > 1 ? (K - 1) / (3 * k.rows) : 1, most = kChain / (p->tw / 16);
   per = per < least ? least : per;
   per = per > most ? most : per;
   p->per_chunk = static_cast<int>(per);
@@ -422,20 +521,19 @@ extern "C" int dwb_conv2d_nhwc_bwd_weight_act8(const void* codes, const void* sc
   }
   float* part = static_cast<float*>(workspace);
   void* a1[] = {&codes, &scales, &dy, &part, &p};
-  const void* fn = wgrad8_fn(K);
-  const int smem = wgrad8_smem(p);
-  cudaError_t e = allow_large_cta(fn);
+  const Wgrad8Kernel k = wgrad8_kernel_for(K, p.tw);
+  cudaError_t e = allow_large_cta(k.fn);
   if (e == cudaSuccess)
-    e = launch_kernel(fn, dim3(static_cast<unsigned>((C + kWgChannels - 1) / kWgChannels), p.chunks, p.col_tiles),
-                      dim3(kWgThreads), a1, smem, st);
+    e = launch_kernel(k.fn, dim3(static_cast<unsigned>((C + kWgChannels - 1) / kWgChannels), p.chunks, p.col_tiles),
+                      dim3(kWgThreads), a1, k.smem, st);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
     return record_cuda_failure("wgrad8_kernel", e);
   }
-  long long n4 = static_cast<long long>(K) * K * C / 4;
+  long long n2 = static_cast<long long>(K) * K * C / 2;
   int slices = p.chunks * p.col_tiles;
-  void* a2[] = {&part, &dw, &n4, &slices};
-  e = launch_kernel(reinterpret_cast<const void*>(&wgrad8_reduce_kernel), dim3(static_cast<unsigned>((n4 + 255) / 256)),
+  void* a2[] = {&part, &dw, &n2, &slices};
+  e = launch_kernel(reinterpret_cast<const void*>(&wgrad8_reduce_kernel), dim3(static_cast<unsigned>((n2 + 255) / 256)),
                     dim3(256), a2, 0, st);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
