@@ -26,23 +26,19 @@ namespace dwb {
 
 enum : int { kActSilu = 3 };  // after kActNone, kActRelu, kActGelu
 
-// erfc(a / sqrt 2) / 2 = exp(-a^2 / 2) * poly(t) t for a = |u|, t = 1 / (1 + p a): Abramowitz & Stegun
-// 7.1.26 (|error| <= 1.5e-7), as gelu_erf2 uses it.  Returns -a, poly(t), t and the exponential.
-struct HalfErfc {
-  f32x2 na, poly, t, e;
-};
-__device__ __forceinline__ HalfErfc half_erfc2(f32x2 u) {
-  HalfErfc r;
-  r.na = u | 0x8000000080000000ull;
-  const float2 d = bits_f2(fma2(r.na, splat2(-0.3275911f * 0.70710678118654752f), splat2(1.0f)));
-  r.t = f2_bits(make_float2(rcp_approx(d.x), rcp_approx(d.y)));
-  f32x2 q = fma2(splat2(0.5f * 1.061405429f), r.t, splat2(0.5f * -1.453152027f));
-  q = fma2(q, r.t, splat2(0.5f * 1.421413741f));
-  q = fma2(q, r.t, splat2(0.5f * -0.284496736f));
-  r.poly = fma2(q, r.t, splat2(0.5f * 0.254829592f));
-  const float2 x = bits_f2(fmul2(fmul2(u, splat2(-0.5f * 1.4426950408889634f)), u));
-  r.e = f2_bits(make_float2(ex2_approx(x.x), ex2_approx(x.y)));
-  return r;
+// Q(a) = erfc(a / sqrt 2) / 2 for a >= 0 as 2^P(a): log2 Q is so smooth that a polynomial of degree 8 has |Q| to
+// 6e-8 and a Q to 3.5e-8 (a weighted least-squares fit on [0, 5.5], reweighted towards its largest error); further
+// out P goes on falling and a Q stays below 1e-7.  One special-function operation a value.
+__device__ __forceinline__ f32x2 normal_tail2(f32x2 a) {
+  f32x2 p = fma2(splat2(-2.0400157e-06f), a, splat2(2.9838166e-05f));
+  p = fma2(p, a, splat2(-0.00014074291f));
+  p = fma2(p, a, splat2(-0.00024707115f));
+  p = fma2(p, a, splat2(0.0072080679f));
+  p = fma2(p, a, splat2(-0.0525972135f));
+  p = fma2(p, a, splat2(-0.459174216f));
+  p = fma2(p, a, splat2(-1.15110946f));
+  const float2 e = bits_f2(fma2(p, a, splat2(-0.99999988f)));
+  return f2_bits(make_float2(ex2_approx(e.x), ex2_approx(e.y)));
 }
 
 template <int ACT>
@@ -51,11 +47,10 @@ __device__ __forceinline__ f32x2 act_value2(f32x2 u) {
     const float2 f = bits_f2(u);  // a comparison, not fmaxf: NaN stays NaN
     return f2_bits(make_float2(f.x < 0.0f ? 0.0f : f.x, f.y < 0.0f ? 0.0f : f.y));
   } else if constexpr (ACT == kActGelu) {
-    // u Phi(u) = max(u, 0) - |u| erfc(|u| / sqrt 2) / 2, on both sides of 0: no selection
-    const HalfErfc h = half_erfc2(u);
+    // u Phi(u) = max(u, 0) - |u| Q(|u|) on both sides of 0: no selection
     const float2 f = bits_f2(u);
-    const f32x2 lost = fmul2(fmul2(h.poly, h.t), h.e);
-    return fma2(h.na, lost, f2_bits(make_float2(fmaxf(f.x, 0.0f), fmaxf(f.y, 0.0f))));
+    return fma2(u | 0x8000000080000000ull, normal_tail2(u & 0x7fffffff7fffffffull),
+                f2_bits(make_float2(fmaxf(f.x, 0.0f), fmaxf(f.y, 0.0f))));
   } else if constexpr (ACT == kActSilu) {
     const float2 e = bits_f2(fmul2(u, splat2(-1.4426950408889634f)));
     const f32x2 d = fma2(f2_bits(make_float2(ex2_approx(e.x), ex2_approx(e.y))), splat2(1.0f), splat2(1.0f));
@@ -73,12 +68,20 @@ __device__ __forceinline__ f32x2 act_slope2(f32x2 u) {
     const float2 f = bits_f2(u);
     return f2_bits(make_float2(f.x > 0.0f ? 1.0f : 0.0f, f.y > 0.0f ? 1.0f : 0.0f));
   } else if constexpr (ACT == kActGelu) {
-    // Phi(u) + u phi(u) with k = erfc(|u| / sqrt 2) / 2 - |u| phi(u) is k below 0 and 1 - k above:
-    // 1/2 plus k - 1/2 with its sign turned where u is positive.  phi has the exponential that erfc has.
-    const HalfErfc h = half_erfc2(u);
-    const f32x2 k = fma2(h.poly, h.t, fmul2(h.na, splat2(0.3989422804014327f)));
+    // Phi(u) + u phi(u).  With k = erfc(|u| / sqrt 2) / 2 - |u| phi(u) it is k below 0 and 1 - k above: 1/2 plus
+    // k - 1/2 with its sign turned where u is positive.  erfc from Abramowitz & Stegun 7.1.26, as gelu_erf2 has it
+    // (|error| <= 1.5e-7): exp(-u^2 / 2) poly(t) t, t = 1 / (1 + p |u|), whose exponential phi shares.
+    const f32x2 na = u | 0x8000000080000000ull;
+    const float2 d = bits_f2(fma2(na, splat2(-0.3275911f * 0.70710678118654752f), splat2(1.0f)));
+    const f32x2 t = f2_bits(make_float2(rcp_approx(d.x), rcp_approx(d.y)));
+    f32x2 poly = fma2(splat2(0.5f * 1.061405429f), t, splat2(0.5f * -1.453152027f));
+    poly = fma2(poly, t, splat2(0.5f * 1.421413741f));
+    poly = fma2(poly, t, splat2(0.5f * -0.284496736f));
+    poly = fma2(poly, t, splat2(0.5f * 0.254829592f));
+    const f32x2 k = fma2(poly, t, fmul2(na, splat2(0.3989422804014327f)));
+    const float2 x = bits_f2(fmul2(fmul2(u, splat2(-0.5f * 1.4426950408889634f)), u));
     f32x2 r = splat2(0.5f);
-    fadd2(r, fma2(k, h.e, splat2(-0.5f)) ^ (~u & 0x8000000080000000ull));
+    fadd2(r, fma2(k, f2_bits(make_float2(ex2_approx(x.x), ex2_approx(x.y))), splat2(-0.5f)) ^ (~u & 0x8000000080000000ull));
     return r;
   } else if constexpr (ACT == kActSilu) {
     const float2 e = bits_f2(fmul2(u, splat2(-1.4426950408889634f)));
