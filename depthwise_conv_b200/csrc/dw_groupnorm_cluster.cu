@@ -419,8 +419,7 @@ static int gcd_int(int a, int b) { return b == 0 ? a : gcd_int(b, a % b); }
 
 static int gn_sub(const GnShape& s) { return s.Cg % 8 == 0 ? 8 : s.Cg % 4 == 0 ? 4 : 1; }
 
-static bool gn_resident_fill(const GnShape& s, GnPass pass, int slab, int cluster, int limit, GnResident* p) {
-  const int most = kGnThreads;
+static bool gn_resident_fill(const GnShape& s, GnPass pass, int slab, int cluster, int most, int limit, GnResident* p) {
   // a thread's 8 (forward) or 4 channels of a pixel
   const int bytes = pass == GnPass::kForward ? 16 : pass == GnPass::kBackward16 ? 24 : 20;
   p->slab = slab;
@@ -448,7 +447,9 @@ static bool gn_resident_fill(const GnShape& s, GnPass pass, int slab, int cluste
 }
 
 // The rule.  A unit's pixels are shared by the fewest CTAs (1 to 8) that hold them four to an SM, else two to an SM:
-// 32x32x1536, 32 groups, B = 16, forward: 33 us with 4 CTAs of 49 KB, 35 with 2 of 98 KB, 40 with 8 of 25 KB.  What
+// 32x32x1536, 32 groups, B = 16, forward: 32 us with 4 CTAs of 49 KB, 34 with 2 of 98 KB, 39 with 8 of 25 KB and as many
+// threads.  With as many units as SMs, 8 CTAs of half the threads, eight to an SM, where they hold a unit: 31.5 us there,
+// 92.7 against 97.5 us at 56x56x1024, B = 32, 47.0 against 50.8 us with a checkpoint at 56x56x128, B = 64.  What
 // needs more goes to the streaming passes (one group over 32x32x768, B = 8: 8 CTAs of 196 KB 14.2 us, 16 of 98 KB
 // 11.4 us, streaming 11.2 us).
 // Backward, the streaming passes are faster from about 7 CTAs an SM on: 32x32x1536 with B = 2 / 4 / 8 / 16, resident
@@ -456,21 +457,25 @@ static bool gn_resident_fill(const GnShape& s, GnPass pass, int slab, int cluste
 // little that four CTAs an SM bring along.  Forward the resident kernels stay ahead at every size (56x56x1024,
 // B = 32: 97 against 119 us): they move two thirds of the data.
 bool gn_resident_plan(const GnShape& s, GnPass pass, GnResident* p) {
-  // shared memory of four and two CTAs an SM: 228 KB less 1 KB each
-  constexpr int kFour = 56 * 1024, kTwo = 113 * 1024;
+  // shared memory of eight, four and two CTAs an SM: 228 KB less 1 KB each
+  constexpr int kEight = 27 * 1024 + 512, kFour = 56 * 1024, kTwo = 113 * 1024;
   // whole groups; forward: whole blocks of a checkpoint (with and without one: the same plan, the same bits), backward:
   // whole vectors and, where it can be, 64 bytes of a pixel
   const int align = pass == GnPass::kForward ? kAct8Block : 8;
   const long long unit_ll = static_cast<long long>(s.Cg) / gcd_int(s.Cg, align) * align;
   int unit = unit_ll < s.C ? static_cast<int>(unit_ll) : s.C;
   for (int k = unit; unit < 32 && unit < s.C;) unit = unit + k < s.C ? unit + k : s.C;
+  // many units: clusters of 8 small CTAs, eight to an SM, that are seldom in the same phase
+  if (pass == GnPass::kForward && gn_resident_fill(s, pass, unit, 8, kGnThreads / 2, kEight, p) &&
+      static_cast<long long>(s.B) * p->slabs >= kSmCount)
+    return true;
   for (int limit : {kFour, kTwo})
     for (int cluster = 1; cluster <= 8; cluster *= 2)
-      if (gn_resident_fill(s, pass, unit, cluster, limit, p)) {
+      if (gn_resident_fill(s, pass, unit, cluster, kGnThreads, limit, p)) {
         // few clusters: more CTAs share a sample, as long as each thread keeps a few pixels
         GnResident wider;
         while (static_cast<long long>(s.B) * p->slabs * p->cluster < 2 * kSmCount && p->cluster < 8 && p->iters > 4 &&
-               gn_resident_fill(s, pass, unit, p->cluster * 2, limit, &wider))
+               gn_resident_fill(s, pass, unit, p->cluster * 2, kGnThreads, limit, &wider))
           *p = wider;
         return pass == GnPass::kForward || static_cast<long long>(s.B) * p->slabs * p->cluster <= 7 * kSmCount;
       }

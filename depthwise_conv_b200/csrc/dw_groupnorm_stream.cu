@@ -69,6 +69,14 @@ constexpr int kForwardRing = kForwardBatches * kBatch * kThreads * 16;
 constexpr int kBackwardRing = kBackwardBatches * kBatch * kThreads * 16;  // of dy
 constexpr int kFinMost = kApplyLanes * 8 + 1;  // groups that 128 channels can belong to
 
+// The first launch of a call waits for the kernel before it, which may make its inputs.  The others read nothing but
+// what that launch could read, and the entries of the launch before them: they begin to load first (q.early), while
+// that launch's last CTAs run, and wait for it then.
+__device__ __forceinline__ void begin_after_previous() {
+  griddep_wait();
+  griddep_launch_dependents();
+}
+
 // Place of a thread in a tile.
 struct StreamThread {
   int lane_row, vec, r0, rows;
@@ -115,14 +123,15 @@ __device__ __forceinline__ void stats_cta(const T* __restrict__ x, float2* __res
   const StreamThread t(q, q.lanes, q.lane_mul, q.rows, chunk, static_cast<int>(s.P));
   const int c = tile.c0 + t.vec * 8, tid = threadIdx.x;
   const int n = t.vec * 8 < tile.width ? t.mine(q.rl) : 0;
+  const T* p = x + (static_cast<long long>(sample) * s.P + t.r0 + t.lane_row) * s.C + c;
+  const long long step = static_cast<long long>(q.rl) * s.C;
+  Stream<16, kForwardBatches> in(ring, p, step * sizeof(T), n);
+  for (int k = 0; k < kForwardBatches; ++k) {
+    in.issue(k);
+    cp_async_commit();
+  }
+  if (q.early) begin_after_previous();
   if (n) {
-    const T* p = x + (static_cast<long long>(sample) * s.P + t.r0 + t.lane_row) * s.C + c;
-    const long long step = static_cast<long long>(q.rl) * s.C;
-    Stream<16, kForwardBatches> in(ring, p, step * sizeof(T), n);
-    for (int k = 0; k < kForwardBatches; ++k) {
-      in.issue(k);
-      cp_async_commit();
-    }
     GnSums sums;
     f32x2 f[4];
     wait_batch<kForwardBatches>();
@@ -208,6 +217,7 @@ __device__ __forceinline__ void apply_cta(const T* __restrict__ x, const void* _
     in.issue(k);
     cp_async_commit();
   }
+  if (q.early) begin_after_previous();
   f32x2 w[4], b[4], m[kParts];
   if (active) gn_load_params<T>(weight, bias, c, s, w, b);
   // the CTA of a chunk's first rows and of a group's first channels writes the group's mean and rstd
@@ -274,8 +284,7 @@ __global__ void __launch_bounds__(kThreads, 3)
   extern __shared__ __align__(16) unsigned char smem[];
   unsigned char* const ring = smem;
   float2* const ent = reinterpret_cast<float2*>(smem + kForwardRing);
-  griddep_wait();
-  griddep_launch_dependents();
+  if (!q.early) begin_after_previous();
   unsigned work;
   if (second_pass(q, blockIdx.x, &work)) {
     const unsigned per = q.apply_tiles * q.apply_chunks, sample = work / per;
@@ -353,27 +362,27 @@ __device__ __forceinline__ void grad_sums_cta(const T* __restrict__ dy, const vo
   const StreamThread t(q, q.lanes, q.lane_mul, q.rows, chunk, static_cast<int>(s.P));
   const int c = tile.c0 + t.vec * 8, tid = threadIdx.x;
   const int n = t.vec * 8 < tile.width ? t.mine(q.rl) : 0;
+  using In = SavedInput<T, SRC8, SUB>;
+  const long long pixel = static_cast<long long>(sample) * s.P + t.r0 + t.lane_row;
+  const long long sblocks = (s.C + kAct8Block - 1) / kAct8Block, sstep = q.rl * sblocks;
+  const long long step = static_cast<long long>(q.rl) * s.C, first = pixel * s.C + c;
+  Stream<16, kBackwardBatches> grad(ring, dy + first, step * sizeof(T), n);
+  Stream<In::kBytes, kBackwardBatches> saved(ring + kBackwardRing, static_cast<const unsigned char*>(src) + first * (SRC8 ? 1 : 2),
+                                             step * (SRC8 ? 1 : 2), n);
+  for (int k = 0; k < kBackwardBatches; ++k) {
+    grad.issue(k);
+    saved.issue(k);
+    cp_async_commit();
+  }
+  if (q.early) begin_after_previous();
   f32x2 sg[4], sx[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) sg[j] = sx[j] = f32x2_zero();
   if (n) {
-    using In = SavedInput<T, SRC8, SUB>;
-    f32x2 w[4], b[4];
-    In in;
-    const long long pixel = static_cast<long long>(sample) * s.P + t.r0 + t.lane_row;
-    const long long sblocks = (s.C + kAct8Block - 1) / kAct8Block, sstep = q.rl * sblocks;
-    const long long step = static_cast<long long>(q.rl) * s.C;
-    const long long first = pixel * s.C + c;
-    Stream<16, kBackwardBatches> grad(ring, dy + first, step * sizeof(T), n);
-    Stream<In::kBytes, kBackwardBatches> saved(ring + kBackwardRing, static_cast<const unsigned char*>(src) + first * (SRC8 ? 1 : 2),
-                             step * (SRC8 ? 1 : 2), n);
-    for (int k = 0; k < kBackwardBatches; ++k) {
-      grad.issue(k);
-      saved.issue(k);
-      cp_async_commit();
-    }
     Exponents ex{scales + (SRC8 ? pixel * sblocks + c / kAct8Block : 0), sstep, SRC8 ? n : 0};
     if constexpr (SRC8) ex.fetch();
+    f32x2 w[4], b[4];
+    In in;
     gn_load_params<T>(weight, bias, c, s, w, b);
     in.load_stats(mean, rstd, s, sample, c);
     int batch = 0;
@@ -461,6 +470,7 @@ __device__ __forceinline__ void grad_apply_cta(const T* __restrict__ dy, const v
     saved.issue(k);
     cp_async_commit();
   }
+  if (q.early) begin_after_previous();
   Exponents ex{scales + (SRC8 ? pixel * sblocks + c / kAct8Block : 0), sstep, SRC8 ? n : 0};
   if constexpr (SRC8) ex.fetch();
   f32x2 w[4], b[4];
@@ -527,8 +537,7 @@ __global__ void __launch_bounds__(kThreads, 3)
   extern __shared__ __align__(16) unsigned char smem[];
   unsigned char* const ring = smem;
   float2* const fin = reinterpret_cast<float2*>(smem + kBackwardRing * (SRC8 ? 3 : 4) / 2);
-  griddep_wait();
-  griddep_launch_dependents();
+  if (!q.early) begin_after_previous();
   unsigned work;
   if (second_pass(q, blockIdx.x, &work)) {
     const unsigned per = q.apply_tiles * q.apply_chunks, sample = work / per;
@@ -596,6 +605,7 @@ bool gn_stream_plan(const GnShape& s, int bytes_per_value, GnStream* q) {
               &q->apply_chunks);
   q->first_sample = q->second_sample = 0;
   q->first_ctas = q->second_ctas = 0;
+  q->early = 0;
   // CTAs of a launch: grid x
   const long long a = static_cast<long long>(q->tiles) * q->chunks * q->samples;
   const long long b = static_cast<long long>(q->apply_tiles) * q->apply_chunks * q->samples;
@@ -611,6 +621,7 @@ static int stream_groups(const GnShape& s, GnStream q, Launch launch) {
     const int first = left <= 0 ? 0 : left < q.samples ? left : q.samples;
     q.second_sample = done < 0 ? 0 : done;
     q.first_sample = next;
+    q.early = done >= 0;
     q.second_ctas = static_cast<unsigned>(second) * q.apply_tiles * q.apply_chunks;
     q.first_ctas = static_cast<unsigned>(first) * q.tiles * q.chunks;
     const int rc = launch(q, dim3(q.first_ctas + q.second_ctas));

@@ -26,6 +26,7 @@ struct GnStream {
   // one launch: what it does
   int first_sample, second_sample;
   unsigned first_ctas, second_ctas;
+  int early;                  // its inputs are ready whatever the launch before it does
 };
 
 // bytes_per_value: what the two passes read of a value.  False: too many CTAs for a grid.
