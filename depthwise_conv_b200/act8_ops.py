@@ -12,8 +12,8 @@ it came from.  A block that holds an infinity or a NaN reads back as NaN.
 ``codes``: int8, the activation's shape, channels_last.  ``scales``: uint8
 [B, H, W, ceil(C / 32)], contiguous.
 
-Everything here validates tensors and calls the C ABI on the current stream;
-there is no CPU or PyTorch fallback.  The reference's ops are inference-only
+Everything here checks its tensors and calls the C ABI on the current stream
+(through the compiled module ``_train_bind``); there is no CPU or PyTorch fallback.  The reference's ops are inference-only
 (convmixer/kernels/depthwise_torch_ops.py:157-159) and keep nothing.
 
 Torch ops:
@@ -28,93 +28,51 @@ Torch ops:
 """
 from __future__ import annotations
 
-import ctypes
-import functools
-
 import torch
 
 from . import _lib, dw_ops
-from .dw_ops import _DeviceGuard
 
 BLOCK = 32
 DTYPE_CODES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
+_bind = None
 
-def launch(name: str, where: str, device: torch.device, *args) -> None:
-    """Call an entry point with the device's current stream as its last argument, that device being current."""
-    index = device.index
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch._C._cuda_getDevice() == index:
-        _lib.call(name, *args, stream)
-    else:
-        with _DeviceGuard(device):
-            _lib.call(name, *args, stream)
+
+def bind():
+    """The compiled host side of the training ops (checks, allocation, the C ABI's call); loaded once."""
+    global _bind
+    if _bind is None:
+        _lib.load()
+        try:
+            from . import _train_bind
+        except ImportError as e:
+            raise RuntimeError("depthwise_conv_b200: _train_bind.so is missing or does not load; build it with "
+                               "`python -m depthwise_conv_b200.csrc.build` (there is no fallback)") from e
+        _bind = _train_bind
+    return _bind
+
+
+def after_launch(t: torch.Tensor, where: str) -> None:
+    """The opt-in check of the device error word behind a launch on the tensor's device."""
     if _lib.check_device_error_enabled():
-        with _DeviceGuard(device):
-            _lib.after_launch(stream, where)
-
-
-def check_nhwc(x: torch.Tensor, name: str = "input") -> int:
-    """A channels_last float16 or bfloat16 CUDA tensor [B, C, H, W] with C % 8 == 0; returns its dwb_dtype."""
-    if not x.is_cuda:
-        raise RuntimeError(f"{name} must be a CUDA tensor (the engine has no CPU path)")
-    code = DTYPE_CODES.get(x.dtype)
-    if code is None:
-        raise RuntimeError(f"{name} must be float16 or bfloat16, got {x.dtype}")
-    if x.dim() != 4:
-        raise RuntimeError(f"{name} must be 4-D [B, C, H, W], got {tuple(x.shape)}")
-    if not x.is_contiguous(memory_format=torch.channels_last):
-        raise RuntimeError(f"{name} must be channels_last")
-    return code
-
-
-def check_checkpoint(codes: torch.Tensor, scales: torch.Tensor) -> None:
-    if not codes.is_cuda or codes.dtype != torch.int8 or codes.dim() != 4:
-        raise RuntimeError(f"codes must be a 4-D int8 CUDA tensor, got {codes.dtype} {tuple(codes.shape)} on {codes.device}")
-    if not codes.is_contiguous(memory_format=torch.channels_last):
-        raise RuntimeError("codes must be channels_last")
-    B, C, H, W = codes.shape
-    want = (B, H, W, -(-C // BLOCK))
-    if scales.dtype != torch.uint8 or tuple(scales.shape) != want or not scales.is_contiguous():
-        raise RuntimeError(f"scales must be contiguous uint8 {want}, got {scales.dtype} {tuple(scales.shape)}")
-    if scales.device != codes.device:
-        raise RuntimeError(f"scales is on {scales.device}, codes on {codes.device}")
-
-
-def empty_checkpoint(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """Unwritten codes and scales for an activation like ``x``."""
-    B, C, H, W = x.shape
-    codes = torch.empty_like(x, dtype=torch.int8)  # keeps the strides
-    return codes, x.new_empty((B, H, W, -(-C // BLOCK)), dtype=torch.uint8)
+        with dw_ops._DeviceGuard(t.device):
+            _lib.after_launch(dw_ops._stream_of(t), where)
 
 
 def act8_encode(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(codes, scales) of a channels_last float16 or bfloat16 activation."""
-    dtype = check_nhwc(x)
-    B, C, H, W = x.shape
-    codes, scales = empty_checkpoint(x)
-    launch("dwb_act8_encode_nhwc", "depthwise act8_encode", x.device, x.data_ptr(), codes.data_ptr(), scales.data_ptr(),
-           B * H * W, C, dtype)
-    return codes, scales
+    kept = bind().act8_encode(x)
+    after_launch(x, "depthwise act8_encode")
+    return kept
 
 
 def act8_decode(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.float16) -> torch.Tensor:
     """The activation a checkpoint stands for, channels_last; ``dtype``: the type it was made from."""
-    check_checkpoint(codes, scales)
     if dtype not in DTYPE_CODES:
         raise RuntimeError(f"dtype must be float16 or bfloat16, got {dtype}")
-    B, C, H, W = codes.shape
-    x = torch.empty_like(codes, dtype=dtype)
-    launch("dwb_act8_decode_nhwc", "depthwise act8_decode", codes.device, codes.data_ptr(), scales.data_ptr(), x.data_ptr(),
-           B * H * W, C, DTYPE_CODES[dtype])
+    x = bind().act8_decode(codes, scales, DTYPE_CODES[dtype])
+    after_launch(x, "depthwise act8_decode")
     return x
-
-
-@functools.lru_cache(maxsize=1024)
-def _wgrad_workspace_bytes(B: int, H: int, W: int, C: int, K: int) -> int:
-    n = ctypes.c_int64(0)
-    _lib.call("dwb_conv2d_nhwc_bwd_weight_act8_workspace", B, H, W, C, K, ctypes.byref(n))
-    return n.value
 
 
 def conv2d_nhwc_backward_weight_act8(codes: torch.Tensor, scales: torch.Tensor, dy: torch.Tensor, K: int) -> torch.Tensor:
@@ -122,20 +80,15 @@ def conv2d_nhwc_backward_weight_act8(codes: torch.Tensor, scales: torch.Tensor, 
 
     The sums have a fixed order: the same bits on every call.  An infinity or a NaN
     in ``dy`` or the checkpoint may spread to every tap of its channel."""
-    check_checkpoint(codes, scales)
-    dw_ops.check_input(dy, "grad_output")
-    if dy.shape != codes.shape:
-        raise RuntimeError(f"grad_output shape {tuple(dy.shape)} != checkpoint shape {tuple(codes.shape)}")
-    if dy.device != codes.device:
-        raise RuntimeError(f"grad_output is on {dy.device}, checkpoint on {codes.device}")
-    B, C, H, W = dy.shape
-    K = int(K)
-    nbytes = _wgrad_workspace_bytes(B, H, W, C, K)
-    dw = dy.new_empty((K, K, C), dtype=torch.float32)
-    ws = dy.new_empty((max(16, nbytes),), dtype=torch.uint8)
-    launch("dwb_conv2d_nhwc_bwd_weight_act8", "depthwise conv2d_nhwc weight gradient from a checkpoint", dy.device,
-           codes.data_ptr(), scales.data_ptr(), dy.data_ptr(), dw.data_ptr(), ws.data_ptr(), nbytes, B, H, W, C, K)
+    dw = bind().backward_weight_act8(codes, scales, dy, int(K))
+    after_launch(dw, "depthwise conv2d_nhwc weight gradient from a checkpoint")
     return dw
+
+
+def empty_checkpoint(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Unwritten codes and scales for an activation like ``x`` (the fake impls' outputs)."""
+    B, C, H, W = x.shape
+    return torch.empty_like(x, dtype=torch.int8), x.new_empty((B, H, W, -(-C // BLOCK)), dtype=torch.uint8)
 
 
 def conv2d_nhwc_act8(x: torch.Tensor, w: torch.Tensor, bias=None) -> torch.Tensor:

@@ -4,7 +4,8 @@ Compiles every ``*.cu`` in this directory with nvcc
 (``-gencode arch=compute_100a,code=sm_100a``) and the planner with g++, in
 parallel, into ``depthwise_conv_b200/_build/``, then links the shared library
 into the package directory.  An object is rebuilt only when its source or a
-header that it includes is newer.  The library depends on the CUDA runtime only (no torch).
+header that it includes is newer.  The library depends on the CUDA runtime only (no torch);
+the training ops' host side, ``_train_bind.so``, is a Python module over PyTorch and it.
 
     python -m depthwise_conv_b200.csrc.build        # or: python build.py
     python -m depthwise_conv_b200.csrc.build --regcaps   # regenerate dw_regcaps.inc first
@@ -33,6 +34,8 @@ PKG = os.path.dirname(HERE)
 ROOT = os.path.dirname(PKG)
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libdwconv_b200.so")
+BIND_SRC = os.path.join(HERE, "bind", "train_bind.cpp")
+BIND = os.path.join(PKG, "_train_bind.so")
 INCLUDE = os.path.join(ROOT, "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -100,7 +103,30 @@ def build(verbose: bool = False, jobs: int | None = None) -> str:
             raise RuntimeError(f"link failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
         if verbose:
             print(f"linked {LIB}")
+    build_bind(verbose)
     return LIB
+
+
+def build_bind(verbose: bool = False) -> str:
+    """Compile the training ops' host side (a Python module over PyTorch and the library); returns its path."""
+    if os.path.exists(BIND) and os.path.getmtime(BIND) >= _inputs_mtime(BIND_SRC):
+        return BIND
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    inc = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(_cuda_home(), "include"), INCLUDE]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_API_INCLUDE_EXTENSION_H",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in inc), BIND_SRC, "-o", BIND,
+           f"-L{lib}", f"-L{PKG}", "-l:libdwconv_b200.so", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
+           "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+    if verbose:
+        print(f"built {BIND}")
+    return BIND
 
 
 REGCAPS = os.path.join(HERE, "dw_regcaps.inc")

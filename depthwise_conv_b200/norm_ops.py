@@ -12,8 +12,8 @@ input (``act8_ops``), from which the backward pass then works, so that the graph
 keeps 1 + 1/32 bytes a value instead of 2.  The statistics are those of the
 input itself in both cases.
 
-Everything here validates tensors and calls the C ABI on the current stream;
-there is no CPU or PyTorch fallback.  The reference's networks normalise with an
+Everything here checks its tensors and calls the C ABI on the current stream
+(through the compiled module ``_train_bind``); there is no CPU or PyTorch fallback.  The reference's networks normalise with an
 inference BatchNorm (convmixer/convmixer.py:93-127) and have no counterpart.
 
 Torch op (differentiable in input, weight and bias):
@@ -23,13 +23,10 @@ float32 [B, G]; without a checkpoint codes and scales are empty.
 """
 from __future__ import annotations
 
-import ctypes
-import functools
-
 import torch
 
 from . import _lib
-from .act8_ops import check_checkpoint, check_nhwc, empty_checkpoint, launch
+from .act8_ops import after_launch, bind, empty_checkpoint
 
 ACT_CODES = _lib.NORM_ACT_CODES
 
@@ -42,60 +39,14 @@ def _act_code(act) -> int:
     return int(act)
 
 
-def _check_param(name: str, t, like: torch.Tensor) -> None:
-    if not t.is_cuda or t.dtype not in (like.dtype, torch.float32) or t.shape != like.shape[1:2] or not t.is_contiguous():
-        raise RuntimeError(f"{name} must be a contiguous {like.dtype} or float32 CUDA tensor with {like.shape[1]} elements, "
-                           f"got {t.dtype} {tuple(t.shape)}")
-    if t.device != like.device:
-        raise RuntimeError(f"{name} is on {t.device}, input on {like.device}")
-
-
-def _check_params(weight, bias, like: torch.Tensor, dtype_code: int):
-    """Pointers of the parameter vectors and their dwb_dtype."""
-    wp = bp = None
-    if weight is not None:
-        _check_param("weight", weight, like)
-        wp = weight.data_ptr()
-    if bias is not None:
-        _check_param("bias", bias, like)
-        bp = bias.data_ptr()
-        if weight is not None and weight.dtype != bias.dtype:
-            raise RuntimeError(f"weight and bias must have one type, got {weight.dtype} and {bias.dtype}")
-    first = bias if weight is None else weight
-    return wp, bp, _lib.F32 if first is not None and first.dtype == torch.float32 else dtype_code
-
-
-@functools.lru_cache(maxsize=1024)
-def _workspace_bytes(B: int, H: int, W: int, C: int, G: int, backward: int) -> int:
-    n = ctypes.c_int64(0)
-    _lib.call("dwb_group_norm_act_workspace", B, H, W, C, G, backward, ctypes.byref(n))
-    return n.value
-
-
-def _workspace(x: torch.Tensor, B: int, H: int, W: int, C: int, G: int, backward: int):
-    n = _workspace_bytes(B, H, W, C, G, backward)
-    return (x.new_empty((n,), dtype=torch.uint8) if n else None), n
-
-
 def group_norm_act_forward(x: torch.Tensor, num_groups: int, weight=None, bias=None, eps: float = 1e-5,
                            act: int | str = 0, checkpoint: bool = False):
     """(y, mean, rstd), with ``checkpoint`` (y, mean, rstd, codes, scales).
 
     x: channels_last [B, C, H, W], float16 or bfloat16, C % 8 == 0; y like x; mean, rstd: float32 [B, num_groups]."""
-    dtype = check_nhwc(x)
-    B, C, H, W = x.shape
-    G, act_code = int(num_groups), _act_code(act)
-    wp, bp, param_dtype = _check_params(weight, bias, x, dtype)
-    ws, nbytes = _workspace(x, B, H, W, C, G, 0)
-    y = torch.empty_like(x)  # keeps the strides
-    mean = x.new_empty((B, G), dtype=torch.float32)
-    rstd = torch.empty_like(mean)
-    codes, scales = empty_checkpoint(x) if checkpoint else (None, None)
-    launch("dwb_group_norm_act_nhwc_fwd", "depthwise group_norm_act", x.device, x.data_ptr(), wp, bp, y.data_ptr(),
-           mean.data_ptr(), rstd.data_ptr(), codes.data_ptr() if checkpoint else None,
-           scales.data_ptr() if checkpoint else None, ws.data_ptr() if nbytes else None, nbytes, B, H, W, C, G, float(eps),
-           act_code, dtype, param_dtype)
-    return (y, mean, rstd, codes, scales) if checkpoint else (y, mean, rstd)
+    out = bind().group_norm_act_forward(x, num_groups, weight, bias, eps, _act_code(act), checkpoint)
+    after_launch(x, "depthwise group_norm_act")
+    return out
 
 
 def group_norm_act_backward(dy: torch.Tensor, saved, mean: torch.Tensor, rstd: torch.Tensor, num_groups: int,
@@ -103,33 +54,10 @@ def group_norm_act_backward(dy: torch.Tensor, saved, mean: torch.Tensor, rstd: t
     """(dx, dweight, dbias) of the forward pass; dweight, dbias in the parameters' type, None where there is none.
 
     ``saved``: the forward pass's input, or the (codes, scales) of its checkpoint."""
-    dtype = check_nhwc(dy, "grad_output")
-    B, C, H, W = dy.shape
-    G, act_code = int(num_groups), _act_code(act)
-    if isinstance(saved, torch.Tensor):
-        check_nhwc(saved, "saved input")
-        if saved.dtype != dy.dtype:
-            raise RuntimeError(f"saved input is {saved.dtype}, grad_output {dy.dtype}")
-        first, xp, qp, sp = saved, saved.data_ptr(), None, None
-    else:
-        codes, scales = saved
-        check_checkpoint(codes, scales)
-        first, xp, qp, sp = codes, None, codes.data_ptr(), scales.data_ptr()
-    if first.shape != dy.shape or first.device != dy.device:
-        raise RuntimeError("what was saved must match grad_output in shape and device")
-    wp, bp, param_dtype = _check_params(weight, bias, dy, dtype)
-    for name, t in (("mean", mean), ("rstd", rstd)):
-        if t.dtype != torch.float32 or t.shape != (B, G) or not t.is_contiguous() or t.device != dy.device:
-            raise RuntimeError(f"{name} must be a contiguous float32 tensor [{B}, {G}] on {dy.device}")
-    ws, nbytes = _workspace(dy, B, H, W, C, G, 1)
-    dx = torch.empty_like(dy)
-    dweight = torch.empty_like(weight) if weight is not None else None
-    dbias = torch.empty_like(bias) if bias is not None else None
-    launch("dwb_group_norm_act_nhwc_bwd", "depthwise group_norm_act gradient", dy.device, dy.data_ptr(), xp, qp, sp,
-           mean.data_ptr(), rstd.data_ptr(), wp, bp, dx.data_ptr(), dweight.data_ptr() if dweight is not None else None,
-           dbias.data_ptr() if dbias is not None else None, ws.data_ptr() if nbytes else None, nbytes, B, H, W, C, G,
-           act_code, dtype, param_dtype)
-    return dx, dweight, dbias
+    x, codes, scales = (saved, None, None) if isinstance(saved, torch.Tensor) else (None, *saved)
+    out = bind().group_norm_act_backward(dy, x, codes, scales, mean, rstd, num_groups, weight, bias, _act_code(act))
+    after_launch(dy, "depthwise group_norm_act gradient")
+    return out
 
 
 def group_norm_act(x: torch.Tensor, num_groups: int, weight=None, bias=None, eps: float = 1e-5, act: int | str = 0,
