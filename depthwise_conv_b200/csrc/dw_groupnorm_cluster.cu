@@ -448,8 +448,7 @@ static bool gn_resident_fill(const GnShape& s, GnPass pass, int slab, int cluste
 
 // The rule.  A unit's pixels are shared by the fewest CTAs (1 to 8) that hold them four to an SM, else two to an SM:
 // 32x32x1536, 32 groups, B = 16, forward: 32 us with 4 CTAs of 49 KB, 34 with 2 of 98 KB, 39 with 8 of 25 KB and as many
-// threads.  With as many units as SMs, 8 CTAs of half the threads, eight to an SM, where they hold a unit: 31.5 us there,
-// 92.7 against 97.5 us at 56x56x1024, B = 32, 47.0 against 50.8 us with a checkpoint at 56x56x128, B = 64.  What
+// threads.  Where that makes eight CTAs an SM or more, CTAs of half the threads, eight to an SM: 31.5 us there, 92.7 against 97.5 us at 56x56x1024, B = 32, 47.0 against 50.8 us with a checkpoint at 56x56x128, B = 64.  What
 // needs more goes to the streaming passes (one group over 32x32x768, B = 8: 8 CTAs of 196 KB 14.2 us, 16 of 98 KB
 // 11.4 us, streaming 11.2 us).
 // Backward, the streaming passes are faster from about 7 CTAs an SM on: 32x32x1536 with B = 2 / 4 / 8 / 16, resident
@@ -465,10 +464,13 @@ bool gn_resident_plan(const GnShape& s, GnPass pass, GnResident* p) {
   const long long unit_ll = static_cast<long long>(s.Cg) / gcd_int(s.Cg, align) * align;
   int unit = unit_ll < s.C ? static_cast<int>(unit_ll) : s.C;
   for (int k = unit; unit < 32 && unit < s.C;) unit = unit + k < s.C ? unit + k : s.C;
-  // many units: clusters of 8 small CTAs, eight to an SM, that are seldom in the same phase
-  if (pass == GnPass::kForward && gn_resident_fill(s, pass, unit, 8, kGnThreads / 2, kEight, p) &&
-      static_cast<long long>(s.B) * p->slabs >= kSmCount)
-    return true;
+  // many units: small CTAs, eight to an SM, that are seldom in the same phase
+  if (pass == GnPass::kForward)
+    for (int cluster = 1; cluster <= 8; cluster *= 2)
+      if (gn_resident_fill(s, pass, unit, cluster, kGnThreads / 2, kEight, p)) {
+        if (static_cast<long long>(s.B) * p->slabs * cluster < 8 * kSmCount) break;
+        return true;
+      }
   for (int limit : {kFour, kTwo})
     for (int cluster = 1; cluster <= 8; cluster *= 2)
       if (gn_resident_fill(s, pass, unit, cluster, kGnThreads, limit, p)) {

@@ -587,8 +587,10 @@ bool gn_stream_plan(const GnShape& s, int bytes_per_value, GnStream* q) {
   q->lanes = (q->tile + 7) / 8;
   q->lane_mul = 65536u / q->lanes + 1;  // exact for thread < 256
   q->rl = kThreads / q->lanes;
-  const int quads = (s.C + kAct8Block - 1) / kAct8Block * 4;
-  q->apply_lanes = quads < kApplyLanes ? quads : kApplyLanes;
+  // second pass: even tiles of whole checkpoint blocks (168 channels are 96 + 72, not 128 + 40)
+  const int blocks = (s.C + kAct8Block - 1) / kAct8Block, most = kApplyLanes / 4;
+  q->apply_tiles = (blocks + most - 1) / most;
+  q->apply_lanes = (blocks + q->apply_tiles - 1) / q->apply_tiles * 4;
   q->apply_lane_mul = 65536u / q->apply_lanes + 1;
   q->apply_rl = kThreads / q->apply_lanes;
   q->apply_tiles = (s.C + q->apply_lanes * 8 - 1) / (q->apply_lanes * 8);

@@ -407,21 +407,39 @@ __global__ void __launch_bounds__(kWgThreads, kWgCtas<MT, PACK>) wgrad8_kernel(c
   S::write(acc, part + slice * p.K * p.K * p.C, c0 + (tid >> 5) * 4, p.C, p.K);
 }
 
-// dw[i] = the slices' values added in slice order (n2 pairs).
-__global__ void __launch_bounds__(256) wgrad8_reduce_kernel(const float2* __restrict__ part, float2* __restrict__ dw,
-                                                            long long n2, int slices) {
+// dw[i] = the slices' values added up (n2 pairs).  Row y of a block takes every ROWS-th slice in order, and the rows
+// are added in order.  ROWS: 8 from 16 slices on, else 1 (many slices of few taps, 272 of 15 x 15 x 8, are one long
+// chain of loads with one row: 35 us for the gradient, 19.5 with 8; four slices of 27 x 27 x 512 are 19.9 us with 8
+// rows, 16.1 with one).
+constexpr int kReduceThreads = 256;
+template <int ROWS>
+__global__ void __launch_bounds__(kReduceThreads) wgrad8_reduce_kernel(const float2* __restrict__ part,
+                                                                       float2* __restrict__ dw, long long n2, int slices) {
+  constexpr int kAcross = kReduceThreads / ROWS;
+  __shared__ float2 sums[ROWS][kAcross + 1];
   griddep_wait();
   griddep_launch_dependents();
-  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= n2) return;
-  float2 a = part[i];
+  const int row = threadIdx.x / kAcross, lane = threadIdx.x % kAcross;
+  const long long i = static_cast<long long>(blockIdx.x) * kAcross + lane;
+  float2 a = make_float2(0.0f, 0.0f);
+  if (i < n2)
 #pragma unroll 8
-  for (int s = 1; s < slices; ++s) {
-    const float2 v = part[s * n2 + i];
-    a.x += v.x;
-    a.y += v.y;
+    for (int s = row; s < slices; s += ROWS) {
+      const float2 v = part[s * n2 + i];
+      a.x += v.x;
+      a.y += v.y;
+    }
+  if constexpr (ROWS > 1) {
+    sums[row][lane] = a;
+    __syncthreads();
+    if (row != 0) return;
+#pragma unroll
+    for (int r = 1; r < ROWS; ++r) {
+      a.x += sums[r][lane].x;
+      a.y += sums[r][lane].y;
+    }
   }
-  dw[i] = a;
+  if (i < n2) dw[i] = a;
 }
 
 // The kernel for K and a tile of columns, its rows a step and its shared memory.
@@ -533,8 +551,10 @@ extern "C" int dwb_conv2d_nhwc_bwd_weight_act8(const void* codes, const void* sc
   long long n2 = static_cast<long long>(K) * K * C / 2;
   int slices = p.chunks * p.col_tiles;
   void* a2[] = {&part, &dw, &n2, &slices};
-  e = launch_kernel(reinterpret_cast<const void*>(&wgrad8_reduce_kernel), dim3(static_cast<unsigned>((n2 + 255) / 256)),
-                    dim3(256), a2, 0, st);
+  const int rows = slices >= 16 ? 8 : 1;
+  e = launch_kernel(rows > 1 ? reinterpret_cast<const void*>(&wgrad8_reduce_kernel<8>)
+                             : reinterpret_cast<const void*>(&wgrad8_reduce_kernel<1>),
+                    dim3(static_cast<unsigned>((n2 * rows + kReduceThreads - 1) / kReduceThreads)), dim3(kReduceThreads), a2, 0, st);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
     return record_cuda_failure("wgrad8_reduce_kernel", e);
