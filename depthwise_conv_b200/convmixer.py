@@ -20,7 +20,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
-from . import dw_ops  # noqa: F401  (registers depthwise::conv2d_nhwc_fused)
+from . import act8_ops, dw_ops, norm_ops  # noqa: F401  (register the depthwise:: ops)
 
 CONVMIXER_MODELS = {
     '768_32': {'dim': 768, 'depth': 32, 'kernel_size': 7, 'patch_size': 7, 'activation': 'relu', 'n_classes': 1000},
@@ -110,6 +110,29 @@ class FusedDWBlock(nn.Module):
     def forward(self, x):
         return torch.ops.depthwise.conv2d_nhwc_fused(x, self.weight, self.bias, self.scale, self.shift, x,
                                                      self.act_code)
+
+
+class TrainableDWBlock(nn.Module):
+    """Residual(DW conv -> group norm -> act) in training, on the engine's differentiable ops.
+
+    ``checkpoint8``: what the backward pass needs of the convolution's and the norm's inputs is kept
+    in 8 bits (``act8_ops``): 1 + 1/32 bytes a value instead of 2.  A group norm, since a batch norm's
+    statistics (convmixer/convmixer.py:116-118) say little with few images a GPU.  channels_last
+    float16 in and out; the weight has the engine's [K, K, C] layout, the norm's parameters are float32.
+    """
+
+    def __init__(self, dim: int, kernel_size: int, num_groups: int = 32, activation: str = 'gelu', eps: float = 1e-5,
+                 checkpoint8: bool = False):
+        super().__init__()
+        self.num_groups, self.activation, self.eps, self.checkpoint8 = num_groups, activation, eps, checkpoint8
+        self.weight = nn.Parameter((torch.randn(kernel_size, kernel_size, dim) / kernel_size).half())
+        self.norm_weight = nn.Parameter(torch.ones(dim))
+        self.norm_bias = nn.Parameter(torch.zeros(dim))
+
+    def forward(self, x):
+        conv = act8_ops.conv2d_nhwc_act8 if self.checkpoint8 else torch.ops.depthwise.conv2d_nhwc
+        return x + norm_ops.group_norm_act(conv(x, self.weight), self.num_groups, self.norm_weight, self.norm_bias,
+                                           self.eps, self.activation, checkpoint=self.checkpoint8)
 
 
 def _epilogue(z, bias, scale, shift, act):

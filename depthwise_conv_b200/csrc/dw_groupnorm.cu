@@ -13,29 +13,31 @@
 
 namespace dwb {
 
-// dweight[c] and dbias[c]: the rows of sums added up, 8 threads a channel, each over every 8th row in order.
+// dweight[c] and dbias[c]: the rows of sums added up, 32 threads a channel, each over every 32nd row in order (the
+// rows of a large batch are one round of loads then: the gradient at 32x32x1536, B = 16, 67.1 us with 8, 65.9 with 32).
+constexpr int kParamChannels = 8, kParamParts = 32;
 template <typename T>
-__global__ void __launch_bounds__(256) gn_grad_params_kernel(const float2* __restrict__ sums, long long rows,
-                                                             void* __restrict__ dweight, void* __restrict__ dbias,
-                                                             const GnShape s) {
-  __shared__ float2 ent[8][33];
+__global__ void __launch_bounds__(kParamChannels * kParamParts)
+    gn_grad_params_kernel(const float2* __restrict__ sums, long long rows, void* __restrict__ dweight, void* __restrict__ dbias,
+                          const GnShape s) {
+  __shared__ float2 ent[kParamParts][kParamChannels + 1];
   griddep_wait();
   griddep_launch_dependents();
-  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;
+  const int lane = threadIdx.x % kParamChannels, part = threadIdx.x / kParamChannels;
+  const int c = blockIdx.x * kParamChannels + lane;  // C is a multiple of 8
   float2 a = make_float2(0.0f, 0.0f);
-  if (c < s.C)
 #pragma unroll 8
-    for (long long r = part; r < rows; r += 8) {
-      const float2 e = sums[r * s.C + c];
-      a.x += e.x;
-      a.y += e.y;
-    }
+  for (long long r = part; r < rows; r += kParamParts) {
+    const float2 e = sums[r * s.C + c];
+    a.x += e.x;
+    a.y += e.y;
+  }
   ent[part][lane] = a;
   __syncthreads();
-  if (part != 0 || c >= s.C) return;
+  if (part != 0) return;
   a = make_float2(0.0f, 0.0f);
-  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+  for (int i = 0; i < kParamParts; ++i) {
     a.x += ent[i][lane].x;
     a.y += ent[i][lane].y;
   }
@@ -127,8 +129,8 @@ static int gn_backward(const void* dy, const void* x, const void* codes, const v
   }
   if (rc != DWB_OK || (!dweight && !dbias)) return rc;
   void* args[] = {&sums, &rows, &dweight, &dbias, &s};
-  return gn_launch(reinterpret_cast<const void*>(&gn_grad_params_kernel<T>), "gn_grad_params_kernel", dim3((s.C + 31) / 32), 256,
-                   args, stream);
+  return gn_launch(reinterpret_cast<const void*>(&gn_grad_params_kernel<T>), "gn_grad_params_kernel",
+                   dim3(s.C / kParamChannels), kParamChannels * kParamParts, args, stream);
 }
 
 }  // namespace dwb

@@ -545,3 +545,72 @@ def test_a_training_block(eng):
     n = B * H * W * C
     assert kept["16"] >= 2 * n * 3 and kept["8"] <= 0.72 * kept["16"]
     assert eng.device_error() == 0
+
+
+@pytest.mark.parametrize("checkpoint8", [False, True])
+def test_trainable_blocks_in_a_model(eng, checkpoint8):
+    """Two ConvMixer training blocks: every gradient against float64 autograd of the same blocks, and one
+    gradient step that changes every parameter."""
+    import torch.nn.functional as F
+
+    from depthwise_conv_b200.convmixer import TrainableDWBlock
+    torch.manual_seed(5)
+    B, C, H, W, K = 2, 96, 16, 18, 9
+    blocks = torch.nn.Sequential(*(TrainableDWBlock(C, K, 12, act, checkpoint8=checkpoint8) for act in ("gelu", "silu"))).cuda()
+    x = nhwc(B, C, H, W, 31, torch.float16).requires_grad_()
+    dy = nhwc(B, C, H, W, 32, torch.float16)
+    y = blocks(x)
+    assert y.is_contiguous(memory_format=torch.channels_last) and y.dtype == torch.float16
+    y.backward(dy)
+    r = x.detach().double().requires_grad_()
+    z, leaves = r, []
+    for b in blocks:
+        p = [t.detach().double().requires_grad_() for t in (b.weight, b.norm_weight, b.norm_bias)]
+        leaves.append(p)
+        u = F.group_norm(F.conv2d(z, p[0].permute(2, 0, 1).unsqueeze(1), padding=K // 2, groups=C), 12, p[1], p[2], b.eps)
+        z = z + (F.gelu(u) if b.activation == "gelu" else F.silu(u))
+    z.backward(dy.double())
+    bar = 4e-2 if checkpoint8 else 5e-3  # as in test_a_training_block
+    assert (x.grad.double() - r.grad).norm() <= bar * r.grad.norm()
+    for b, p in zip(blocks, leaves):
+        for v, ref in zip((b.weight, b.norm_weight, b.norm_bias), p):
+            assert (v.grad.double() - ref.grad).norm() <= bar * ref.grad.norm()
+    before = [p.detach().clone() for p in blocks.parameters()]
+    torch.optim.SGD(blocks.parameters(), lr=0.1).step()
+    assert all(not torch.equal(a, b.detach()) for a, b in zip(before, blocks.parameters()))
+
+
+@pytest.mark.parametrize("checkpoint8", [False, True])
+def test_training_step_captured_and_replayed(eng, checkpoint8):
+    """Forward and backward of a block captured into a graph on leaves of their own, replayed with new data:
+    the gradients of an eager step on that data, bit for bit."""
+    from depthwise_conv_b200.convmixer import TrainableDWBlock
+    torch.manual_seed(6)
+    B, C, H, W = 2, 64, 20, 20
+    block = TrainableDWBlock(C, 7, 8, "gelu", checkpoint8=checkpoint8).cuda()
+    data = [(nhwc(B, C, H, W, s, torch.float16), nhwc(B, C, H, W, s + 1, torch.float16)) for s in (50, 60)]
+
+    def step(module, x, dy):
+        return torch.autograd.grad(module(x), list(module.parameters()), dy)
+
+    prev = torch.are_deterministic_algorithms_enabled()
+    torch.use_deterministic_algorithms(True, warn_only=True)  # the 16-bit weight gradient in a fixed order
+    try:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(block, *data[0])  # warm-up
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        x, dy = data[0][0].clone(memory_format=torch.preserve_format), data[0][1].clone(memory_format=torch.preserve_format)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            grads = step(block, x, dy)
+        x.copy_(data[1][0])
+        dy.copy_(data[1][1])
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(block, *data[1])
+    finally:
+        torch.use_deterministic_algorithms(prev)
+    assert all(torch.equal(g, w) for g, w in zip(grads, want))

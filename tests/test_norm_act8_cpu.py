@@ -204,3 +204,11 @@ def test_fake_impls():
         assert back.dtype == torch.bfloat16 and back.stride() == x.stride()
         y, codes, scales = torch.ops.depthwise.conv2d_nhwc_act8(x, w)
         assert y.stride() == x.stride() and codes.shape == x.shape and scales.dtype == torch.uint8
+
+
+def test_trainable_block_on_cpu_fails_loudly():
+    from depthwise_conv_b200.convmixer import TrainableDWBlock
+    x = torch.zeros(1, 64, 8, 8, dtype=torch.float16).contiguous(memory_format=torch.channels_last)
+    for checkpoint8 in (False, True):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            TrainableDWBlock(64, 5, 8, checkpoint8=checkpoint8)(x)
