@@ -29,11 +29,21 @@
 // range of rows.  A row of x (converted to fp16, transposed to channel-major) is
 // kept twice, the second time one element further, so that the pairs (w, w + 1)
 // of odd taps are aligned words too; the rows of dy stand in a ring.  A warp owns
-// 4 channels and keeps their taps in the accumulators.  While it multiplies, the
-// next rows travel from global memory into registers.  Partial sums go to slices
-// of the workspace that a second kernel adds in order; a chain of accumulations
-// is at most kChain products long, because the tensor core's accumulator rounds
-// towards zero, which a long chain would turn into a bias.
+// 4 channels and keeps their taps in the accumulators.  The codes and values of
+// the next two steps travel by cp.async into places that only their own thread
+// reads, so a step has one barrier.  Partial sums go to slices of the workspace
+// that a second kernel adds in order; a chain of accumulations is at most kChain
+// products long, because the tensor core's accumulator rounds towards zero, which
+// a long chain would turn into a bias.
+//
+// Measured (both kernels; the framework's 16-bit weight gradient on the CUDA
+// cores in brackets): 16x32x32x768 k7 36.7 us (64.3), 16x32x32x1536 k9 80.6 (182),
+// 8x56x56x1024 k13 137 (310), 8x56x56x128 k31 43 (171), 2x14x14x512 k27 11.7.
+// What bounds it is the issue of the instructions around the products, most of
+// all the conversion and transposition of x and dy: at 16x32x32x768 k7 the
+// 38 MB read need 5.8 us and the products' FMAs on the CUDA cores would need
+// 14.8.  Items of 4 channels, which spread a row over twice the threads, were
+// slower; so was one step of read-ahead.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -53,9 +63,9 @@ struct Wgrad8Params {
   int B, H, W, C, K;
   int tw;           // columns of dy a tile holds (16, 32, 48 or 64)
   int col_tiles;
-  int units;        // B * ceil(H / ROWS) steps of ROWS rows of x
-  int unit_rows;    // ceil(H / ROWS)
-  int per_chunk;    // units a CTA takes
+  int units;        // B * unit_rows steps
+  int unit_rows;    // ceil(H / rows of x a step)
+  int per_chunk;    // steps a CTA takes
   int chunks;
 };
 
@@ -99,30 +109,33 @@ __device__ __forceinline__ void copy16(void* dst, const void* src, bool on) {
 constexpr int up_to(int v, int to, int mod) { return v % mod == to % mod ? v : up_to(v + 1, to, mod); }
 constexpr int smaller(int a, int b) { return a < b ? a : b; }
 
-// MT x NT: 16-tap by 8-row products of one x row; ROWS: x rows a step; PACK: both rows in one product; TW: columns.
+// MT x NT: 16-tap by 8-row products of one x row; ROWS: x rows that meet the same rows of dy at once; PACK: both in one
+// product; TW: columns; SETS: sets of ROWS rows a step (narrow tiles: a barrier for more work, and items for more
+// threads).
 //
-// Shared memory, in words of two columns: x [2 buffers][ROWS][2 copies][32 channels][XP], dy [ring][32 channels][DP].
+// Shared memory, in words of two columns: x [2 buffers][kStep rows][2 copies][32 channels][XP], dy [ring][32 channels][DP].
 // In x, channel 8 v + k has place 4 k + v and XP is 8 or 24 modulo 32; in dy, places are channels and DP is odd: the
 // stores of a warp (4 vectors of 8 channels times 8 column pairs of x, or 8 words of dy) fall in 32 banks.  The copies
 // are 16 banks apart and the rows of dy 4, so that a fragment's 32 words do too.  Behind them, for each step read
 // ahead, the codes and values that a thread has under way: each in places of its own, which need no barrier.
-template <int MT, int NT, int ROWS, bool PACK, int TW>
+template <int MT, int NT, int ROWS, bool PACK, int TW, int SETS>
 struct Wgrad8 {
+  static constexpr int kStep = SETS * ROWS;  // rows of x a step
   static constexpr int kXWords = (TW + (PACK ? 8 : 16 * MT)) / 2, kDWords = TW / 2;
   static constexpr int XP = smaller(up_to(kXWords, 8, 32), up_to(kXWords, 24, 32));
   static constexpr int DP = kDWords | 1;
-  static constexpr int kCopy = kWgChannels * XP + 16, kXRow = 2 * kCopy, kXBuffer = ROWS * kXRow;
+  static constexpr int kCopy = kWgChannels * XP + 16, kXRow = 2 * kCopy, kXBuffer = kStep * kXRow;
   static constexpr int kDRow = kWgChannels * DP + 4;
   static constexpr int kDItems = TW * 2;  // of a row of dy: 2 columns x 8 channels
   static constexpr int kBlocks = TW / 16;
   static constexpr int kAcc = PACK ? 1 : ROWS;
   typedef float Acc[4][kAcc][MT][NT][4];
 
-  static constexpr int ring(int K) { return K - 1 + 2 * ROWS; }
+  static constexpr int ring(int K) { return K - 1 + 2 * kStep; }
   static constexpr int x_items(int K) { return (TW + K - 1 + 3) / 4 * 4; }  // of a row of x
   static constexpr int fixed_words(int K) { return (2 * kXBuffer + ring(K) * kDRow + 3) / 4 * 4; }
   static constexpr int smem(int K) {
-    return 4 * fixed_words(K) + kAhead * ROWS * (x_items(K) * 5 * 8 + kDItems * 2 * 16);
+    return 4 * fixed_words(K) + kAhead * kStep * (x_items(K) * 5 * 8 + kDItems * 2 * 16);
   }
 
   // even copy: words (4i, 4i + 1), (4i + 2, 4i + 3); odd copy: (4i + 1, 4i + 2), (4i + 3, 4i + 4)
@@ -153,7 +166,7 @@ struct Wgrad8 {
     return (warp & 1) * 16 + (warp >> 1);
   }
 
-  // One step: ROWS rows of x at `xs` against the ring rows first, first + 1, ...
+  // One set: ROWS rows of x at `xs` against the ring rows first, first + 1, ...
   static __device__ __forceinline__ void multiply(Acc& acc, const uint32_t* xs, const uint32_t* ds, int first, int K) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t* xa = xs + (g & 1) * kCopy + warp_place() * XP + (g >> 1) + t;
@@ -253,40 +266,41 @@ struct Wgrad8 {
 template <int MT, bool PACK>
 constexpr int kWgCtas = PACK ? 3 : MT == 1 ? 2 : 1;
 
-template <int MT, int NT, int ROWS, bool PACK, int TW>
+template <int MT, int NT, int ROWS, bool PACK, int TW, int SETS>
 __global__ void __launch_bounds__(kWgThreads, kWgCtas<MT, PACK>) wgrad8_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                             const __half* __restrict__ dy, float* __restrict__ part,
                                                             const Wgrad8Params p) {
-  using S = Wgrad8<MT, NT, ROWS, PACK, TW>;
+  using S = Wgrad8<MT, NT, ROWS, PACK, TW, SETS>;
+  constexpr int kStep = S::kStep;
   extern __shared__ __align__(16) uint32_t smem[];
   uint32_t* const xs = smem;
   uint32_t* const ds = smem + 2 * S::kXBuffer;
   griddep_wait();
   griddep_launch_dependents();
   const int c0 = blockIdx.x * kWgChannels, w0 = static_cast<int>(blockIdx.z) * TW, tid = threadIdx.x;
-  const int sblocks = (p.C + kAct8Block - 1) / kAct8Block, pad = p.K / 2, used = p.K - 1 + ROWS, ring = S::ring(p.K);
+  const int sblocks = (p.C + kAct8Block - 1) / kAct8Block, pad = p.K / 2, used = p.K - 1 + kStep, ring = S::ring(p.K);
 
   // What this thread brings in at every step, a row further each time: one item of x (columns x_col .. x_col + 4, of
-  // row x_row of the step's ROWS) and one of dy (2 columns of row d_row).
+  // row x_row of the step's) and one of dy (2 columns of row d_row).
   const int x_items = S::x_items(p.K);
   const int x_row = tid / x_items, x_item = tid - x_row * x_items;
   const int x_c = c0 + (x_item & 3) * 8, x_col = w0 - pad + (x_item >> 2) * 4;
   unsigned x_mask = 0;
 #pragma unroll
   for (int j = 0; j < 5; ++j)
-    if (x_row < ROWS && x_c < p.C && x_col + j >= 0 && x_col + j < p.W) x_mask |= 1u << j;
+    if (x_row < kStep && x_c < p.C && x_col + j >= 0 && x_col + j < p.W) x_mask |= 1u << j;
   // the last warps begin with dy, so that those that convert codes have none of it where the tile is narrow
   const int d_tid = kWgThreads - 1 - tid, d_row = d_tid / S::kDItems, d_item = d_tid - d_row * S::kDItems;
   const int d_c = c0 + (d_item & 3) * 8, d_col = w0 + (d_item >> 2) * 2;
   unsigned d_mask = 0;
 #pragma unroll
   for (int j = 0; j < 2; ++j)
-    if (d_row < ROWS && d_c < p.C && d_col + j < p.W) d_mask |= 1u << j;
+    if (d_row < kStep && d_c < p.C && d_col + j < p.W) d_mask |= 1u << j;
   const long long line = static_cast<long long>(p.W) * p.C, s_line = static_cast<long long>(p.W) * sblocks;
   unsigned char* const raw = reinterpret_cast<unsigned char*>(smem + S::fixed_words(p.K));
   uint2* const x_raw = reinterpret_cast<uint2*>(raw) + tid;                                              // [kAhead][5][items]
-  uint4* const d_raw = reinterpret_cast<uint4*>(raw + kAhead * ROWS * x_items * 5 * 8) + d_tid;           // [kAhead][2][items]
-  const int x_many = ROWS * x_items, d_many = ROWS * S::kDItems;
+  uint4* const d_raw = reinterpret_cast<uint4*>(raw + kAhead * kStep * x_items * 5 * 8) + d_tid;           // [kAhead][2][items]
+  const int x_many = kStep * x_items, d_many = kStep * S::kDItems;
 
   // A row past the image: codes of 0, whatever the step.
   auto load_scales = [&](XScales& s, const uint8_t* e, bool on) {
@@ -294,14 +308,14 @@ __global__ void __launch_bounds__(kWgThreads, kWgCtas<MT, PACK>) wgrad8_kernel(c
     for (int j = 0; j < 5; ++j) s.e[j] = on && (x_mask >> j & 1) ? e[j * sblocks] : static_cast<uint8_t>(127);
   };
   auto fetch = [&](int place, const int8_t* q, bool x_on, const __half* d, bool d_on) {
-    if (x_row < ROWS) {
+    if (x_row < kStep) {
 #pragma unroll
       for (int j = 0; j < 5; ++j) {
         const bool on = x_on && (x_mask >> j & 1);
         copy8(x_raw + (place * 5 + j) * x_many, on ? q + j * p.C : codes, on);
       }
     }
-    if (d_row < ROWS) {
+    if (d_row < kStep) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const bool on = d_on && (d_mask >> j & 1);
@@ -331,9 +345,9 @@ __global__ void __launch_bounds__(kWgThreads, kWgCtas<MT, PACK>) wgrad8_kernel(c
   while (u < u1) {  // one image's part of the range at a time
     const int b = u / p.unit_rows;
     const int s0 = u - b * p.unit_rows, steps = min(p.unit_rows - s0, u1 - u);
-    const int top = s0 * ROWS + pad - (p.K - 1);  // first row of dy that the first row of x meets
+    const int top = s0 * kStep + pad - (p.K - 1);  // first row of dy that the first row of x meets
     // of x and dy, this thread's next to fetch; of the exponent bytes, its next to load
-    int row = s0 * ROWS + x_row, drow = top + used + d_row;
+    int row = s0 * kStep + x_row, drow = top + used + d_row;
     const long long x_at = (static_cast<long long>(b) * p.H + row) * p.W + x_col;
     const int8_t* q = codes + x_at * p.C + x_c;
     const uint8_t* e = scales + x_at * sblocks + x_c / kAct8Block;
@@ -342,19 +356,19 @@ __global__ void __launch_bounds__(kWgThreads, kWgCtas<MT, PACK>) wgrad8_kernel(c
     auto next = [&](int step) {
       if (step < steps) fetch(step & 1, q, row < p.H, d, drow >= 0 && drow < p.H);
       cp_async_commit();
-      row += ROWS;
-      drow += ROWS;
-      q += ROWS * line;
-      d += ROWS * line;
+      row += kStep;
+      drow += kStep;
+      q += kStep * line;
+      d += kStep * line;
     };
     __syncthreads();  // the last image's rows have been read
     // the first step: its row of x, and all rows of dy that it meets
     XScales sc[2];
-    load_scales(sc[0], e, s0 * ROWS + x_row < p.H);
+    load_scales(sc[0], e, s0 * kStep + x_row < p.H);
     fetch(0, q, row < p.H, d, false);
     cp_async_commit();
-    row += ROWS;
-    q += ROWS * line;
+    row += kStep;
+    q += kStep * line;
     for (int i = tid; i < used * S::kDItems; i += kWgThreads) {
       const int r = i / S::kDItems, item = i - r * S::kDItems, at = top + r;
       const int c = c0 + (item & 3) * 8, col = w0 + (item >> 2) * 2;
@@ -367,37 +381,42 @@ __global__ void __launch_bounds__(kWgThreads, kWgCtas<MT, PACK>) wgrad8_kernel(c
       S::store_dy(v, ds + r * S::kDRow, item);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    if (x_row < ROWS) {
+    if (x_row < kStep) {
       uint2 v[5];
       fetched_x(0, v);
       S::store_x(v, sc[0], xs + x_row * S::kXRow, x_item);
     }
-    e += ROWS * s_line;
-    load_scales(sc[0], e, steps > 1 && s0 * ROWS + ROWS + x_row < p.H);  // step 1
+    e += kStep * s_line;
+    load_scales(sc[0], e, steps > 1 && s0 * kStep + kStep + x_row < p.H);  // step 1
     next(1);
     __syncthreads();
     int first = 0;  // ring slot of the row of dy with j = 0
     for (int s = 0; s < steps; ++s) {
       const bool more = s + 1 < steps;
-      e += ROWS * s_line;
-      load_scales(sc[1], e, s + 2 < steps && (s0 + s + 2) * ROWS + x_row < p.H);
+      e += kStep * s_line;
+      load_scales(sc[1], e, s + 2 < steps && (s0 + s + 2) * kStep + x_row < p.H);
       next(s + 2);
-      S::multiply(acc, xs + (s & 1) * S::kXBuffer, ds, first, p.K);
+#pragma unroll 1
+      for (int i = 0; i < SETS; ++i) {
+        if (SETS > 1 && (s0 + s) * kStep + i * ROWS >= p.H) break;  // rows past the image
+        const int at = first + i * ROWS;
+        S::multiply(acc, xs + (s & 1) * S::kXBuffer + i * ROWS * S::kXRow, ds, at < ring ? at : at - ring, p.K);
+      }
       asm volatile("cp.async.wait_group 1;" ::: "memory");  // step s + 1 is here
-      if (more && x_row < ROWS) {
+      if (more && x_row < kStep) {
         uint2 v[5];
         fetched_x((s + 1) & 1, v);
         S::store_x(v, sc[0], xs + ((s + 1) & 1) * S::kXBuffer + x_row * S::kXRow, x_item);
       }
-      if (more && d_row < ROWS) {
-        // the ring has ROWS rows more than a step reads: these slots belong to no row of this step
+      if (more && d_row < kStep) {
+        // the ring has kStep rows more than a step reads: these slots belong to no row of this step
         int slot = first + used + d_row;
         slot -= slot >= ring ? ring : 0;
         const uint4 v[2] = {d_raw[((s + 1) & 1) * 2 * d_many], d_raw[(((s + 1) & 1) * 2 + 1) * d_many]};
         S::store_dy(v, ds + slot * S::kDRow, d_item);
       }
       sc[0] = sc[1];
-      first += ROWS;
+      first += kStep;
       first -= first >= ring ? ring : 0;
       __syncthreads();
     }
@@ -445,19 +464,29 @@ __global__ void __launch_bounds__(kReduceThreads) wgrad8_reduce_kernel(const flo
 // The kernel for K and a tile of columns, its rows a step and its shared memory.
 struct Wgrad8Kernel {
   const void* fn;
-  int rows, ctas, smem;  // ctas: an SM, by registers
+  int step, sets, ctas, smem;  // rows and sets a step; CTAs an SM, by registers
 };
-template <int MT, int NT, int ROWS, bool PACK, int TW>
+template <int MT, int NT, int ROWS, bool PACK, int TW, int SETS>
 static Wgrad8Kernel wgrad8_kernel_of(int K) {
-  return {reinterpret_cast<const void*>(&wgrad8_kernel<MT, NT, ROWS, PACK, TW>), ROWS,
-          kWgCtas<MT, PACK>, Wgrad8<MT, NT, ROWS, PACK, TW>::smem(K)};
+  using S = Wgrad8<MT, NT, ROWS, PACK, TW, SETS>;
+  return {reinterpret_cast<const void*>(&wgrad8_kernel<MT, NT, ROWS, PACK, TW, SETS>), S::kStep, SETS, kWgCtas<MT, PACK>,
+          S::smem(K)};
 }
+static int wgrad8_room(const Wgrad8Kernel& k) { return 228 * 1024 / (k.smem + 1024); }  // CTAs an SM, by shared memory
+// Sets: as many as a step's items of x have threads for.  A step of one set leaves most threads of a narrow tile without
+// an item and has a barrier for few products (19x14x8x1424 k9: 40.2 us with one set, 32.4 with two; 8x14x14x512 k27: 21.0
+// with one, 17.7 with four; 8x32x32x1536 k27: 165 with one, 146 with two).  But not where the longer ring then leaves
+// room for fewer CTAs an SM (16x32x32x1536 k11: 86.0 us with one set and two CTAs, 145 with two sets and one).
 template <int TW>
 static Wgrad8Kernel wgrad8_kernel_for(int K) {
-  if (K <= 7) return wgrad8_kernel_of<1, 1, 2, true, TW>(K);
-  if (K <= 15) return wgrad8_kernel_of<1, 2, 2, false, TW>(K);
-  if (K <= 23) return wgrad8_kernel_of<2, 3, 1, false, TW>(K);
-  return wgrad8_kernel_of<2, 4, 1, false, TW>(K);
+  constexpr int kPair = TW <= 32 ? 2 : 1, kOne = TW == 16 ? 4 : TW == 32 ? 2 : 1;
+  if (K <= 7) return wgrad8_kernel_of<1, 1, 2, true, TW, kPair>(K);
+  if (K <= 15) {
+    const Wgrad8Kernel k = wgrad8_kernel_of<1, 2, 2, false, TW, kPair>(K);
+    return kPair > 1 && wgrad8_room(k) < k.ctas ? wgrad8_kernel_of<1, 2, 2, false, TW, 1>(K) : k;
+  }
+  if (K <= 23) return wgrad8_kernel_of<2, 3, 1, false, TW, kOne>(K);
+  return wgrad8_kernel_of<2, 4, 1, false, TW, kOne>(K);
 }
 static Wgrad8Kernel wgrad8_kernel_for(int K, int tw) {
   switch (tw) {
@@ -480,17 +509,17 @@ static int wgrad8_plan(int64_t B, int64_t H, int64_t W, int64_t C, int K, Wgrad8
   p->tw = ((p->W + p->col_tiles - 1) / p->col_tiles + 15) / 16 * 16;  // even tiles: W = 65 is 48 + 17, not 64 + 1
   p->col_tiles = (p->W + p->tw - 1) / p->tw;
   const Wgrad8Kernel k = wgrad8_kernel_for(K, p->tw);
-  p->unit_rows = (p->H + k.rows - 1) / k.rows;
+  p->unit_rows = (p->H + k.step - 1) / k.step;
   p->units = p->B * p->unit_rows;
   // As many ranges as CTAs run at once (a range more on some SMs would double the time), and none whose chains get too
   // long.  However short: the rows of dy that a range brings in before its first product cost less than idle SMs
   // (14x14x512 k27, B = 2: 28.8 us with ranges of 26 rows, 16.2 with 8, 14.7 with 4).
   const long long base = (C + kWgChannels - 1) / kWgChannels * p->col_tiles;
-  const int room = 228 * 1024 / (k.smem + 1024);
+  const int room = wgrad8_room(k);
   const long long at_once = static_cast<long long>(room < k.ctas ? room : k.ctas) * kSmCount;
   const long long ranges = at_once / base > 1 ? at_once / base : 1;
   long long per = (p->units + ranges - 1) / ranges;
-  const long long most = kChain / (p->tw / 16);
+  const long long most = kChain / (p->tw / 16 * k.sets);
   per = per < 1 ? 1 : per > most ? most : per;
   p->per_chunk = static_cast<int>(per);
   p->chunks = (p->units + p->per_chunk - 1) / p->per_chunk;
