@@ -59,6 +59,20 @@ def after_launch(t: torch.Tensor, where: str) -> None:
             _lib.after_launch(dw_ops._stream_of(t), where)
 
 
+def incoming(grad: torch.Tensor) -> torch.Tensor:
+    """A gradient from autograd as the kernels take it: channels_last, on a 16-byte boundary."""
+    g = grad.contiguous(memory_format=torch.channels_last)
+    return g if g.data_ptr() % 16 == 0 else g.clone()
+
+
+def first_order(name: str, *grads):
+    """The gradients a backward pass returns; differentiating them again raises instead of leaving terms out."""
+    if torch.is_grad_enabled():  # under create_graph=True
+        refuse = torch._C._functions.DelayedError(f"{name}: the backward pass is not differentiable", 1)
+        grads = tuple(g if g is None else refuse(g.requires_grad_()) for g in grads)
+    return grads
+
+
 def act8_encode(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(codes, scales) of a channels_last float16 or bfloat16 activation."""
     kept = bind().act8_encode(x)
@@ -146,12 +160,11 @@ def _conv2d_nhwc_act8_backward(ctx, grad, _codes, _scales):
     if grad is None:
         return None, None, None
     w, codes, scales = ctx.saved_tensors
-    g = grad if grad.is_contiguous(memory_format=torch.channels_last) else grad.contiguous(
-        memory_format=torch.channels_last)
+    g = incoming(grad)
     dx = dw_ops.conv2d_nhwc_backward_input(g, w) if ctx.needs_input_grad[0] else None
     dw = conv2d_nhwc_backward_weight_act8(codes, scales, g, w.shape[0]).to(w.dtype) if ctx.needs_input_grad[1] else None
-    db = g.float().sum(dim=(0, 2, 3)).to(g.dtype) if ctx.has_bias and ctx.needs_input_grad[2] else None
-    return dx, dw, db
+    db = g.float().sum(dim=(0, 2, 3)).to(g.dtype).detach() if ctx.has_bias and ctx.needs_input_grad[2] else None
+    return first_order("conv2d_nhwc_act8", dx, dw, db)
 
 
 torch.library.register_autograd("depthwise::conv2d_nhwc_act8", _conv2d_nhwc_act8_backward,

@@ -26,7 +26,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .act8_ops import after_launch, bind, empty_checkpoint
+from .act8_ops import after_launch, bind, empty_checkpoint, first_order, incoming
 
 ACT_CODES = _lib.NORM_ACT_CODES
 
@@ -104,12 +104,12 @@ def _group_norm_act_backward(ctx, grad, *_):
     if grad is None:
         return (None,) * 7
     x, weight, bias, mean, rstd, codes, scales = ctx.saved_tensors
-    g = grad if grad.is_contiguous(memory_format=torch.channels_last) else grad.contiguous(
-        memory_format=torch.channels_last)
-    dx, dweight, dbias = group_norm_act_backward(g, (codes, scales) if ctx.checkpoint else x, mean, rstd, ctx.num_groups,
-                                                 weight, bias, ctx.act)
+    dx, dweight, dbias = group_norm_act_backward(incoming(grad), (codes, scales) if ctx.checkpoint else x, mean, rstd,
+                                                 ctx.num_groups, weight, bias, ctx.act)
     need = ctx.needs_input_grad
-    return (dx if need[0] else None, None, dweight if need[2] else None, dbias if need[3] else None, None, None, None)
+    dx, dweight, dbias = first_order("group_norm_act", dx if need[0] else None, dweight if need[2] else None,
+                                     dbias if need[3] else None)
+    return dx, None, dweight, dbias, None, None, None
 
 
 torch.library.register_autograd("depthwise::group_norm_act", _group_norm_act_backward,

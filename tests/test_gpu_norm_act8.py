@@ -614,3 +614,119 @@ def test_training_step_captured_and_replayed(eng, checkpoint8):
     finally:
         torch.use_deterministic_algorithms(prev)
     assert all(torch.equal(g, w) for g, w in zip(grads, want))
+
+
+# ---- calls at the edges of what the ops take -------------------------------------------------------------
+
+@pytest.mark.parametrize("K", [1, 5, 7, 9, 11, 15, 17, 23, 25, 31])
+def test_weight_gradient_over_kernel_sizes_and_widths(eng, K):
+    """Every width of a tile, just below, at and above it, with heights that end inside a step."""
+    for i, W in enumerate((4, 16, 17, 32, 33, 48, 49, 64, 65)):
+        B, H, C = 2 + i % 2, 1 + (5 * i + K) % 11, (24, 40, 64)[i % 3]
+        (codes, scales), dy = _wgrad_problem(B, H, W, C, K)
+        dw = eng.act8_ops.conv2d_nhwc_backward_weight_act8(codes, scales, dy, K)
+        ref, size = R.dw_weight_grad(R.act8_decode(codes, scales), dy, K)
+        assert ((dw.double() - ref).abs() <= 2.0**-16 * size).all(), (B, H, W, C)
+
+
+@pytest.mark.parametrize("act", ["gelu", "none"])
+def test_many_small_samples(eng, act):
+    """More samples than a grid's second dimension takes: forward, backward and the checkpoint."""
+    B, H, W, C, G = 70000, 1, 2, 16, 2
+    x, dy = nhwc(B, C, H, W, 1, torch.float16), nhwc(B, C, H, W, 2, torch.float16, offset=0.1)
+    w, b = params(C, 3, torch.float32)
+    out = eng.norm_ops.group_norm_act_forward(x, G, w, b, act=act, checkpoint=True)
+    check_forward(out, x, G, w, b, 1e-5, act)
+    assert all(torch.equal(i, j) for i, j in zip(out[3:], eng.act8_encode(x)))
+    mean, rstd = (t.float() for t in R.stats(x, G, 1e-5))
+    dx = eng.norm_ops.group_norm_act_backward(dy, x, mean, rstd, G, w, b, act)[0]
+    r = R.group_norm_act_grad(dy, x, mean, rstd, G, w, b, act)
+    far = 1 + R._per_channel((mean.double() * rstd.double()).abs(), C)
+    assert ((dx.double() - r["dx"]).abs() <= rounded(r["dx"], dx.dtype) + 64 * E32 * far * r["dx_size"]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", [(2, 9, 7, 72, 8), (2, 61, 47, 1536, 2)])
+def test_parameters_at_any_offset(eng, shape, dtype):
+    """Slices of one flat buffer, each a value further than a vector load could start: the same bits."""
+    B, H, W, C, G = shape
+    x, dy = nhwc(B, C, H, W, 1, torch.float16), nhwc(B, C, H, W, 2, torch.float16)
+    w, b = params(C, 3, dtype)
+    flat = torch.zeros(2 * C + 8, dtype=dtype, device="cuda")
+    wv, bv = flat[1:1 + C].copy_(w), flat[C + 3:2 * C + 3].copy_(b)
+    n = eng.norm_ops
+    want, got = n.group_norm_act_forward(x, G, w, b, act="gelu"), n.group_norm_act_forward(x, G, wv, bv, act="gelu")
+    assert all(torch.equal(i, j) for i, j in zip(want, got))
+    want, got = (n.group_norm_act_backward(dy, x, *want[1:], G, p, q, "gelu") for p, q in ((w, b), (wv, bv)))
+    assert all(torch.equal(i, j) for i, j in zip(want, got))
+
+
+def test_offsets_past_32_bits(eng):
+    """One image of 2^31 values and more, most of them zero: its last rows against the same rows by themselves."""
+    H, W, C, G, K, tail = 8200, 8200, 32, 2, 3, 5
+    x = torch.zeros(1, H, W, C, dtype=torch.float16, device="cuda").permute(0, 3, 1, 2)
+    dy = torch.zeros_like(x)
+    x[:, :, -tail:] = nhwc(1, C, tail, W, 1, torch.float16)
+    dy[:, :, -tail:] = nhwc(1, C, tail, W, 2, torch.float16)
+    w, b = params(C, 3, torch.float32)
+    xt, dyt = x[:, :, -tail:], dy[:, :, -tail:]
+    y, mean, rstd, codes, scales = eng.norm_ops.group_norm_act_forward(x, G, w, b, act="silu", checkpoint=True)
+    small = eng.act8_encode(xt)
+    assert torch.equal(codes[:, :, -tail:], small[0]) and torch.equal(scales[:, -tail:], small[1])
+    assert not codes[:, :, :-tail].any()
+    kept = eng.act8_encode(x)
+    assert torch.equal(kept[0], codes) and torch.equal(kept[1], scales)
+    assert torch.equal(eng.act8_decode(codes, scales)[:, :, -tail:], eng.act8_decode(*small))
+    # a thread adds up to 2^10 values that are not zero: 2^10 e32 of the sum of the magnitudes
+    v = xt.double().reshape(G, -1)
+    n = H * W * C // G
+    mr = v.sum(1) / n
+    rr = (((v - mr[:, None])**2).sum(1) / n + (1 - v.shape[1] / n) * mr**2 + 1e-5).rsqrt()
+    assert ((mean[0].double() - mr).abs() <= 2.0**-14 * v.abs().sum(1) / n + 2 * E32 * mr.abs()).all()
+    assert ((rstd[0].double() - rr).abs() <= 2.0**-14 * rr).all()
+    md, rd = mean.double(), rstd.double()
+    u = R.normalised(xt, md, rd) * w.double()[:, None, None] + b.double()[:, None, None]
+    yr, _ = R.act_and_slope(u, "silu")
+    xh = R.normalised(xt, md, rd)
+    size = w.double().abs()[:, None, None] * (xh.abs() + R._per_channel((md * rd).abs(), C)) + b.double().abs()[:, None, None]
+    assert ((y[:, :, -tail:].double() - yr).abs() <= rounded(yr, y.dtype) + 64 * E32 * size).all()
+    assert (y[:, :, :-tail] == y[:, :, :1, :1]).all()
+    del y, kept
+    # the input gradient: the sums over the rows with a gradient, then every pixel by itself
+    d = [eng.norm_ops.group_norm_act_backward(dy, saved, mean, rstd, G, w, b, "none")[0] for saved in (x, (codes, scales))]
+    for dx, values in zip(d, (xt, eng.act8_decode(*small))):
+        xh, g = R.normalised(values, md, rd), dyt.double() * w.double()[:, None, None]
+        m1, m2 = (R._per_channel(t.reshape(1, G, -1).sum(2) / n, C) for t in (g, g * xh))
+        s1, s2 = (R._per_channel(t.abs().reshape(1, G, -1).sum(2) / n, C) for t in (g, g * xh))
+        rc = R._per_channel(rd, C)
+        ref, size = rc * (g - m1 - xh * m2), rc * (g.abs() + s1 + xh.abs() * s2)
+        far = 1 + R._per_channel((md * rd).abs(), C)
+        assert ((dx[:, :, -tail:].double() - ref).abs() <= rounded(ref, dx.dtype) + 2.0**-13 * far * size).all()
+    del d
+    dw = eng.act8_ops.conv2d_nhwc_backward_weight_act8(codes, scales, dy, K)
+    ref, size = R.dw_weight_grad(R.act8_decode(*small), dyt, K)
+    assert ((dw.double() - ref).abs() <= 2.0**-16 * size).all()
+    assert eng.device_error() == 0
+
+
+def test_a_second_derivative_is_refused(eng):
+    """The backward passes are not differentiable: a gradient of a gradient raises, a first one with a graph does not."""
+    x = nhwc(1, 32, 6, 5, 1, torch.float16).requires_grad_()
+    w = torch.ones(3, 3, 32, dtype=torch.float16, device="cuda", requires_grad=True)
+    for f in (lambda: eng.group_norm_act(x, 4, act="gelu"), lambda: eng.conv2d_nhwc_act8(x, w)):
+        plain, = torch.autograd.grad(f().sum(), x)
+        first, = torch.autograd.grad(f().sum(), x, create_graph=True)
+        assert torch.equal(first, plain)
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            (first.square().sum() + x.sum()).backward()
+
+
+def test_a_gradient_off_the_vector_boundary(eng):
+    """A gradient that autograd cuts out of a larger one at an odd place is copied, not refused."""
+    x = nhwc(3, 32, 1, 1, 1, torch.float16).requires_grad_()
+    y = eng.group_norm_act(x, 4, act="gelu")
+    odd = torch.zeros(3, device="cuda", dtype=torch.float16, requires_grad=True)
+    dy = torch.randn(99, device="cuda").half()
+    torch.cat([odd, y.flatten()]).backward(dy)
+    want = torch.autograd.grad(eng.group_norm_act(x, 4, act="gelu"), x, dy[3:].clone().view(3, 32, 1, 1))[0]
+    assert torch.equal(x.grad, want)
