@@ -229,15 +229,12 @@ __device__ __forceinline__ void warp_sum2(float& a, float& b) {
   }
 }
 
-// Sum over the CTA (blockDim.x a multiple of 32, at most 1024); `scratch` holds 33 floats.
-__device__ __forceinline__ float block_sum(float v, float* scratch) {
-  v = warp_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float s = 0.0f;
-  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) s += scratch[w];
-  return s;
+// The mean of a group, from its offset to a pivot or from the plain mean of the same values.  The pivot takes out a mean
+// that is large against the deviations; but where the mean is small against the pivot, pivot + off has the pivot's
+// rounding, and the plain mean that of the values only (7x7x1024, 32 groups: the means' error 1.9e-7 of their size with
+// the pivot alone, 7e-8 so).
+__device__ __forceinline__ float gn_mean(float pivot, float off, float plain) {
+  return fabsf(plain) < 0.5f * fabsf(pivot) ? plain : pivot + off;
 }
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
@@ -319,9 +316,9 @@ struct GnMerge {
   // (mean, M2) over `rows` pixels of `channels`; (0, 0) without pixels.
   template <int SUB>
   __device__ __forceinline__ float2 run(const float2* first, int rows, int channels) const {
-    // about one thread's mean, which is a mean of its values already: nothing cancels in the last step
+    // about one thread's mean, which is a mean of its values already: nothing cancels in the squares
     const float pivot = live ? first[0].x : 0.0f;
-    float s1 = 0.0f, s2 = 0.0f;
+    float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f;
     if (r0 < r_step)
 #pragma unroll 4
       for (int r = r0; r < live; r += r_step) {
@@ -329,14 +326,16 @@ struct GnMerge {
         for (int k = k0; k < per_row; k += k_step) {
           const float2 v = first[r * row_words + k];
           const float d = v.x - pivot;
+          s0 += n * v.x;
           s1 += n * d;
           s2 += v.y + n * d * d;
         }
       }
     warp_sum2(s1, s2);
+    s0 = warp_sum(s0);
     if (!rows) return make_float2(0.0f, 0.0f);
-    const float d = s1 / (static_cast<float>(rows) * static_cast<float>(channels));
-    return make_float2(pivot + d, not_negative(s2 - s1 * d));
+    const float n = static_cast<float>(rows) * static_cast<float>(channels), d = s1 / n;
+    return make_float2(gn_mean(pivot, d, s0 / n), not_negative(s2 - s1 * d));
   }
 };
 

@@ -164,8 +164,8 @@ __global__ void __launch_bounds__(kGnThreads, 4)
       // a CTA without pixels has no weight
       float s1 = n > 0.0f ? n * d : 0.0f, s2 = n > 0.0f ? v.y + n * d * d : 0.0f;
       warp_sum2(s1, s2);
-      const float off = s1 / (static_cast<float>(s.P) * static_cast<float>(s.Cg));
-      mean = pivot + off;
+      const float all = static_cast<float>(s.P) * static_cast<float>(s.Cg), off = s1 / all;
+      mean = gn_mean(pivot, off, warp_sum(n * v.x) / all);
       m2 = not_negative(s2 - s1 * off);
     }
     const float rstd = 1.0f / sqrtf(m2 / (static_cast<float>(s.P) * static_cast<float>(s.Cg)) + s.eps);

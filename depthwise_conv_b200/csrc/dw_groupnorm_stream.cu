@@ -171,20 +171,22 @@ __device__ __forceinline__ void merge_stats(const float2* __restrict__ part, con
   const int last = static_cast<int>(s.P) - (q.chunks - 1) * q.rows;
   for (int g = g0 + (threadIdx.x >> 5); g <= g1; g += kThreads / 32) {
     const float2* first = of_sample + g * per;
-    // about the first entry's mean: entries are means of many values, nothing cancels in the last step
+    // about the first entry's mean: entries are means of many values, nothing cancels in the squares
     const float pivot = first[0].x;
-    float s1 = 0.0f, s2 = 0.0f;
+    float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f;
     for (int e = lane; e < q.chunks * per; e += 32) {
       const int chunk = e / per, k = e - chunk * per;
       const float2 v = first[static_cast<long long>(chunk) * q.entries + k];
       const float n = static_cast<float>(chunk == q.chunks - 1 ? last : q.rows) * static_cast<float>(entry_width(s, q, k));
       const float d = v.x - pivot;
+      s0 += n * v.x;
       s1 += n * d;
       s2 += v.y + n * d * d;
     }
     warp_sum2(s1, s2);
+    s0 = warp_sum(s0);
     const float n = static_cast<float>(s.P) * static_cast<float>(s.Cg), off = s1 / n;
-    const float mean = pivot + off, rstd = 1.0f / sqrtf(not_negative(s2 - s1 * off) / n + s.eps);
+    const float mean = gn_mean(pivot, off, s0 / n), rstd = 1.0f / sqrtf(not_negative(s2 - s1 * off) / n + s.eps);
     if (lane == 0) {
       fin[g - g0] = make_float2(mean, rstd);
       if (mean_out && g * s.Cg >= c0) {
