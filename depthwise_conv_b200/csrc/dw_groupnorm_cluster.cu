@@ -12,6 +12,12 @@
 // or the channel sums (backward) of the cluster's CTAs are exchanged through
 // distributed shared memory, and every CTA adds them up in rank order: the same
 // bits in every CTA and on every run.
+//
+// Measured, forward: 31.9 us at 16x32x32x1536, 32 groups, GELU (3.2 TB/s; a plain
+// copy of that size takes 19 to 21), 93 to 98 us at 32x56x56x1024, 64 groups, SiLU,
+// bf16 (4.2 to 4.4 TB/s), 53 us with a checkpoint at 64x56x56x128 (2.4 TB/s).  What
+// bounds it then is issue: 13 instructions a value, 48 with a checkpoint's block
+// maxima, exponents and codes, and CTAs of one wave that load and compute in step.
 #include <cuda_runtime.h>
 
 #include "../../include/dwconv_b200.h"
