@@ -457,10 +457,14 @@ static bool gn_resident_fill(const GnShape& s, GnPass pass, int slab, int cluste
 // threads.  Where that makes eight CTAs an SM or more, CTAs of half the threads, eight to an SM: 31.5 us there, 92.7 against 97.5 us at 56x56x1024, B = 32, 47.0 against 50.8 us with a checkpoint at 56x56x128, B = 64.  What
 // needs more goes to the streaming passes (one group over 32x32x768, B = 8: 8 CTAs of 196 KB 14.2 us, 16 of 98 KB
 // 11.4 us, streaming 11.2 us).
-// Backward, the streaming passes are faster from about 7 CTAs an SM on: 32x32x1536 with B = 2 / 4 / 8 / 16, resident
-// 12.5 / 24.3 / 44.1 / 81 us, streaming 17.9 / 25.9 / 41.2 / 67 us; a cluster's exchange (3.7 us) is too long for the
-// little that four CTAs an SM bring along.  Forward the resident kernels stay ahead at every size (56x56x1024,
-// B = 32: 97 against 119 us): they move two thirds of the data.
+// Backward, the streaming passes are faster where clusters have more than about 1.75 turns of the CTAs that run at
+// once, because a cluster's exchange (3.7 us) is too long for the little that two or four CTAs an SM bring along.
+// Four an SM: 32x32x1536 with B = 2 / 4 / 8 / 16, resident 12.3 / 23.8 / 42.1 / 81 us, streaming 16.2 / 24.1 / 37.2 /
+// 63 us; two an SM, from a checkpoint: 56x56x768 with B = 2 / 4 / 8, 18.6 / 41.7 / 81.4 and 24.0 / 38.6 / 57.8 us.
+// CTAs by themselves have no exchange: 14x14x512 with B = 128 / 512, GELU, 35.0 / 122 and 41.0 / 136 us; 7x7x768,
+// B = 256, no activation, 30.7 and 36.2 us (at worst 64.8 against 60.6 us: 7x7x1024, B = 256, from a checkpoint).
+// Forward the resident kernels stay ahead at every size (56x56x1024, B = 32: 97 against 119 us): they move two thirds
+// of the data.
 bool gn_resident_plan(const GnShape& s, GnPass pass, GnResident* p) {
   // shared memory of eight, four and two CTAs an SM: 228 KB less 1 KB each
   constexpr int kEight = 27 * 1024 + 512, kFour = 56 * 1024, kTwo = 113 * 1024;
@@ -485,7 +489,8 @@ bool gn_resident_plan(const GnShape& s, GnPass pass, GnResident* p) {
         while (static_cast<long long>(s.B) * p->slabs * p->cluster < 2 * kSmCount && p->cluster < 8 && p->iters > 4 &&
                gn_resident_fill(s, pass, unit, p->cluster * 2, kGnThreads, limit, &wider))
           *p = wider;
-        return pass == GnPass::kForward || static_cast<long long>(s.B) * p->slabs * p->cluster <= 7 * kSmCount;
+        return pass == GnPass::kForward || p->cluster == 1 ||
+               static_cast<long long>(s.B) * p->slabs * p->cluster * 4 <= 7LL * kSmCount * (p->smem <= kFour ? 4 : 2);
       }
   return false;
 }

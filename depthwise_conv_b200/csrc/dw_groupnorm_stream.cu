@@ -562,9 +562,8 @@ __global__ void __launch_bounds__(kThreads, 3)
 
 static int gcd_int(int a, int b) { return b == 0 ? a : gcd_int(b, a % b); }
 
-// Row chunks: about `want` CTAs a group of samples, at least 8 pixels a thread.
-static void stream_rows(long long P, int rl, long long ctas_per_chunk, long long want, int* rows, int* chunks) {
-  long long n = (want + ctas_per_chunk - 1) / ctas_per_chunk;
+// Row chunks: `n`, with at least 8 pixels a thread.
+static void stream_rows(long long P, int rl, long long n, int* rows, int* chunks) {
   const long long most = (P + 8LL * rl - 1) / (8LL * rl);
   n = n < most ? n : most;
   n = n < 1 ? 1 : n;
@@ -608,10 +607,12 @@ bool gn_stream_plan(const GnShape& s, int bytes_per_value, GnStream* q) {
   const long long groups = (s.B + samples - 1) / samples;
   q->samples = static_cast<int>((s.B + groups - 1) / groups);
   // CTAs of a pass: about as many as run at once (3 an SM), long ones: more, shorter ones pay their ramp more often
-  // (32x32x1536, B = 16, gradient: 67 us with 2 and 3 an SM, 70 with 3 and 5; forward 39 us with 3, 45 with 9)
-  stream_rows(s.P, q->rl, static_cast<long long>(q->tiles) * q->samples, (bytes_per_value > 2 ? 2LL : 3LL) * kSmCount, &q->rows,
-              &q->chunks);
-  stream_rows(s.P, q->apply_rl, static_cast<long long>(q->apply_tiles) * q->samples, 3LL * kSmCount, &q->apply_rows,
+  // (32x32x1536, B = 16, gradient: 67 us with 2 and 3 an SM, 70 with 3 and 5; forward 39 us with 3, 45 with 9).  Second
+  // pass: at most 4 an SM and as near as can be, since a few CTAs more than run at once are a turn of their own (56x56x128,
+  // B = 64, gradient from a checkpoint: 83.7 us with 448 CTAs, 77.1 with 576; 32x32x1536, B = 8: 39.5 with 480, 37.2 with 576)
+  const long long a_chunk = static_cast<long long>(q->tiles) * q->samples, want = (bytes_per_value > 2 ? 2 : 3) * kSmCount;
+  stream_rows(s.P, q->rl, (want + a_chunk - 1) / a_chunk, &q->rows, &q->chunks);
+  stream_rows(s.P, q->apply_rl, 4 * kSmCount / (static_cast<long long>(q->apply_tiles) * q->samples), &q->apply_rows,
               &q->apply_chunks);
   q->first_sample = q->second_sample = 0;
   q->first_ctas = q->second_ctas = 0;
