@@ -214,18 +214,21 @@ struct GnSums {
   }
 };
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-// Two sums at once: the shuffles of one hide those of the other.
+// Two or three sums at once: the shuffles of one hide those of the others.
 __device__ __forceinline__ void warp_sum2(float& a, float& b) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     a += __shfl_xor_sync(0xffffffffu, a, o);
     b += __shfl_xor_sync(0xffffffffu, b, o);
+  }
+}
+
+__device__ __forceinline__ void warp_sum3(float& a, float& b, float& c) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+    b += __shfl_xor_sync(0xffffffffu, b, o);
+    c += __shfl_xor_sync(0xffffffffu, c, o);
   }
 }
 
@@ -331,8 +334,7 @@ struct GnMerge {
           s2 += v.y + n * d * d;
         }
       }
-    warp_sum2(s1, s2);
-    s0 = warp_sum(s0);
+    warp_sum3(s0, s1, s2);
     if (!rows) return make_float2(0.0f, 0.0f);
     const float n = static_cast<float>(rows) * static_cast<float>(channels), d = s1 / n;
     return make_float2(gn_mean(pivot, d, s0 / n), not_negative(s2 - s1 * d));

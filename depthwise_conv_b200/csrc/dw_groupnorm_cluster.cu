@@ -159,23 +159,36 @@ __global__ void __launch_bounds__(kGnThreads, 4)
   } else {
     __syncthreads();
   }
-  // a lane a rank: all of the cluster's moments of a group at once, added up the same way in every CTA
-  for (int g = tid >> 5; g < here; g += warps) {
-    float mean = grp[g].x, m2 = grp[g].y;
+  // a lane a rank, four groups a warp: all of the cluster's moments of a group at once, added up the same way in every CTA
+  const int rank = lane & 7;
+  const float all = static_cast<float>(s.P) * static_cast<float>(s.Cg);
+  for (int g0 = (tid >> 5) * 4; g0 < here; g0 += warps * 4) {
+    const int g = g0 + (lane >> 3);
+    const bool on = g < here;
+    float mean = 0.0f, m2 = 0.0f;
     if (p.cluster > 1) {
       // about rank 0's mean (rank 0 always has pixels)
-      const float n = lane < p.cluster ? static_cast<float>(GnPlace::rows_of(s, p, lane)) * static_cast<float>(s.Cg) : 0.0f;
-      const float2 v = lane < p.cluster ? cluster_load(grp + g, lane) : make_float2(0.0f, 0.0f);
-      const float pivot = __shfl_sync(0xffffffffu, v.x, 0), d = v.x - pivot;
+      const bool has = on && rank < p.cluster;
+      const float n = has ? static_cast<float>(GnPlace::rows_of(s, p, rank)) * static_cast<float>(s.Cg) : 0.0f;
+      const float2 v = has ? cluster_load(grp + g, rank) : make_float2(0.0f, 0.0f);
+      const float pivot = __shfl_sync(0xffffffffu, v.x, lane & 24), d = v.x - pivot;
       // a CTA without pixels has no weight
-      float s1 = n > 0.0f ? n * d : 0.0f, s2 = n > 0.0f ? v.y + n * d * d : 0.0f;
-      warp_sum2(s1, s2);
-      const float all = static_cast<float>(s.P) * static_cast<float>(s.Cg), off = s1 / all;
-      mean = gn_mean(pivot, off, warp_sum(n * v.x) / all);
+      float s0 = n * v.x, s1 = n > 0.0f ? n * d : 0.0f, s2 = n > 0.0f ? v.y + n * d * d : 0.0f;
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) {
+        s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+        s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+        s2 += __shfl_xor_sync(0xffffffffu, s2, o);
+      }
+      const float off = s1 / all;
+      mean = gn_mean(pivot, off, s0 / all);
       m2 = not_negative(s2 - s1 * off);
+    } else if (on) {
+      mean = grp[g].x;
+      m2 = grp[g].y;
     }
-    const float rstd = 1.0f / sqrtf(m2 / (static_cast<float>(s.P) * static_cast<float>(s.Cg)) + s.eps);
-    if (lane == 0) {
+    const float rstd = 1.0f / sqrtf(m2 / all + s.eps);
+    if (on && rank == 0) {
       fin[g] = make_float2(mean, rstd);
       if (at.rank == 0) {
         const long long o = at.sample * s.G + at.c_base / s.Cg + g;
@@ -454,8 +467,9 @@ static bool gn_resident_fill(const GnShape& s, GnPass pass, int slab, int cluste
 
 // The rule.  A unit's pixels are shared by the fewest CTAs (1 to 8) that hold them four to an SM, else two to an SM:
 // 32x32x1536, 32 groups, B = 16, forward: 32 us with 4 CTAs of 49 KB, 34 with 2 of 98 KB, 39 with 8 of 25 KB and as many
-// threads.  Where that makes eight CTAs an SM or more, CTAs of half the threads, eight to an SM: 31.5 us there, 92.7 against 97.5 us at 56x56x1024, B = 32, 47.0 against 50.8 us with a checkpoint at 56x56x128, B = 64.  What
-// needs more goes to the streaming passes (one group over 32x32x768, B = 8: 8 CTAs of 196 KB 14.2 us, 16 of 98 KB
+// threads.  Where that makes eight CTAs an SM or more, CTAs of half the threads, seven or eight to
+// an SM: 31.8 us there, 95 against 97.5 us at 56x56x1024, B = 32, 47.5 against 51.3 us with a checkpoint at 56x56x128,
+// B = 64.  What needs more goes to the streaming passes (one group over 32x32x768, B = 8: 8 CTAs of 196 KB 14.2 us, 16 of 98 KB
 // 11.4 us, streaming 11.2 us).
 // Backward, the streaming passes are faster where clusters have more than about 1.75 turns of the CTAs that run at
 // once, because a cluster's exchange (3.7 us) is too long for the little that two or four CTAs an SM bring along.
@@ -466,18 +480,18 @@ static bool gn_resident_fill(const GnShape& s, GnPass pass, int slab, int cluste
 // Forward the resident kernels stay ahead at every size (56x56x1024, B = 32: 97 against 119 us): they move two thirds
 // of the data.
 bool gn_resident_plan(const GnShape& s, GnPass pass, GnResident* p) {
-  // shared memory of eight, four and two CTAs an SM: 228 KB less 1 KB each
-  constexpr int kEight = 27 * 1024 + 512, kFour = 56 * 1024, kTwo = 113 * 1024;
+  // shared memory of seven, four and two CTAs an SM: 228 KB less 1 KB each
+  constexpr int kSmall = 31 * 1024 + 512, kFour = 56 * 1024, kTwo = 113 * 1024;
   // whole groups; forward: whole blocks of a checkpoint (with and without one: the same plan, the same bits), backward:
   // whole vectors and, where it can be, 64 bytes of a pixel
   const int align = pass == GnPass::kForward ? kAct8Block : 8;
   const long long unit_ll = static_cast<long long>(s.Cg) / gcd_int(s.Cg, align) * align;
   int unit = unit_ll < s.C ? static_cast<int>(unit_ll) : s.C;
   for (int k = unit; unit < 32 && unit < s.C;) unit = unit + k < s.C ? unit + k : s.C;
-  // many units: small CTAs, eight to an SM, that are seldom in the same phase
+  // many units: small CTAs that are seldom in the same phase
   if (pass == GnPass::kForward)
     for (int cluster = 1; cluster <= 8; cluster *= 2)
-      if (gn_resident_fill(s, pass, unit, cluster, kGnThreads / 2, kEight, p)) {
+      if (gn_resident_fill(s, pass, unit, cluster, kGnThreads / 2, kSmall, p)) {
         if (static_cast<long long>(s.B) * p->slabs * cluster < 8 * kSmCount) break;
         return true;
       }

@@ -189,8 +189,7 @@ __device__ __forceinline__ void merge_stats(const float2* __restrict__ part, con
       s1 += n * d;
       s2 += v.y + n * d * d;
     }
-    warp_sum2(s1, s2);
-    s0 = warp_sum(s0);
+    warp_sum3(s0, s1, s2);
     const float n = static_cast<float>(s.P) * static_cast<float>(s.Cg), off = s1 / n;
     const float mean = gn_mean(pivot, off, s0 / n), rstd = 1.0f / sqrtf(not_negative(s2 - s1 * off) / n + s.eps);
     if (lane == 0) {
