@@ -14,9 +14,9 @@
 // bits in every CTA and on every run.
 //
 // Measured, forward: 31.9 us at 16x32x32x1536, 32 groups, GELU (3.2 TB/s; a plain
-// copy of that size takes 19 to 21), 93 to 98 us at 32x56x56x1024, 64 groups, SiLU,
-// bf16 (4.2 to 4.4 TB/s), 53 us with a checkpoint at 64x56x56x128 (2.4 TB/s).  What
-// bounds it then is issue: 13 instructions a value, 48 with a checkpoint's block
+// copy of that size takes 19 to 21), 93 to 100 us at 32x56x56x1024, 64 groups, SiLU,
+// bf16 (4.1 to 4.4 TB/s), 45 us with a checkpoint at 64x56x56x128 (2.9 TB/s).  What
+// bounds it then is issue: 25 instructions a value, 36 with a checkpoint's block
 // maxima, exponents and codes, and CTAs of one wave that load and compute in step.
 #include <cuda_runtime.h>
 
@@ -159,7 +159,8 @@ __global__ void __launch_bounds__(kGnThreads, 4)
   } else {
     __syncthreads();
   }
-  // a lane a rank, four groups a warp: all of the cluster's moments of a group at once, added up the same way in every CTA
+  // a lane a rank, four groups a warp: all of the cluster's moments of a group at once, added up the same way in every
+  // CTA (one group a warp: 37.9 us at 64x56x56x128 with 32 groups, so 34.7)
   const int rank = lane & 7;
   const float all = static_cast<float>(s.P) * static_cast<float>(s.Cg);
   for (int g0 = (tid >> 5) * 4; g0 < here; g0 += warps * 4) {

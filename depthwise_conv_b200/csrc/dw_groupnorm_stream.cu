@@ -3,9 +3,9 @@
 // gradient), which merges the partial sums it needs first.  The formulas stand
 // in dw_groupnorm.cuh.
 //
-// Measured, gradient: 65.9 us at 16x32x32x1536, 32 groups, GELU; 197 us at
-// 32x56x56x1024.  Each pass reads dy and the input, 252 MB with dx in the first of
-// these, 3.8 TB/s, and issues 12 instructions a value (27 to 29 from a checkpoint),
+// Measured, gradient: 65.9 us at 16x32x32x1536, 32 groups, GELU; 186 us at
+// 32x56x56x1024, SiLU.  Each pass reads dy and the input, 252 MB with dx in the first of
+// these, 3.8 TB/s, and issues 24 instructions a value (27 to 30 from a checkpoint),
 // most of them for the activation's slope, which both passes compute: keeping it
 // would write and read 2 bytes a value more.
 //
