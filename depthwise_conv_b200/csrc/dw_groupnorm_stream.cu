@@ -74,6 +74,7 @@ __device__ __forceinline__ void wait_batch() {
 constexpr int kForwardRing = kForwardBatches * kBatch * kThreads * 16;
 constexpr int kBackwardRing = kBackwardBatches * kBatch * kThreads * 16;  // of dy
 constexpr int kFinMost = kApplyLanes * 8 + 1;  // groups that 128 channels can belong to
+constexpr int kFinBytes = kFinMost * 8 + kThreads / 32 * 3 * 4;  // and the sums of warps that share a group
 
 // The first launch of a call waits for the kernel before it, which may make its inputs.  The others read nothing but
 // what that launch could read, and the entries of the launch before them: they begin to load first (q.early), while
@@ -161,6 +162,28 @@ __device__ __forceinline__ void stats_cta(const T* __restrict__ x, float2* __res
     gn_hand_over<SUB>(mean, m2, static_cast<float>(n), ent + tid * kEnt);
   }
   __syncthreads();
+  if constexpr (SUB == 1) {
+    if (q.entries_per_group > 1) {  // single channels: a thread each, over the lane rows (a warp each: 22.0 us, so 10.1,
+      // at 1x36x18x1208, 4 groups)
+      const int live = min(t.rows, q.rl), full = t.rows / q.rl, rest = t.rows - full * q.rl;
+      for (int j = tid; j < tile.width; j += kThreads) {
+        const float pivot = ent[j].x;
+        float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f;
+#pragma unroll 4
+        for (int r = 0; r < live; ++r) {
+          const float2 v = ent[r * q.lanes * kEnt + j];
+          const float m = static_cast<float>(full + (r < rest)), d = v.x - pivot;
+          s0 += m * v.x;
+          s1 += m * d;
+          s2 += v.y + m * d * d;
+        }
+        const float rows = static_cast<float>(t.rows), off = s1 / rows;
+        part[(static_cast<long long>(sample) * q.chunks + chunk) * q.entries + tile.entry + j] =
+            make_float2(gn_mean(pivot, off, s0 / rows), not_negative(s2 - s1 * off));
+      }
+      return;
+    }
+  }
   const int lane = tid & 31, segments = tile.width / tile.seg;
   const GnMerge merge(lane, tile.seg / SUB, t.rows, q.rl, q.lanes * kEnt);
   for (int g = tid >> 5; g < segments; g += kThreads / 32) {
@@ -169,30 +192,70 @@ __device__ __forceinline__ void stats_cta(const T* __restrict__ x, float2* __res
   }
 }
 
+// How a CTA's warps share the entries of its groups: a warp a group, or with SHARE (an entry may be a channel) `split`
+// warps a group where it has few groups of many entries (1x36x18x1208, 4 groups: 302 entries a group and chunk).
+template <bool SHARE>
+struct EntryShare {
+  int split = 1, of, slice = 0;
+  __device__ __forceinline__ EntryShare(int groups, int entries) {
+    of = threadIdx.x >> 5;
+    if constexpr (SHARE) {
+      while (split * 2 * groups <= kThreads / 32 && split * 64 <= entries) split *= 2;
+      slice = of % split;
+      of /= split;
+    }
+  }
+  __device__ __forceinline__ int groups_at_once() const { return kThreads / 32 / split; }  // all of them where split > 1
+  // The sums of a group's warps, in order, in the first of them; `sums` has three places a warp.  Every thread of the
+  // CTA calls it.
+  __device__ __forceinline__ void add(float& a, float& b, float& c, float* sums) const {
+    if (!SHARE || split == 1) return;
+    float* const mine = sums + 3 * (threadIdx.x >> 5);
+    if ((threadIdx.x & 31) == 0) {
+      mine[0] = a;
+      mine[1] = b;
+      mine[2] = c;
+    }
+    __syncthreads();
+    if (slice == 0)
+      for (int i = 1; i < split; ++i) {
+        a += mine[3 * i];
+        b += mine[3 * i + 1];
+        c += mine[3 * i + 2];
+      }
+  }
+};
+
 // Mean and rstd of the groups that channels [c0, c0 + width) belong to, from their entries.
+template <bool SHARE>
 __device__ __forceinline__ void merge_stats(const float2* __restrict__ part, const GnShape& s, const GnStream& q, int sample, int c0,
                                             int width, float2* fin, float* mean_out, float* rstd_out) {
   const int lane = threadIdx.x & 31, g0 = c0 / s.Cg, g1 = (c0 + width - 1) / s.Cg, per = q.entries_per_group;
   const float2* of_sample = part + static_cast<long long>(sample) * q.chunks * q.entries;
   const int last = static_cast<int>(s.P) - (q.chunks - 1) * q.rows;
-  for (int g = g0 + (threadIdx.x >> 5); g <= g1; g += kThreads / 32) {
-    const float2* first = of_sample + g * per;
-    // about the first entry's mean: entries are means of many values, nothing cancels in the squares
-    const float pivot = first[0].x;
-    float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f;
-    for (int e = lane; e < q.chunks * per; e += 32) {
-      const int chunk = e / per, k = e - chunk * per;
-      const float2 v = first[static_cast<long long>(chunk) * q.entries + k];
-      const float n = static_cast<float>(chunk == q.chunks - 1 ? last : q.rows) * static_cast<float>(entry_width(s, q, k));
-      const float d = v.x - pivot;
-      s0 += n * v.x;
-      s1 += n * d;
-      s2 += v.y + n * d * d;
+  const EntryShare<SHARE> share(g1 - g0 + 1, q.chunks * per);
+  for (int next = g0; next <= g1; next += share.groups_at_once()) {
+    const int g = next + share.of;
+    float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f, pivot = 0.0f;
+    if (g <= g1) {
+      const float2* first = of_sample + g * per;
+      // about the first entry's mean: entries are means of many values, nothing cancels in the squares
+      pivot = first[0].x;
+      for (int e = share.slice * 32 + lane; e < q.chunks * per; e += 32 * share.split) {
+        const int chunk = e / per, k = e - chunk * per;
+        const float2 v = first[static_cast<long long>(chunk) * q.entries + k];
+        const float n = static_cast<float>(chunk == q.chunks - 1 ? last : q.rows) * static_cast<float>(entry_width(s, q, k));
+        const float d = v.x - pivot;
+        s0 += n * v.x;
+        s1 += n * d;
+        s2 += v.y + n * d * d;
+      }
     }
     warp_sum3(s0, s1, s2);
+    share.add(s0, s1, s2, reinterpret_cast<float*>(fin + kFinMost));
     const float n = static_cast<float>(s.P) * static_cast<float>(s.Cg), off = s1 / n;
     const float mean = gn_mean(pivot, off, s0 / n), rstd = 1.0f / sqrtf(not_negative(s2 - s1 * off) / n + s.eps);
-    if (lane == 0) {
+    if (g <= g1 && share.slice == 0 && lane == 0) {
       fin[g - g0] = make_float2(mean, rstd);
       if (mean_out && g * s.Cg >= c0) {
         mean_out[static_cast<long long>(sample) * s.G + g] = mean;
@@ -228,7 +291,7 @@ __device__ __forceinline__ void apply_cta(const T* __restrict__ x, const void* _
   f32x2 w[4], b[4], m[kParts];
   if (active) gn_load_params<T>(weight, bias, c, s, w, b);
   // the CTA of a chunk's first rows and of a group's first channels writes the group's mean and rstd
-  merge_stats(part, s, q, sample, c0, width, fin, chunk == 0 ? mean_out : nullptr, rstd_out);
+  merge_stats<SUB == 1>(part, s, q, sample, c0, width, fin, chunk == 0 ? mean_out : nullptr, rstd_out);
   if (active) {
     f32x2 rs[kParts];
     gn_read_groups<SUB>(fin, c, s.Cg, c0 / s.Cg, m, rs);
@@ -436,8 +499,11 @@ __device__ __forceinline__ void grad_sums_cta(const T* __restrict__ dy, const vo
     }
     chan[row * s.C + tile.c0 + j] = a;
     const float wj = gn_param<T>(weight, tile.c0 + j, s.param_f32, 1.0f);
-    ent[j] = make_float2(a.x * wj, a.y * wj);  // lane row 0's place of this channel: this thread has just read it
+    a = make_float2(a.x * wj, a.y * wj);
+    if (q.entries_per_group > 1 && q.tiles_per_group == 1) part[row * q.entries + tile.entry + j] = a;  // single channels
+    else ent[j] = a;  // lane row 0's place of this channel: this thread has just read it
   }
+  if (q.entries_per_group > 1 && q.tiles_per_group == 1) return;
   __syncthreads();
   const int lane = tid & 31, segments = tile.width / tile.seg;
   for (int g = tid >> 5; g < segments; g += kThreads / 32) {
@@ -489,17 +555,22 @@ __device__ __forceinline__ void grad_apply_cta(const T* __restrict__ dy, const v
   {
     const int lane = threadIdx.x & 31, g0 = c0 / s.Cg, g1 = (c0 + width - 1) / s.Cg, per = q.entries_per_group;
     const float inv = 1.0f / (static_cast<float>(s.P) * static_cast<float>(s.Cg));
-    for (int g = g0 + (threadIdx.x >> 5); g <= g1; g += kThreads / 32) {
-      const float2* entry = part + static_cast<long long>(sample) * q.chunks * q.entries + g * per;
-      float m1 = 0.0f, m2 = 0.0f;
-      for (int e = lane; e < q.chunks * per; e += 32) {
-        const int k = e / per;
-        const float2 v = entry[static_cast<long long>(k) * q.entries + (e - k * per)];
-        m1 += v.x;
-        m2 += v.y;
+    const EntryShare<SUB == 1> share(g1 - g0 + 1, q.chunks * per);
+    for (int next = g0; next <= g1; next += share.groups_at_once()) {
+      const int g = next + share.of;
+      float m1 = 0.0f, m2 = 0.0f, none = 0.0f;
+      if (g <= g1) {
+        const float2* entry = part + static_cast<long long>(sample) * q.chunks * q.entries + g * per;
+        for (int e = share.slice * 32 + lane; e < q.chunks * per; e += 32 * share.split) {
+          const int k = e / per;
+          const float2 v = entry[static_cast<long long>(k) * q.entries + (e - k * per)];
+          m1 += v.x;
+          m2 += v.y;
+        }
       }
       warp_sum2(m1, m2);
-      if (lane == 0) fin[g - g0] = make_float2(m1 * inv, -m2 * inv);
+      share.add(m1, m2, none, reinterpret_cast<float*>(fin + kFinMost));
+      if (g <= g1 && share.slice == 0 && lane == 0) fin[g - g0] = make_float2(m1 * inv, -m2 * inv);
     }
     __syncthreads();
   }
@@ -684,6 +755,7 @@ int gn_stream_forward(const void* x, const void* weight, const void* bias, void*
                       void* scales, float2* part, const GnShape& shape, const GnStream& plan, int act, cudaStream_t stream) {
   const void* fn = codes ? stream_fn<T, true>(plan.sub, act) : stream_fn<T, false>(plan.sub, act);
   GnShape s = shape;
+  static_assert(kFinBytes <= kThreads * static_cast<int>(sizeof(float2)), "the second pass in the first one's entries");
   const int smem = kForwardRing + kThreads * (8 / plan.sub) * static_cast<int>(sizeof(float2));
   return stream_groups(shape, plan, [&](GnStream q, dim3 grid) {
     void* args[] = {&x, &weight, &bias, &part, &y, &mean, &rstd, &codes, &scales, &s, &q};
@@ -699,7 +771,7 @@ int gn_stream_backward(const void* dy, const void* x, const void* codes, const v
       codes ? stream_grad_fn<T, true>(plan.sub, act) : stream_grad_fn<T, false>(plan.sub, act);
   const void* src = codes ? codes : x;
   GnShape s = shape;
-  const int smem = kBackwardRing * (codes ? 3 : 4) / 2 + kFinMost * static_cast<int>(sizeof(float2));
+  const int smem = kBackwardRing * (codes ? 3 : 4) / 2 + kFinBytes;
   return stream_groups(shape, plan, [&](GnStream q, dim3 grid) {
     void* args[] = {&dy, &src, &scales, &weight, &bias, &mean, &rstd, &part, &chan, &dx, &s, &q};
     return stream_launch(fn, "gn_stream_grad_kernel", grid, smem, args, stream);

@@ -730,3 +730,18 @@ def test_a_gradient_off_the_vector_boundary(eng):
     torch.cat([odd, y.flatten()]).backward(dy)
     want = torch.autograd.grad(eng.group_norm_act(x, 4, act="gelu"), x, dy[3:].clone().view(3, 32, 1, 1))[0]
     assert torch.equal(x.grad, want)
+
+
+@pytest.mark.parametrize("shape", [(1, 36, 18, 1208, 4), (4, 28, 28, 1544, 8), (1, 5, 3, 1032, 2), (2, 90, 70, 4104, 8)])
+def test_large_groups_of_odd_sizes(eng, shape):
+    """Groups too large for a tile and no multiple of 8 channels: an entry a channel, few groups of many entries."""
+    B, H, W, C, G = shape
+    x, dy = nhwc(B, C, H, W, 1, torch.float16), nhwc(B, C, H, W, 2, torch.float16, offset=0.1)
+    w, b = params(C, 3, torch.float32)
+    out = eng.norm_ops.group_norm_act_forward(x, G, w, b, act="gelu", checkpoint=True)
+    check_forward(out, x, G, w, b, 1e-5, "gelu")
+    assert all(torch.equal(i, j) for i, j in zip(out[3:], eng.act8_encode(x)))
+    mean, rstd = (t.float() for t in R.stats(x, G, 1e-5))
+    for kept, values in ((x, x), (out[3:], R.act8_decode(*R.act8_encode(x)))):
+        got = eng.norm_ops.group_norm_act_backward(dy, kept, mean, rstd, G, w, b, "gelu")
+        check_backward(got, dy, values, mean, rstd, G, w, b, "gelu")
