@@ -476,8 +476,8 @@ static bool gn_resident_fill(const GnShape& s, GnPass pass, int slab, int cluste
 // once, because a cluster's exchange (3.7 us) is too long for the little that two or four CTAs an SM bring along.
 // Four an SM: 32x32x1536 with B = 2 / 4 / 8 / 16, resident 12.3 / 23.8 / 42.1 / 81 us, streaming 16.2 / 24.1 / 37.2 /
 // 63 us; two an SM, from a checkpoint: 56x56x768 with B = 2 / 4 / 8, 18.6 / 41.7 / 81.4 and 24.0 / 38.6 / 57.8 us.
-// CTAs by themselves have no exchange: 14x14x512 with B = 128 / 512, GELU, 35.0 / 122 and 41.0 / 136 us; 7x7x768,
-// B = 256, no activation, 30.7 and 36.2 us (at worst 64.8 against 60.6 us: 7x7x1024, B = 256, from a checkpoint).
+// CTAs by themselves have no exchange: 14x14x512 with B = 128 / 512, GELU, 35.0 / 122 and 41.0 / 136 us (at worst, B = 256
+// without activation, 56.5 and 53.1 us).
 // Forward the resident kernels stay ahead at every size (56x56x1024, B = 32: 97 against 119 us): they move two thirds
 // of the data.
 bool gn_resident_plan(const GnShape& s, GnPass pass, GnResident* p) {
@@ -489,6 +489,12 @@ bool gn_resident_plan(const GnShape& s, GnPass pass, GnResident* p) {
   const long long unit_ll = static_cast<long long>(s.Cg) / gcd_int(s.Cg, align) * align;
   int unit = unit_ll < s.C ? static_cast<int>(unit_ll) : s.C;
   for (int k = unit; unit < 32 && unit < s.C;) unit = unit + k < s.C ? unit + k : s.C;
+  // few pixels: more units a CTA, until it has 512 vectors of 8 channels or an SM would go without (7x7x1024, 32 groups,
+  // B = 256: forward 35.7 us with one unit of 32 channels, 20.3 so, gradient 59 and 34.5; with 1024 vectors the gradient
+  // 70.2).  At most 1024 channels, a thread for every vector of a pixel.
+  for (const int k = unit; unit + k <= s.C && unit + k <= 8 * kGnThreads / 2 && s.P * unit < 8 * 512 &&
+                           static_cast<long long>(s.B) * ((s.C + unit + k - 1) / (unit + k)) >= kSmCount;)
+    unit += k;
   // many units: small CTAs that are seldom in the same phase
   if (pass == GnPass::kForward)
     for (int cluster = 1; cluster <= 8; cluster *= 2)

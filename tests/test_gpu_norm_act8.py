@@ -745,3 +745,20 @@ def test_large_groups_of_odd_sizes(eng, shape):
     for kept, values in ((x, x), (out[3:], R.act8_decode(*R.act8_encode(x)))):
         got = eng.norm_ops.group_norm_act_backward(dy, kept, mean, rstd, G, w, b, "gelu")
         check_backward(got, dy, values, mean, rstd, G, w, b, "gelu")
+
+
+@pytest.mark.parametrize("shape", [(160, 1, 1, 1024, 32), (150, 2, 2, 2048, 4), (100, 3, 3, 768, 768), (75, 7, 4, 1424, 356),
+                                   (149, 1, 2, 1208, 151), (37, 7, 7, 1024, 32)])
+def test_batches_of_few_pixels(eng, shape):
+    """CTAs that take many units of channels, up to as many as they have threads for."""
+    B, H, W, C, G = shape
+    x, dy = nhwc(B, C, H, W, 1, torch.float16), nhwc(B, C, H, W, 2, torch.float16, offset=0.1)
+    w, b = params(C, 3, torch.float16)
+    out = eng.norm_ops.group_norm_act_forward(x, G, w, b, act="silu", checkpoint=True)
+    check_forward(out, x, G, w, b, 1e-5, "silu")
+    assert all(torch.equal(i, j) for i, j in zip(out[:3], eng.norm_ops.group_norm_act_forward(x, G, w, b, act="silu")))
+    assert all(torch.equal(i, j) for i, j in zip(out[3:], eng.act8_encode(x)))
+    mean, rstd = (t.float() for t in R.stats(x, G, 1e-5))
+    for kept, values in ((x, x), (out[3:], R.act8_decode(*R.act8_encode(x)))):
+        got = eng.norm_ops.group_norm_act_backward(dy, kept, mean, rstd, G, w, b, "silu")
+        check_backward(got, dy, values, mean, rstd, G, w, b, "silu")
