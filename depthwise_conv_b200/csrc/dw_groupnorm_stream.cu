@@ -251,6 +251,7 @@ __device__ __forceinline__ void merge_stats(const float2* __restrict__ part, con
         s2 += v.y + n * d * d;
       }
     }
+    if (!SHARE && g > g1) break;
     warp_sum3(s0, s1, s2);
     share.add(s0, s1, s2, reinterpret_cast<float*>(fin + kFinMost));
     const float n = static_cast<float>(s.P) * static_cast<float>(s.Cg), off = s1 / n;
@@ -489,6 +490,7 @@ __device__ __forceinline__ void grad_sums_cta(const T* __restrict__ dy, const vo
   }
   __syncthreads();
   const long long row = static_cast<long long>(sample) * q.chunks + chunk;
+  const bool single = SUB == 1 && q.entries_per_group > 1;  // an entry a channel
   for (int j = tid; j < tile.width; j += kThreads) {
     float2 a = make_float2(0.0f, 0.0f);
 #pragma unroll 8
@@ -500,10 +502,10 @@ __device__ __forceinline__ void grad_sums_cta(const T* __restrict__ dy, const vo
     chan[row * s.C + tile.c0 + j] = a;
     const float wj = gn_param<T>(weight, tile.c0 + j, s.param_f32, 1.0f);
     a = make_float2(a.x * wj, a.y * wj);
-    if (q.entries_per_group > 1 && q.tiles_per_group == 1) part[row * q.entries + tile.entry + j] = a;  // single channels
+    if (single) part[row * q.entries + tile.entry + j] = a;
     else ent[j] = a;  // lane row 0's place of this channel: this thread has just read it
   }
-  if (q.entries_per_group > 1 && q.tiles_per_group == 1) return;
+  if (single) return;
   __syncthreads();
   const int lane = tid & 31, segments = tile.width / tile.seg;
   for (int g = tid >> 5; g < segments; g += kThreads / 32) {
@@ -568,6 +570,7 @@ __device__ __forceinline__ void grad_apply_cta(const T* __restrict__ dy, const v
           m2 += v.y;
         }
       }
+      if (SUB != 1 && g > g1) break;  // no warp shares
       warp_sum2(m1, m2);
       share.add(m1, m2, none, reinterpret_cast<float*>(fin + kFinMost));
       if (g <= g1 && share.slice == 0 && lane == 0) fin[g - g0] = make_float2(m1 * inv, -m2 * inv);
