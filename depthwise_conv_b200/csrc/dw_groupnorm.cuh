@@ -49,8 +49,11 @@ __device__ __forceinline__ f32x2 act_value2(f32x2 u) {
   } else if constexpr (ACT == kActGelu) {
     // u Phi(u) = max(u, 0) - |u| Q(|u|) on both sides of 0: no selection
     const float2 f = bits_f2(u);
-    return fma2(u | 0x8000000080000000ull, normal_tail2(u & 0x7fffffff7fffffffull),
-                f2_bits(make_float2(fmaxf(f.x, 0.0f), fmaxf(f.y, 0.0f))));
+    // |u| stays finite in the product, whose other factor is 0 long before: an infinite u leaves max(u, 0); a NaN goes
+    // through Q
+    constexpr float kMost = 3.4028235e38f;
+    return fma2(f2_bits(make_float2(fmaxf(-fabsf(f.x), -kMost), fmaxf(-fabsf(f.y), -kMost))),
+                normal_tail2(u & 0x7fffffff7fffffffull), f2_bits(make_float2(fmaxf(f.x, 0.0f), fmaxf(f.y, 0.0f))));
   } else if constexpr (ACT == kActSilu) {
     const float2 e = bits_f2(fmul2(u, splat2(-1.4426950408889634f)));
     const f32x2 d = fma2(f2_bits(make_float2(ex2_approx(e.x), ex2_approx(e.y))), splat2(1.0f), splat2(1.0f));

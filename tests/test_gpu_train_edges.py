@@ -1,0 +1,53 @@
+"""Group norm, checkpoints and the weight gradient from a checkpoint at the ends of their ranges, on the GPU
+against float64 (oracle/train_ref.py).
+
+Bounds as in test_gpu_norm_act8.py: one rounding to the output's type, 64 e32 (e32 = 2^-24) of the terms'
+magnitudes for what a value passes through in fp32.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from oracle import train_ref as R
+
+pytestmark = pytest.mark.gpu
+
+E32 = 2.0**-24
+
+
+@pytest.fixture(scope="module")
+def eng():
+    import depthwise_conv_b200 as d
+    return d
+
+
+def of_bias(eng, u, act, dtype, P=5, G=1):
+    """act(u) through the norm: with a weight of 0 the activation's input is the bias.  [C] in float64.
+
+    G = 1 and P = 5 run in the resident kernel."""
+    C = u.numel()
+    g = torch.Generator(device="cuda").manual_seed(C)
+    x = torch.randn(1, P, 1, C, device="cuda", generator=g).to(dtype).permute(0, 3, 1, 2)
+    y = eng.norm_ops.group_norm_act_forward(x, G, torch.zeros(C, device="cuda"), u.float().cuda(), act=act)[0]
+    assert torch.equal(y.float().nan_to_num(7), y[:, :, :1].float().nan_to_num(7).expand_as(y)), "pixels differ"
+    return y[0, :, 0, 0].double()
+
+
+@pytest.mark.parametrize("act,ends", [("gelu", (math.inf, 0.0)), ("relu", (math.inf, 0.0)), ("none", (math.inf, -math.inf))])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("P", [5, 100000])
+def test_infinite_activation_inputs(eng, act, ends, dtype, P):
+    """An activation's input that is infinite (here the bias) gives the activation's limit, a NaN a NaN, and the
+    channels beside it their own values; P = 5 in shared memory, 100000 in two passes."""
+    u = torch.zeros(64, dtype=torch.float64)
+    u[3], u[8], u[17], u[40] = math.inf, -math.inf, math.nan, 2.0
+    y = of_bias(eng, u, act, dtype, P)
+    assert y[3] == ends[0] and y[8] == ends[1] and torch.isnan(y[17])
+    two = R.act_and_slope(u[40], act)[0].item()
+    assert abs(y[40] - two) <= 2.0**-8 * two
+    rest = torch.ones(64, dtype=torch.bool)
+    rest[[3, 8, 17, 40]] = False
+    assert (y[rest.cuda()] == 0).all()
