@@ -26,18 +26,19 @@ namespace dwb {
 
 enum : int { kActSilu = 3 };  // after kActNone, kActRelu, kActGelu
 
-// Q(a) = erfc(a / sqrt 2) / 2 for a >= 0 as 2^P(a): log2 Q is so smooth that a polynomial of degree 8 has |Q| to
-// 6e-8 and a Q to 3.5e-8 (a weighted least-squares fit on [0, 5.5], reweighted towards its largest error); further
-// out P goes on falling and a Q stays below 1e-7.  One special-function operation a value.
+// Q(a) = erfc(a / sqrt 2) / 2 for a >= 0 as 2^P(a): log2 Q is so smooth that a polynomial of degree 8 (a weighted
+// least-squares fit on [0, 8], reweighted towards its largest error) has a Q to 7.5e-8 and, up to a = 8, to 1.5e-3 of
+// itself: GELU's small values below zero are a Q alone, and half a step of bf16 is 3.9e-3 of a value.  Further out P
+// falls faster than log2 Q: 6% of a Q are missing at a = 9, where it is 1e-18.  One special-function operation a value.
 __device__ __forceinline__ f32x2 normal_tail2(f32x2 a) {
-  f32x2 p = fma2(splat2(-2.0400157e-06f), a, splat2(2.9838166e-05f));
-  p = fma2(p, a, splat2(-0.00014074291f));
-  p = fma2(p, a, splat2(-0.00024707115f));
-  p = fma2(p, a, splat2(0.0072080679f));
-  p = fma2(p, a, splat2(-0.0525972135f));
-  p = fma2(p, a, splat2(-0.459174216f));
-  p = fma2(p, a, splat2(-1.15110946f));
-  const float2 e = bits_f2(fma2(p, a, splat2(-0.99999988f)));
+  f32x2 p = fma2(splat2(-1.86687586e-07f), a, splat2(2.77648019e-06f));
+  p = fma2(p, a, splat2(1.80209154e-05f));
+  p = fma2(p, a, splat2(-0.000729526568f));
+  p = fma2(p, a, splat2(0.0080255894f));
+  p = fma2(p, a, splat2(-0.0533717498f));
+  p = fma2(p, a, splat2(-0.458785474f));
+  p = fma2(p, a, splat2(-1.15119958f));
+  const float2 e = bits_f2(fma2(p, a, splat2(-0.999993145f)));
   return f2_bits(make_float2(ex2_approx(e.x), ex2_approx(e.y)));
 }
 

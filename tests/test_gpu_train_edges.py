@@ -51,3 +51,22 @@ def test_infinite_activation_inputs(eng, act, ends, dtype, P):
     rest = torch.ones(64, dtype=torch.bool)
     rest[[3, 8, 17, 40]] = False
     assert (y[rest.cuda()] == 0).all()
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("P", [5, 5000])
+def test_small_values_of_an_activation(eng, act, dtype, P):
+    """Far below zero a value is small but still the activation's: little more than one rounding of the type.
+
+    GELU's tail a Q(a) is off by at most 7.5e-8 < 1.3 e32, its ex2 and its product by 1 e32 more (a Q <= 0.17): 4 e32;
+    and by at most 1.5e-3 < 2^-9 of itself up to |u| = 8.  The value's own fp32 operations, and SiLU's exponential,
+    quotient and the exponent's argument (below 2^4, rounded at e32 of itself), are within 32 e32 of the value."""
+    u = torch.linspace(-8, 8, 2048, dtype=torch.float64).float().double()
+    y = of_bias(eng, u, act, dtype, P).cpu()
+    ref = R.act_and_slope(u, act)[0]
+    half = 2.0**-11 if dtype == torch.float16 else 2.0**-8
+    finest = 2.0**-25 if dtype == torch.float16 else 0.0
+    tail = torch.minimum(torch.full_like(ref, 4 * E32), 2.0**-9 * ref.abs())
+    limit = half * ref.abs() + finest + tail + 32 * E32 * ref.abs()
+    assert ((y - ref).abs() <= limit).all(), ((y - ref).abs() / limit).max()
