@@ -70,3 +70,41 @@ def test_small_values_of_an_activation(eng, act, dtype, P):
     tail = torch.minimum(torch.full_like(ref, 4 * E32), 2.0**-9 * ref.abs())
     limit = half * ref.abs() + finest + tail + 32 * E32 * ref.abs()
     assert ((y - ref).abs() <= limit).all(), ((y - ref).abs() / limit).max()
+
+
+@pytest.mark.parametrize("shape,kept", [((70000, 1, 2, 16, 2), "input"), ((70000, 1, 2, 16, 2), "checkpoint"),
+                                        ((400000, 1, 2, 8, 1), "input")])
+def test_parameter_gradients_of_many_samples(eng, shape, kept):
+    """dweight and dbias where their sums over the samples are longest: gradients that are the same in every sample and
+    fill a float's 24 bits, so that a chain of additions loses the same way again and again.
+
+    In a sample (2 pixels at most) and over 32 partial sums fewer than 64 roundings, each at most e32 of the sum of the
+    magnitudes; none from the number of samples.  x_hat's and the slope's roundings: 8 e32 of each term, and mean * rstd
+    among x_hat's terms."""
+    B, H, W, C, G = shape
+    g = torch.Generator(device="cuda").manual_seed(B)
+    x = torch.randn(B, H, W, C, device="cuda", generator=g).half().permute(0, 3, 1, 2)
+    dy = torch.stack([torch.ones(C, device="cuda"), 1e-3 * (0.5 + torch.rand(C, device="cuda", generator=g))])
+    dy = dy.half().expand(B, H, W, C).contiguous().permute(0, 3, 1, 2)
+    w = torch.ones(C, device="cuda")
+    mean, rstd = (t.float() for t in R.stats(x, G, 1e-5))
+    saved = x if kept == "input" else eng.act8_encode(x)
+    values = x if kept == "input" else R.act8_decode(*saved)
+    _, dw, db = eng.norm_ops.group_norm_act_backward(dy, saved, mean, rstd, G, w, torch.zeros_like(w), "none")
+    xh = R.normalised(values, mean, rstd)
+    far = 1 + R._per_channel((mean.double() * rstd.double()).abs(), C)
+    sums, size = (dy.double() * xh).sum(dim=(0, 2, 3)), (dy.double() * (xh.abs() + far)).sum(dim=(0, 2, 3))
+    assert ((db.double() - dy.double().sum(dim=(0, 2, 3))).abs() <= 64 * E32 * dy.double().sum(dim=(0, 2, 3))).all()
+    assert ((dw.double() - sums).abs() <= 64 * E32 * size).all()
+
+
+def test_parameter_gradients_that_are_infinite(eng):
+    """An infinite gradient gives an infinite sum (and a NaN where two of them cancel), in its own channel only."""
+    x = torch.randn(40, 16, 3, 3, device="cuda").half().contiguous(memory_format=torch.channels_last)
+    dy = torch.ones_like(x)
+    dy[3, 4, 1, 1] = dy[30, 5, 0, 0] = math.inf
+    dy[0, 6, 0, 0], dy[39, 6, 2, 2] = math.inf, -math.inf
+    mean, rstd = (t.float() for t in R.stats(x, 2, 1e-5))
+    db = eng.norm_ops.group_norm_act_backward(dy, x, mean, rstd, 2, None, torch.zeros(16, device="cuda"), "none")[2]
+    assert db[4] == math.inf and db[5] == math.inf and torch.isnan(db[6])
+    assert (db[[0, 1, 2, 3, *range(7, 16)]] == 360).all()
