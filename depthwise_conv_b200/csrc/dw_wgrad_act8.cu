@@ -31,14 +31,18 @@
 // of odd taps are aligned words too; the rows of dy stand in a ring.  A warp owns
 // 4 channels and keeps their taps in the accumulators.  The codes and values of
 // the next two steps travel by cp.async into places that only their own thread
-// reads, so a step has one barrier.  Partial sums go to slices of the workspace
-// that a second kernel adds in order; a chain of accumulations is at most kChain
-// products long, because the tensor core's accumulator rounds towards zero, which
-// a long chain would turn into a bias.
+// reads, so a step has one barrier.  A CTA's sums go to its slice of the workspace,
+// and a second kernel adds the slices in order.  A chain of accumulations is at
+// most kChain products long, because the tensor core's accumulator rounds towards
+// zero, which a long chain would turn into a bias: then the accumulators are added
+// to the slice and begin again at zero, so that the slices are as many as the CTAs,
+// however long the batch.
 //
 // Measured (both kernels; the framework's 16-bit weight gradient on the CUDA
-// cores in brackets): 16x32x32x768 k7 36.7 us (64.3), 16x32x32x1536 k9 80.6 (182),
-// 8x56x56x1024 k13 137 (310), 8x56x56x128 k31 43 (171), 2x14x14x512 k27 11.7.
+// cores in brackets): 16x32x32x768 k7 34.4 us (64.3), 16x32x32x1536 k9 81.5 (182),
+// 8x56x56x1024 k13 114 (310), 8x56x56x128 k31 42 (171), 2x14x14x512 k27 11.2,
+// 56x56x1024 k31 245 with 8 images, 1732 with 64 (285 and 1905 when a chain's end was
+// a range's: 112 slices, 441 MB of workspace for the 64 images, where 9 are 35 MB).
 // What bounds it is the issue of the instructions around the products, most of
 // all the conversion and transposition of x and dy: at 16x32x32x768 k7 the
 // 38 MB read need 5.8 us and the products' FMAs on the CUDA cores would need
@@ -58,6 +62,8 @@ constexpr int kWgThreads = 256;
 constexpr int kWgChannels = 32;
 constexpr int kWgTile = 64;    // most columns of a tile
 constexpr int kChain = 128;    // most products added up in one accumulator
+constexpr int kTurns = 12;     // most turns of the CTAs that run at once
+constexpr int kFlushes = 256;  // most additions to a slice
 
 struct Wgrad8Params {
   int B, H, W, C, K;
@@ -129,13 +135,29 @@ struct Wgrad8 {
   static constexpr int kDItems = TW * 2;  // of a row of dy: 2 columns x 8 channels
   static constexpr int kBlocks = TW / 16;
   static constexpr int kAcc = PACK ? 1 : ROWS;
+  static constexpr int kMost = kChain / (kBlocks * SETS);  // steps of a chain
+  static constexpr int kTaps = PACK ? 8 : 16, kSumPitch = kWgChannels + 4;  // of the sums in shared memory
   typedef float Acc[4][kAcc][MT][NT][4];
+  static __device__ __forceinline__ void clear(Acc& acc) {
+#pragma unroll
+    for (int ch = 0; ch < 4; ++ch)
+#pragma unroll
+      for (int r = 0; r < kAcc; ++r)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[ch][r][m][n][i] = 0.0f;
+  }
 
   static constexpr int ring(int K) { return K - 1 + 2 * kStep; }
   static constexpr int x_items(int K) { return (TW + K - 1 + 3) / 4 * 4; }  // of a row of x
   static constexpr int fixed_words(int K) { return (2 * kXBuffer + ring(K) * kDRow + 3) / 4 * 4; }
   static constexpr int smem(int K) {
-    return 4 * fixed_words(K) + kAhead * kStep * (x_items(K) * 5 * 8 + kDItems * 2 * 16);
+    const int rows = 4 * fixed_words(K) + kAhead * kStep * (x_items(K) * 5 * 8 + kDItems * 2 * 16);
+    const int sums = 4 * K * kTaps * kSumPitch;
+    return rows > sums ? rows : sums;
   }
 
   // even copy: words (4i, 4i + 1), (4i + 2, 4i + 3); odd copy: (4i + 1, 4i + 2), (4i + 3, 4i + 4)
@@ -217,48 +239,60 @@ struct Wgrad8 {
   }
 
   // Row j of dy and row r of x belong to kh = K - 1 - j + r: the two rows' columns j and j + 1 are added.
-  static __device__ __forceinline__ void write(Acc& acc, float* slice, int c, int C, int K) {
+  //
+  // The sums go through shared memory (`buf`, the place of x and dy between two images or pieces: [K][kTaps][kSumPitch]),
+  // so that the slice is written 32 channels at a time and the accumulators keep the layout of the products: written
+  // from there, 4 channels at a time, they take 60 registers more than there are at K > 23.  A lane's four channels are
+  // turned by t, which spreads a warp's stores over all banks.
+  // `again`: add to what this thread has written there before.  No other thread writes to these places and a thread's
+  // operations on one place keep their order, so the sums are the same bits on every run.
+  static __device__ __forceinline__ void write(Acc& acc, float* buf, float* slice, int c0, int C, int K, bool again) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    if (c >= C) return;
-    auto put = [&](int kh, int kw, float v0, float v1, float v2, float v3) {
-      if (kh >= 0 && kh < K && kw < K)
-        *reinterpret_cast<float4*>(slice + (static_cast<long long>(kh) * K + kw) * C + c) = make_float4(v0, v1, v2, v3);
+    float* const mine = buf + (threadIdx.x >> 5) * 4;
+    auto put = [&](int j, int kw, int ch, float v) {
+      if (j < K) mine[((K - 1 - j) * kTaps + kw) * kSumPitch + ((ch + t) & 3)] = v;
     };
-    if constexpr (PACK) {
-      float lo[4], hi[4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
 #pragma unroll
       for (int ch = 0; ch < 4; ++ch) {
-        float(&d)[4] = acc[ch][0][0][0];
-        lo[ch] = d[0] + d[3];
-        hi[ch] = d[1] + __shfl_down_sync(0xffffffffu, d[2], 1);  // column 2t + 2; past the last one kh < 0
-      }
-      put(K - 1 - 2 * t, g, lo[0], lo[1], lo[2], lo[3]);
-      put(K - 2 - 2 * t, g, hi[0], hi[1], hi[2], hi[3]);
-    } else {
+        if constexpr (PACK) {
+          float(&d)[4] = acc[ch][0][0][0];
+          put(2 * t, g, ch, d[0] + d[3]);
+          put(2 * t + 1, g, ch, d[1] + __shfl_down_sync(0xffffffffu, d[2], 1));  // column 2t + 2; past the last one j >= K
+        } else {
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            float lo[4], hi[4];
-#pragma unroll
-            for (int ch = 0; ch < 4; ++ch) {
-              lo[ch] = acc[ch][0][m][n][half * 2];
-              hi[ch] = acc[ch][0][m][n][half * 2 + 1];
+            for (int half = 0; half < 2; ++half) {
+              float lo = acc[ch][0][m][n][half * 2], hi = acc[ch][0][m][n][half * 2 + 1];
               if constexpr (ROWS == 2) {
-                lo[ch] += acc[ch][1][m][n][half * 2 + 1];
+                lo += acc[ch][1][m][n][half * 2 + 1];
                 // column 2t + 2 of row 1: the next lane's first, or the next tile's
-                const float mine = acc[ch][1][m][n][half * 2];
+                const float own = acc[ch][1][m][n][half * 2];
                 const float next = n + 1 < NT ? acc[ch][1][m][n + 1 < NT ? n + 1 : n][half * 2] : 0.0f;
-                const float from = __shfl_sync(0xffffffffu, t == 0 ? next : mine, (lane & ~3) | ((t + 1) & 3));
-                hi[ch] += from;
+                hi += __shfl_sync(0xffffffffu, t == 0 ? next : own, (lane & ~3) | ((t + 1) & 3));
               }
+              put(n * 8 + 2 * t, half * 8 + g, ch, lo);
+              put(n * 8 + 2 * t + 1, half * 8 + g, ch, hi);
             }
-            const int j = n * 8 + 2 * t, kw = m * 16 + half * 8 + g;
-            put(K - 1 - j, kw, lo[0], lo[1], lo[2], lo[3]);
-            put(K - 2 - j, kw, hi[0], hi[1], hi[2], hi[3]);
-          }
+        }
+      }
+      __syncthreads();
+      const int quad = threadIdx.x & 7, c = c0 + quad * 4;
+      for (int at = threadIdx.x >> 3; at < K * kTaps; at += kWgThreads / 8) {
+        const int kh = at / kTaps, kw = m * kTaps + at % kTaps, turn = (K - 1 - kh) >> 1;
+        float4 v = *reinterpret_cast<const float4*>(buf + at * kSumPitch + quad * 4);
+        if (turn & 1) v = make_float4(v.y, v.z, v.w, v.x);
+        if (turn & 2) v = make_float4(v.z, v.w, v.x, v.y);
+        if (kw >= K || c >= C) continue;
+        float* const to = slice + (static_cast<long long>(kh) * K + kw) * C + c;
+        if (again)
+          asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+        else
+          *reinterpret_cast<float4*>(to) = v;
+      }
+      if (m + 1 < MT) __syncthreads();
     }
   }
 };
@@ -329,22 +363,24 @@ __global__ void __launch_bounds__(kWgThreads, kWgCtas<MT, PACK>) wgrad8_kernel(c
   };
 
   typename S::Acc acc;
-#pragma unroll
-  for (int ch = 0; ch < 4; ++ch)
-#pragma unroll
-    for (int r = 0; r < S::kAcc; ++r)
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[ch][r][m][n][i] = 0.0f;
+  S::clear(acc);
+  int added = 0;         // steps in the accumulators
+  bool written = false;  // whether the slice holds sums of steps before them
 
   const int u1 = min(p.units, static_cast<int>(blockIdx.y + 1) * p.per_chunk);
   int u = blockIdx.y * p.per_chunk;
-  while (u < u1) {  // one image's part of the range at a time
+  while (true) {  // one image's part of the range at a time, in even pieces where it is longer than a chain
     const int b = u / p.unit_rows;
-    const int s0 = u - b * p.unit_rows, steps = min(p.unit_rows - s0, u1 - u);
+    const int s0 = u - b * p.unit_rows, rest = min(p.unit_rows - s0, u1 - u), pieces = (rest + S::kMost - 1) / S::kMost;
+    const int steps = rest > S::kMost ? (rest + pieces - 1) / pieces : rest;
+    if (rest <= 0 || added + steps > S::kMost) {
+      const long long slice = static_cast<long long>(blockIdx.z) * p.chunks + blockIdx.y;
+      S::write(acc, reinterpret_cast<float*>(smem), part + slice * p.K * p.K * p.C, c0, p.C, p.K, written);
+      if (rest <= 0) break;
+      S::clear(acc);
+      added = 0;
+      written = true;
+    }
     const int top = s0 * kStep + pad - (p.K - 1);  // first row of dy that the first row of x meets
     // of x and dy, this thread's next to fetch; of the exponent bytes, its next to load
     int row = s0 * kStep + x_row, drow = top + used + d_row;
@@ -420,10 +456,9 @@ __global__ void __launch_bounds__(kWgThreads, kWgCtas<MT, PACK>) wgrad8_kernel(c
       first -= first >= ring ? ring : 0;
       __syncthreads();
     }
+    added += steps;
     u += steps;
   }
-  const long long slice = static_cast<long long>(blockIdx.z) * p.chunks + blockIdx.y;
-  S::write(acc, part + slice * p.K * p.K * p.C, c0 + (tid >> 5) * 4, p.C, p.K);
 }
 
 // dw[i] = the slices' values added up (n2 pairs).  Row y of a block takes every ROWS-th slice in order, and the rows
@@ -464,12 +499,12 @@ __global__ void __launch_bounds__(kReduceThreads) wgrad8_reduce_kernel(const flo
 // The kernel for K and a tile of columns, its rows a step and its shared memory.
 struct Wgrad8Kernel {
   const void* fn;
-  int step, sets, ctas, smem;  // rows and sets a step; CTAs an SM, by registers
+  int step, most, ctas, smem;  // rows a step; steps of a chain; CTAs an SM, by registers
 };
 template <int MT, int NT, int ROWS, bool PACK, int TW, int SETS>
 static Wgrad8Kernel wgrad8_kernel_of(int K) {
   using S = Wgrad8<MT, NT, ROWS, PACK, TW, SETS>;
-  return {reinterpret_cast<const void*>(&wgrad8_kernel<MT, NT, ROWS, PACK, TW, SETS>), S::kStep, SETS, kWgCtas<MT, PACK>,
+  return {reinterpret_cast<const void*>(&wgrad8_kernel<MT, NT, ROWS, PACK, TW, SETS>), S::kStep, S::kMost, kWgCtas<MT, PACK>,
           S::smem(K)};
 }
 static int wgrad8_room(const Wgrad8Kernel& k) { return 228 * 1024 / (k.smem + 1024); }  // CTAs an SM, by shared memory
@@ -497,6 +532,9 @@ static Wgrad8Kernel wgrad8_kernel_for(int K, int tw) {
   }
 }
 
+static long long min_ll(long long a, long long b) { return a < b ? a : b; }
+static long long max_ll(long long a, long long b) { return a > b ? a : b; }
+
 static int wgrad8_plan(int64_t B, int64_t H, int64_t W, int64_t C, int K, Wgrad8Params* p) {
   if (K < 1 || K > 31 || (K % 2) == 0 || B < 0 || H < 1 || W < 1 || C < 8 || (C % 8) != 0) return DWB_ERR_BAD_SHAPE;
   if (B > (1 << 30) || H > (1 << 24) || W > (1 << 21) || C > (1 << 20) || B * H > (1LL << 30)) return DWB_ERR_BAD_SHAPE;
@@ -511,24 +549,35 @@ static int wgrad8_plan(int64_t B, int64_t H, int64_t W, int64_t C, int K, Wgrad8
   const Wgrad8Kernel k = wgrad8_kernel_for(K, p->tw);
   p->unit_rows = (p->H + k.step - 1) / k.step;
   p->units = p->B * p->unit_rows;
-  // As many ranges as CTAs run at once (a range more on some SMs would double the time), and none whose chains get too
-  // long.  However short: the rows of dy that a range brings in before its first product cost less than idle SMs
-  // (14x14x512 k27, B = 2: 28.8 us with ranges of 26 rows, 16.2 with 8, 14.7 with 4).
+  // As many ranges as CTAs run at once (a range more on some SMs would double the time).  However short: the rows of dy
+  // that a range brings in before its first product cost less than idle SMs (14x14x512 k27, B = 2: 28.8 us with ranges
+  // of 26 rows, 16.2 with 8, 14.7 with 4).  More turns of shorter ranges only where one leaves too many SMs idle (10
+  // tiles of 32 channels on 148 SMs are 14 ranges, but 100 are one): the turns' time is their steps and, for each, a
+  // start of about (K - 1) / 3 rows, and another turn has to save a part in 32 of it, since it has slices of its own.
   const long long base = (C + kWgChannels - 1) / kWgChannels * p->col_tiles;
   const int room = wgrad8_room(k);
   const long long at_once = static_cast<long long>(room < k.ctas ? room : k.ctas) * kSmCount;
-  const long long ranges = at_once / base > 1 ? at_once / base : 1;
-  long long per = (p->units + ranges - 1) / ranges;
-  const long long most = kChain / (p->tw / 16 * k.sets);
-  per = per < 1 ? 1 : per > most ? most : per;
-  p->per_chunk = static_cast<int>(per);
+  // so many steps at most to a range that its slice is added to kFlushes times, as long as a grid takes the ranges
+  const long long longest = max_ll(static_cast<long long>(k.most) * kFlushes, (p->units + 65534LL) / 65535);
+  long long best = 0;
+  p->per_chunk = 1;
+  for (int turns = 1; turns <= kTurns; ++turns) {
+    const long long ranges = max_ll(turns * at_once / base, 1);
+    const long long per = max_ll(min_ll((p->units + ranges - 1) / ranges, longest), 1), chunks = (p->units + per - 1) / per;
+    const long long time = (base * chunks + at_once - 1) / at_once * (3LL * k.step * per + K - 1);
+    if (turns == 1 || time < best - best / 32) {
+      best = time;
+      p->per_chunk = static_cast<int>(per);
+    }
+  }
   p->chunks = (p->units + p->per_chunk - 1) / p->per_chunk;
   if (p->chunks < 1) p->chunks = 1;
-  if (p->chunks > 65535 || p->col_tiles > 65535) return DWB_ERR_BAD_SHAPE;
   return DWB_OK;
 }
 
-// The partial sums: one [K][K][C] slice for every range of rows and tile of columns.
+// The partial sums: one [K][K][C] slice for every range of rows and tile of columns.  base * chunks CTAs write one 32
+// channels of it each, at most kTurns turns of the CTAs that run at once or one for every tile of columns and channels;
+// beyond that only 1 in every kFlushes * kMost steps, 0.5% of the codes and dy that they read at most.
 static int64_t wgrad8_workspace(const Wgrad8Params& p) {
   return static_cast<int64_t>(p.chunks) * p.col_tiles * p.K * p.K * p.C * static_cast<int64_t>(sizeof(float));
 }

@@ -108,3 +108,51 @@ def test_parameter_gradients_that_are_infinite(eng):
     db = eng.norm_ops.group_norm_act_backward(dy, x, mean, rstd, 2, None, torch.zeros(16, device="cuda"), "none")[2]
     assert db[4] == math.inf and db[5] == math.inf and torch.isnan(db[6])
     assert (db[[0, 1, 2, 3, *range(7, 16)]] == 360).all()
+
+
+# ---- weight gradient: ranges of many steps ------------------------------------------------------------
+
+def wgrad_chunks(B, H, W, C, K):
+    """Ranges that the steps of a tile of columns are split into: each has a slice of the workspace."""
+    import ctypes
+
+    from depthwise_conv_b200 import _lib
+    n = ctypes.c_int64(0)
+    _lib.call("dwb_conv2d_nhwc_bwd_weight_act8_workspace", B, H, W, C, K, ctypes.byref(n))
+    return n.value // (K * K * C * 4) // -(-W // 64)
+
+
+def check_wgrad(eng, B, H, W, C, K, seed):
+    """Bound: 128 products of 16 terms in a chain, each truncated at 2^-23 of the sum of the magnitudes at most, are
+    2^-16 of it; as much again for the terms' alignment within a product and the additions of chains and slices."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(B, H, W, C, device="cuda", generator=g) * (0.5 + torch.rand(C, device="cuda", generator=g))
+    codes, scales = eng.act8_encode((x + 0.5).half().permute(0, 3, 1, 2))
+    dy = (0.3 * torch.randn(B, H, W, C, device="cuda", generator=g) + 0.05).half().permute(0, 3, 1, 2)
+    dw = eng.act8_ops.conv2d_nhwc_backward_weight_act8(codes, scales, dy, K)
+    again = eng.act8_ops.conv2d_nhwc_backward_weight_act8(codes, scales, dy, K)
+    assert torch.equal(dw, again)
+    ref, size = R.dw_weight_grad(R.act8_decode(codes, scales), dy, K)
+    assert ((dw.double() - ref).abs() <= 2.0**-15 * size).all(), ((dw.double() - ref).abs() / size).max()
+    assert (dw.double() - ref).norm() <= 1e-5 * ref.norm()  # the bar of the 16-bit weight gradient
+    return (dw.double() - ref).norm() / ref.norm()
+
+
+# a width for each tile (16, 32, 48, 64 columns, two tiles), heights that end inside a step of 2 and 4 rows
+@pytest.mark.parametrize("W,H", [(13, 41), (16, 42), (30, 43), (45, 39), (61, 41), (75, 38)])
+@pytest.mark.parametrize("K", [1, 3, 5, 7, 9, 11, 13, 15, 17, 23, 25, 31])
+def test_weight_gradient_of_one_long_range(eng, K, W, H):
+    """So many channels that a CTA takes the images from the first row to the last: the ring of dy's rows goes round, x
+    changes between its two buffers, images follow each other, and a chain ends in the middle of an image."""
+    B, ctas = 3, 3 if K <= 7 else 2 if K <= 15 else 1
+    C = 32 * 148 * ctas
+    assert wgrad_chunks(B, H, W, C, K) <= 2
+    check_wgrad(eng, B, H, W, C, K, 100 * K + W)
+
+
+@pytest.mark.parametrize("B,H,W,C,K", [(2, 200, 64, 4736, 31), (40, 3, 15, 4736, 27), (1, 300, 33, 4736, 19), (64, 14, 14, 512, 27),
+                                       (70, 7, 7, 9464, 13), (9, 56, 56, 2056, 7), (2, 180, 20, 9472, 9), (17, 1, 64, 14208, 5)])
+def test_weight_gradient_of_long_ranges(eng, B, H, W, C, K):
+    """Tall images, many small ones and a ragged last block of channels, each range several chains or images long."""
+    assert wgrad_chunks(B, H, W, C, K) * 3 <= B * -(-H // 4)
+    check_wgrad(eng, B, H, W, C, K, B + H)

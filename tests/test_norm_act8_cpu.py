@@ -212,3 +212,27 @@ def test_trainable_block_on_cpu_fails_loudly():
     for checkpoint8 in (False, True):
         with pytest.raises(RuntimeError, match="CUDA"):
             TrainableDWBlock(64, 5, 8, checkpoint8=checkpoint8)(x)
+
+
+def _wgrad_workspace(L, *shape):
+    n = ctypes.c_int64(-1)
+    assert L.load().dwb_conv2d_nhwc_bwd_weight_act8_workspace(*shape, ctypes.byref(n)) == L.OK, shape
+    return n.value
+
+
+@pytest.mark.parametrize("H,W,C", [(56, 56, 1024), (56, 56, 128), (32, 32, 768), (14, 14, 512), (7, 7, 1024), (224, 224, 128)])
+def test_weight_gradient_workspace_does_not_grow_with_the_batch(L, H, W, C):
+    """At most 12 turns of the CTAs that run at once (148 SMs, 3 CTAs each at K <= 7, 2 at K <= 15), each with 32
+    channels of K * K sums, and beyond that a slice for every 256 chains of 128 products of 16 columns: 123 KB at most
+    for 16.8 M values, 0.75% of a byte for each (2.3 times that at 7 columns of a tile of 16)."""
+    for K in (3, 7, 9, 13, 15, 21, 27, 31):
+        turns = 12 * 148 * (3 if K <= 7 else 2 if K <= 15 else 1) * 32 * K * K * 4
+        for B in (64, 1024, 4096):
+            assert _wgrad_workspace(L, B, H, W, C, K) <= turns + 0.02 * B * H * W * C
+    assert _wgrad_workspace(L, 64, 56, 56, 1024, 31) <= 40e6
+
+
+def test_weight_gradient_takes_long_batches(L):
+    """As many images as the tensors may have: their number limits neither the ranges nor the workspace."""
+    for B, H, W, C, K in [(1 << 20, 512, 64, 8, 31), (1 << 30, 1, 16, 8, 3), (1 << 18, 56, 56, 128, 31), (1, 1 << 24, 64, 8, 17)]:
+        assert 0 < _wgrad_workspace(L, B, H, W, C, K) <= 0.01 * B * H * W * C + 12 * 148 * 3 * 32 * K * K * 4
