@@ -20,11 +20,12 @@ Torch ops:
 
 * ``depthwise::act8_encode(Tensor input) -> (Tensor codes, Tensor scales)``
 * ``depthwise::act8_decode(Tensor codes, Tensor scales, ScalarType dtype) -> Tensor``
-* ``depthwise::conv2d_nhwc_act8(Tensor input, Tensor weight, Tensor? bias=None)
-  -> (Tensor output, Tensor codes, Tensor scales)``: ``depthwise::conv2d_nhwc``
-  whose backward pass takes the weight gradient from the checkpoint, so that the
-  graph does not keep the input.  The input gradient does not read the input and
-  is the same as the other op's.
+* ``depthwise::conv2d_nhwc_act8(Tensor input, Tensor weight, Tensor? bias=None,
+  bool checkpoint=True) -> (Tensor output, Tensor codes, Tensor scales)``:
+  ``depthwise::conv2d_nhwc`` whose backward pass takes the weight gradient from the
+  checkpoint, so that the graph does not keep the input.  The input gradient does not
+  read the input and is the same as the other op's.  Without a checkpoint codes and
+  scales are empty and there is no weight gradient.
 """
 from __future__ import annotations
 
@@ -105,15 +106,28 @@ def empty_checkpoint(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return torch.empty_like(x, dtype=torch.int8), x.new_empty((B, H, W, -(-C // BLOCK)), dtype=torch.uint8)
 
 
+def no_checkpoint(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The empty codes and scales of an op that was not asked for a checkpoint."""
+    return x.new_empty((0,), dtype=torch.int8), x.new_empty((0,), dtype=torch.uint8)
+
+
+def will_differentiate(*tensors) -> bool:
+    """Whether the graph will hold a call with these inputs (some of them None)."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def conv2d_nhwc_act8(x: torch.Tensor, w: torch.Tensor, bias=None) -> torch.Tensor:
-    """y = conv(x, w) (+ bias), differentiable; keeps the 8-bit checkpoint of x for the weight gradient."""
-    return torch.ops.depthwise.conv2d_nhwc_act8(x, w, bias)[0]
+    """y = conv(x, w) (+ bias), differentiable; keeps the 8-bit checkpoint of x for the weight gradient.
+
+    Where no weight gradient will be taken (grad mode off, a weight that requires none) no checkpoint is made."""
+    return torch.ops.depthwise.conv2d_nhwc_act8(x, w, bias, will_differentiate(w))[0]
 
 
 torch.library.define("depthwise::act8_encode", "(Tensor input) -> (Tensor codes, Tensor scales)")
 torch.library.define("depthwise::act8_decode", "(Tensor codes, Tensor scales, ScalarType dtype) -> Tensor")
 torch.library.define("depthwise::conv2d_nhwc_act8",
-                     "(Tensor input, Tensor weight, Tensor? bias=None) -> (Tensor output, Tensor codes, Tensor scales)")
+                     "(Tensor input, Tensor weight, Tensor? bias=None, bool checkpoint=True) -> "
+                     "(Tensor output, Tensor codes, Tensor scales)")
 
 
 @torch.library.impl("depthwise::act8_encode", "default")
@@ -137,34 +151,36 @@ def _act8_decode_fake(codes, scales, dtype):
 
 
 @torch.library.impl("depthwise::conv2d_nhwc_act8", "default")
-def _conv2d_nhwc_act8_impl(input, weight, bias=None):
+def _conv2d_nhwc_act8_impl(input, weight, bias=None, checkpoint=True):
     y = dw_ops.conv2d_nhwc_fused(input, weight, bias=bias)
-    return y, *act8_encode(input)
+    return y, *(act8_encode(input) if checkpoint else no_checkpoint(input))
 
 
 @torch.library.register_fake("depthwise::conv2d_nhwc_act8")
-def _conv2d_nhwc_act8_fake(input, weight, bias=None):
-    return torch.empty_like(input), *empty_checkpoint(input)
+def _conv2d_nhwc_act8_fake(input, weight, bias=None, checkpoint=True):
+    return torch.empty_like(input), *(empty_checkpoint(input) if checkpoint else no_checkpoint(input))
 
 
 def _conv2d_nhwc_act8_setup(ctx, inputs, output):
-    _, w, bias = inputs
+    _, w, bias, checkpoint = inputs
     _, codes, scales = output
     ctx.save_for_backward(w, codes, scales)
-    ctx.has_bias = bias is not None
+    ctx.has_bias, ctx.checkpoint = bias is not None, checkpoint
     ctx.mark_non_differentiable(codes, scales)
     ctx.set_materialize_grads(False)
 
 
 def _conv2d_nhwc_act8_backward(ctx, grad, _codes, _scales):
     if grad is None:
-        return None, None, None
+        return None, None, None, None
     w, codes, scales = ctx.saved_tensors
+    if ctx.needs_input_grad[1] and not ctx.checkpoint:
+        raise RuntimeError("conv2d_nhwc_act8: the weight gradient needs a checkpoint of the input (checkpoint=True)")
     g = incoming(grad)
     dx = dw_ops.conv2d_nhwc_backward_input(g, w) if ctx.needs_input_grad[0] else None
     dw = conv2d_nhwc_backward_weight_act8(codes, scales, g, w.shape[0]).to(w.dtype) if ctx.needs_input_grad[1] else None
     db = g.float().sum(dim=(0, 2, 3)).to(g.dtype).detach() if ctx.has_bias and ctx.needs_input_grad[2] else None
-    return first_order("conv2d_nhwc_act8", dx, dw, db)
+    return *first_order("conv2d_nhwc_act8", dx, dw, db), None
 
 
 torch.library.register_autograd("depthwise::conv2d_nhwc_act8", _conv2d_nhwc_act8_backward,

@@ -26,7 +26,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .act8_ops import after_launch, bind, empty_checkpoint, first_order, incoming
+from .act8_ops import after_launch, bind, empty_checkpoint, first_order, incoming, no_checkpoint, will_differentiate
 
 ACT_CODES = _lib.NORM_ACT_CODES
 
@@ -62,9 +62,11 @@ def group_norm_act_backward(dy: torch.Tensor, saved, mean: torch.Tensor, rstd: t
 
 def group_norm_act(x: torch.Tensor, num_groups: int, weight=None, bias=None, eps: float = 1e-5, act: int | str = 0,
                    checkpoint: bool = False) -> torch.Tensor:
-    """act(group_norm(x)), differentiable; ``checkpoint``: keep the input for the backward pass in 8 bits."""
+    """act(group_norm(x)), differentiable; ``checkpoint``: keep the input for the backward pass in 8 bits.
+
+    Where there will be no backward pass no checkpoint is made; the result is the same bits."""
     return torch.ops.depthwise.group_norm_act(x, int(num_groups), weight, bias, float(eps), _act_code(act),
-                                              bool(checkpoint))[0]
+                                              bool(checkpoint) and will_differentiate(x, weight, bias))[0]
 
 
 torch.library.define(
@@ -74,20 +76,16 @@ torch.library.define(
 )
 
 
-def _no_checkpoint(x):
-    return x.new_empty((0,), dtype=torch.int8), x.new_empty((0,), dtype=torch.uint8)
-
-
 @torch.library.impl("depthwise::group_norm_act", "default")
 def _group_norm_act_impl(input, num_groups, weight, bias, eps, act, checkpoint):
     out = group_norm_act_forward(input, num_groups, weight, bias, eps, act, checkpoint)
-    return out if checkpoint else (*out, *_no_checkpoint(input))
+    return out if checkpoint else (*out, *no_checkpoint(input))
 
 
 @torch.library.register_fake("depthwise::group_norm_act")
 def _group_norm_act_fake(input, num_groups, weight, bias, eps, act, checkpoint):
     mean = input.new_empty((input.shape[0], num_groups), dtype=torch.float32)
-    kept = empty_checkpoint(input) if checkpoint else _no_checkpoint(input)
+    kept = empty_checkpoint(input) if checkpoint else no_checkpoint(input)
     return torch.empty_like(input), mean, torch.empty_like(mean), *kept
 
 

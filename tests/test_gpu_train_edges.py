@@ -156,3 +156,38 @@ def test_weight_gradient_of_long_ranges(eng, B, H, W, C, K):
     """Tall images, many small ones and a ragged last block of channels, each range several chains or images long."""
     assert wgrad_chunks(B, H, W, C, K) * 3 <= B * -(-H // 4)
     check_wgrad(eng, B, H, W, C, K, B + H)
+
+
+# ---- no checkpoint where nothing reads it ------------------------------------------------------------
+
+def test_evaluation_makes_no_checkpoint(eng):
+    """A checkpointed block under no_grad: the same bits, and no more memory than the one without checkpoints."""
+    from depthwise_conv_b200.convmixer import TrainableDWBlock
+    torch.manual_seed(7)
+    block = TrainableDWBlock(256, 7, 32, "gelu", checkpoint8=True).cuda()
+    x = torch.randn(8, 32, 32, 256, device="cuda").half().permute(0, 3, 1, 2)
+    want = block(x).detach()
+    peak = []
+    for block.checkpoint8 in (False, True):
+        with torch.no_grad():
+            block(x)
+            torch.cuda.synchronize()
+            torch.cuda.reset_peak_memory_stats()
+            before = torch.cuda.memory_allocated()
+            y = block(x)
+            peak.append(torch.cuda.max_memory_allocated() - before)
+            assert torch.equal(y, want)
+            del y
+    assert peak[0] == peak[1]
+
+
+def test_a_frozen_weight_keeps_no_checkpoint(eng):
+    x = torch.randn(4, 28, 28, 128, device="cuda").half().permute(0, 3, 1, 2).requires_grad_()
+    w = (torch.randn(9, 9, 128, device="cuda") / 9).half()
+    dy = torch.randn(4, 28, 28, 128, device="cuda").half().permute(0, 3, 1, 2)
+    dx, = torch.autograd.grad(eng.conv2d_nhwc_act8(x, w.clone().requires_grad_()), x, dy)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    y = eng.conv2d_nhwc_act8(x, w)
+    assert torch.cuda.memory_allocated() - before <= 2 * y.numel() + 4096
+    assert torch.equal(torch.autograd.grad(y, x, dy)[0], dx)

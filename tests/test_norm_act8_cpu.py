@@ -236,3 +236,68 @@ def test_weight_gradient_takes_long_batches(L):
     """As many images as the tensors may have: their number limits neither the ranges nor the workspace."""
     for B, H, W, C, K in [(1 << 20, 512, 64, 8, 31), (1 << 30, 1, 16, 8, 3), (1 << 18, 56, 56, 128, 31), (1, 1 << 24, 64, 8, 17)]:
         assert 0 < _wgrad_workspace(L, B, H, W, C, K) <= 0.01 * B * H * W * C + 12 * 148 * 3 * 32 * K * K * 4
+
+
+def test_no_checkpoint_where_no_gradient_is_taken(monkeypatch):
+    """The differentiable ops with the kernels' calls replaced: who asks for a checkpoint, and when."""
+    import depthwise_conv_b200 as d
+    made = []
+
+    def encode(x):
+        made.append("conv")
+        return d.act8_ops.empty_checkpoint(x)
+
+    def norm(x, num_groups, weight, bias, eps, act, checkpoint):
+        stats = torch.zeros(x.shape[0], num_groups)
+        out = (x.clone(memory_format=torch.preserve_format), stats, stats.clone())
+        if checkpoint:
+            made.append("norm")
+        return (*out, *d.act8_ops.empty_checkpoint(x)) if checkpoint else out
+
+    monkeypatch.setattr(d.act8_ops, "act8_encode", encode)
+    monkeypatch.setattr(d.norm_ops, "group_norm_act_forward", norm)
+    monkeypatch.setattr(d.dw_ops, "conv2d_nhwc_fused", lambda x, w, bias=None: x.clone(memory_format=torch.preserve_format))
+    monkeypatch.setattr(d.dw_ops, "conv2d_nhwc_backward_input", lambda g, w: 2 * g)
+    monkeypatch.setattr(d.act8_ops, "conv2d_nhwc_backward_weight_act8",
+                        lambda codes, scales, g, K: torch.ones(K, K, g.shape[1]))
+
+    def call(f, *args):
+        made.clear()
+        return f(*args)
+
+    x = torch.zeros(2, 64, 4, 4, dtype=torch.float16).contiguous(memory_format=torch.channels_last)
+    w, v = torch.zeros(3, 3, 64, dtype=torch.float16), torch.ones(64)
+    conv = lambda *a: call(d.conv2d_nhwc_act8, *a)  # noqa: E731
+    gn = lambda *a: call(lambda *b: d.group_norm_act(b[0], 8, b[1], b[2], checkpoint=True), *a)  # noqa: E731
+    grad = lambda t: t.clone(memory_format=torch.preserve_format).requires_grad_()  # noqa: E731
+    # nothing to differentiate: grad mode off, or no input that requires it
+    with torch.no_grad():
+        conv(grad(x), grad(w))
+        assert made == []
+        gn(grad(x), grad(v), grad(v))
+        assert made == []
+    with torch.inference_mode():
+        conv(x, w)
+        assert made == []
+    conv(x, w)
+    assert made == []
+    gn(x, v, v)
+    assert made == []
+    # a frozen weight: the input gradient alone, which reads no input
+    xg = grad(x)
+    conv(xg, w).backward(torch.ones_like(x))
+    assert made == [] and (xg.grad == 2).all()
+    # a weight gradient
+    wg = grad(w)
+    conv(x, wg).backward(torch.ones_like(x))
+    assert made == ["conv"] and (wg.grad == 1).all()
+    # every gradient of the norm reads its input
+    for args in ((grad(x), v, v), (x, grad(v), None), (x, None, grad(v))):
+        gn(*args)
+        assert made == ["norm"]
+    # the op itself does what its argument says
+    assert torch.ops.depthwise.conv2d_nhwc_act8(x, w)[1].shape == x.shape
+    y, codes, scales = torch.ops.depthwise.conv2d_nhwc_act8(x, grad(w), None, False)
+    assert codes.numel() == scales.numel() == 0
+    with pytest.raises(RuntimeError, match="needs a checkpoint"):
+        y.backward(torch.ones_like(x))
