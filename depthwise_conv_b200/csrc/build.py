@@ -5,7 +5,8 @@ Compiles every ``*.cu`` in this directory with nvcc
 parallel, into ``depthwise_conv_b200/_build/``, then links the shared library
 into the package directory.  An object is rebuilt only when its source or a
 header that it includes is newer.  The library depends on the CUDA runtime only (no torch);
-the training ops' host side, ``_train_bind.so``, is a Python module over PyTorch and it.
+the training ops' host side, ``_train_bind.so``, is a Python module over PyTorch and it, and
+is left out where there is no PyTorch.
 
     python -m depthwise_conv_b200.csrc.build        # or: python build.py
     python -m depthwise_conv_b200.csrc.build --regcaps   # regenerate dw_regcaps.inc first
@@ -23,6 +24,8 @@ uses it.
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.metadata
+import importlib.util
 import os
 import re
 import shutil
@@ -36,6 +39,7 @@ BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libdwconv_b200.so")
 BIND_SRC = os.path.join(HERE, "bind", "train_bind.cpp")
 BIND = os.path.join(PKG, "_train_bind.so")
+BIND_VERSIONS = os.path.join(BUILD, "train_bind.versions")
 INCLUDE = os.path.join(ROOT, "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -107,9 +111,33 @@ def build(verbose: bool = False, jobs: int | None = None) -> str:
     return LIB
 
 
-def build_bind(verbose: bool = False) -> str:
-    """Compile the training ops' host side (a Python module over PyTorch and the library); returns its path."""
-    if os.path.exists(BIND) and os.path.getmtime(BIND) >= _inputs_mtime(BIND_SRC):
+def _bind_versions() -> str | None:
+    """What the compiled Python module is made for: this Python and this PyTorch; None without PyTorch."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return None
+    try:
+        version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:  # on the path, but not installed as a package
+        version = "unknown"
+    return f"{sys.version}\n{version}\n{spec.origin}\n"
+
+
+def build_bind(verbose: bool = False) -> str | None:
+    """Compile the training ops' host side (a Python module over PyTorch and the library); returns its path.
+
+    Without PyTorch there is nothing that could load it: it is left out, and the path is None.  It is rebuilt when
+    its sources, the Python or the PyTorch that it was made for change."""
+    versions = _bind_versions()
+    if versions is None:
+        if verbose:
+            print(f"PyTorch is not installed: {os.path.basename(BIND)} is not built")
+        return None
+    made_for = ""
+    if os.path.exists(BIND_VERSIONS):
+        with open(BIND_VERSIONS) as f:
+            made_for = f.read()
+    if os.path.exists(BIND) and os.path.getmtime(BIND) >= _inputs_mtime(BIND_SRC) and made_for == versions:
         return BIND
     import sysconfig
 
@@ -124,6 +152,9 @@ def build_bind(verbose: bool = False) -> str:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+    os.makedirs(BUILD, exist_ok=True)
+    with open(BIND_VERSIONS, "w") as f:
+        f.write(versions)
     if verbose:
         print(f"built {BIND}")
     return BIND

@@ -3,6 +3,8 @@ PyTorch, the entry points' refusals, the fake impls, and workspace sizes."""
 from __future__ import annotations
 
 import ctypes
+import importlib.metadata
+import importlib.util
 
 import pytest
 import torch
@@ -301,3 +303,46 @@ def test_no_checkpoint_where_no_gradient_is_taken(monkeypatch):
     assert codes.numel() == scales.numel() == 0
     with pytest.raises(RuntimeError, match="needs a checkpoint"):
         y.backward(torch.ones_like(x))
+
+
+@pytest.fixture
+def bind_build(monkeypatch, tmp_path):
+    """csrc/build.py with the Python module's files in tmp_path and a compiler that only notes its calls."""
+    from depthwise_conv_b200.csrc import build as b
+    calls = []
+
+    class Done:
+        returncode, stdout, stderr = 0, "", ""
+
+    def run(cmd, **_):
+        calls.append(cmd)
+        (tmp_path / "bind.so").write_text("")
+        return Done
+
+    monkeypatch.setattr(b, "BIND", str(tmp_path / "bind.so"))
+    monkeypatch.setattr(b, "BUILD", str(tmp_path / "objects"))
+    monkeypatch.setattr(b, "BIND_VERSIONS", str(tmp_path / "objects" / "versions"), raising=False)
+    monkeypatch.setattr(b.subprocess, "run", run)
+    return b, calls
+
+
+def test_build_without_pytorch(bind_build, monkeypatch):
+    """The library is built without PyTorch; its Python module is left out then."""
+    import sys
+    b, calls = bind_build
+    monkeypatch.setitem(sys.modules, "torch", None)  # `import torch` raises
+    real = importlib.util.find_spec
+    monkeypatch.setattr(importlib.util, "find_spec", lambda name, *a: None if name == "torch" else real(name, *a))
+    assert b.build_bind() is None and calls == []
+
+
+def test_the_python_module_is_rebuilt_for_another_pytorch(bind_build, monkeypatch):
+    b, calls = bind_build
+    assert b.build_bind() == b.BIND and len(calls) == 1
+    assert b.build_bind() == b.BIND and len(calls) == 1  # nothing has changed
+    real = importlib.metadata.version
+    monkeypatch.setattr(importlib.metadata, "version", lambda name: "0.0" if name == "torch" else real(name))
+    b.build_bind()
+    assert len(calls) == 2
+    b.build_bind()
+    assert len(calls) == 2
