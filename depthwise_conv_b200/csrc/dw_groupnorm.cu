@@ -72,11 +72,11 @@ static int gn_shape(int64_t B, int64_t H, int64_t W, int64_t C, int G, double ep
   if (param_dtype != dtype && param_dtype != DWB_F32) return DWB_ERR_BAD_ARG;
   if (act < DWB_ACT_NONE || act > DWB_ACT_SILU) return DWB_ERR_BAD_ARG;
   if (!(eps >= 0.0) || !(eps < 1e30)) return DWB_ERR_BAD_ARG;
-  // B: grid x; H * W: the row index; C: 32-bit channel arithmetic; groups of a call: grid y
+  // B * channels: grid x; H * W: the row index; C: 32-bit channel arithmetic
   if (B < 0 || B > (1 << 30) || H < 1 || W < 1 || H > (1 << 30) || W > (1 << 30) || C < 8 || C > 65536 || (C % 8) != 0)
     return DWB_ERR_BAD_SHAPE;
   if (H * W > 0x7fffffffLL) return DWB_ERR_BAD_SHAPE;
-  if (G < 1 || G > C || (C % G) != 0 || G > 65535) return DWB_ERR_BAD_SHAPE;
+  if (G < 1 || G > C || (C % G) != 0) return DWB_ERR_BAD_SHAPE;
   s->P = H * W;
   s->B = static_cast<int>(B);
   s->C = static_cast<int>(C);

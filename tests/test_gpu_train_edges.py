@@ -191,3 +191,21 @@ def test_a_frozen_weight_keeps_no_checkpoint(eng):
     y = eng.conv2d_nhwc_act8(x, w)
     assert torch.cuda.memory_allocated() - before <= 2 * y.numel() + 4096
     assert torch.equal(torch.autograd.grad(y, x, dy)[0], dx)
+
+
+@pytest.mark.parametrize("G", [65536, 32768, 1])
+@pytest.mark.parametrize("H", [3, 150])
+def test_the_most_channels(eng, G, H):
+    """65536 channels, a group for each of them, for two, and one for all."""
+    from test_gpu_norm_act8 import check_backward, check_forward
+    B, W, C = 2, 3, 65536
+    g = torch.Generator(device="cuda").manual_seed(H)
+    x, dy = (torch.randn(B, H, W, C, device="cuda", generator=g).half().permute(0, 3, 1, 2) for _ in range(2))
+    w, b = 1 + 0.3 * torch.randn(C, device="cuda", generator=g), 0.3 * torch.randn(C, device="cuda", generator=g)
+    out = eng.norm_ops.group_norm_act_forward(x, G, w, b, 1e-5, "silu", checkpoint=True)
+    check_forward(out, x, G, w, b, 1e-5, "silu")
+    assert all(torch.equal(p, q) for p, q in zip(out[3:], eng.act8_encode(x)))
+    mean, rstd = (t.float() for t in R.stats(x, G, 1e-5))
+    for saved, values in ((x, x), (out[3:], R.act8_decode(*out[3:]))):
+        got = eng.norm_ops.group_norm_act_backward(dy, saved, mean, rstd, G, w, b, "silu")
+        check_backward(got, dy, values, mean, rstd, G, w, b, "silu")

@@ -346,3 +346,10 @@ def test_the_python_module_is_rebuilt_for_another_pytorch(bind_build, monkeypatc
     assert len(calls) == 2
     b.build_bind()
     assert len(calls) == 2
+
+
+def test_group_norm_takes_a_group_for_each_of_65536_channels(L):
+    n = ctypes.c_int64(-1)
+    for backward in (0, 1):
+        assert L.load().dwb_group_norm_act_workspace(2, 3, 3, 65536, 65536, backward, ctypes.byref(n)) == L.OK
+    assert _fwd(L, C=65536, G=65536, x=None) == _bwd(L, C=65536, G=65536, dy=None) == L.ERR_NULL_POINTER
