@@ -209,3 +209,99 @@ def test_the_most_channels(eng, G, H):
     for saved, values in ((x, x), (out[3:], R.act8_decode(*out[3:]))):
         got = eng.norm_ops.group_norm_act_backward(dy, saved, mean, rstd, G, w, b, "silu")
         check_backward(got, dy, values, mean, rstd, G, w, b, "silu")
+
+
+# ---- group norm: plans that small tensors do not take ------------------------------------------------
+
+def norm_workspace(B, H, W, C, G, backward):
+    import ctypes
+
+    from depthwise_conv_b200 import _lib
+    n = ctypes.c_int64(0)
+    _lib.call("dwb_group_norm_act_workspace", B, H, W, C, G, backward, ctypes.byref(n))
+    return n.value
+
+
+def whole_norm(eng, B, H, W, C, G, act, dtype, seed):
+    """Forward with and without a checkpoint, the gradient from the input, from the checkpoint and into dy's buffer."""
+    import ctypes
+
+    from depthwise_conv_b200 import _lib
+    from test_gpu_norm_act8 import check_backward, check_forward
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = (torch.randn(B, H, W, C, device="cuda", generator=g) + 0.5 * torch.randn(C, device="cuda", generator=g))
+    x = x.to(dtype).permute(0, 3, 1, 2)
+    dy = (0.3 * torch.randn(B, H, W, C, device="cuda", generator=g)).to(dtype).permute(0, 3, 1, 2)
+    w, b = 1 + 0.3 * torch.randn(C, device="cuda", generator=g), 0.3 * torch.randn(C, device="cuda", generator=g)
+    n = eng.norm_ops
+    out = n.group_norm_act_forward(x, G, w, b, 1e-5, act, checkpoint=True)
+    check_forward(out, x, G, w, b, 1e-5, act)
+    assert all(torch.equal(p, q) for p, q in zip(out, n.group_norm_act_forward(x, G, w, b, 1e-5, act)))
+    assert all(torch.equal(p, q) for p, q in zip(out[3:], eng.act8_encode(x)))
+    codes, scales = out[3:]
+    mean, rstd = (t.float() for t in R.stats(x, G, 1e-5))
+    ws = torch.empty(max(16, norm_workspace(B, H, W, C, G, 1)), dtype=torch.uint8, device="cuda")
+    for saved, values in ((x, x), ((codes, scales), R.act8_decode(codes, scales))):
+        got = n.group_norm_act_backward(dy, saved, mean, rstd, G, w, b, act)
+        check_backward(got, dy, values, mean, rstd, G, w, b, act)
+        place = dy.clone(memory_format=torch.preserve_format)
+        source = (x.data_ptr(), None, None) if saved is x else (None, codes.data_ptr(), scales.data_ptr())
+        _lib.call("dwb_group_norm_act_nhwc_bwd", place.data_ptr(), *source, mean.data_ptr(), rstd.data_ptr(), w.data_ptr(),
+                  b.data_ptr(), place.data_ptr(), None, None, ws.data_ptr(), ws.numel(), B, H, W, C, G,
+                  {"none": 0, "relu": 1, "gelu": 2, "silu": 3}[act], 0 if dtype == torch.float16 else 1, 2,
+                  torch.cuda.current_stream().cuda_stream)
+        assert torch.equal(place, got[0])
+        del got, values
+    assert eng.device_error() == 0
+
+
+@pytest.mark.parametrize("Cg,act,dtype", [(24, "gelu", torch.float16), (12, "silu", torch.bfloat16), (3, "gelu", torch.bfloat16),
+                                          (876, "silu", torch.float16), (1752, "gelu", torch.float16)])
+def test_batches_in_several_groups_of_samples(eng, Cg, act, dtype):
+    """The two streaming passes over three groups of samples and more, the last one shorter: launches that do both
+    passes, one after another, and load before the launch before them has ended.
+
+    A group is 160 MB of what a pass reads: of 11 samples of 35 MB 4 + 4 + 3 forward, 2 x 5 + 1 in the gradient from the
+    input (twice the bytes), 3 x 3 + 2 from a checkpoint.  Groups of whole vectors, of half vectors, of 3 channels, of
+    more than a tile (an entry a channel) and of several tiles."""
+    B, H, W, C = 11, 100, 100, 1752
+    assert B * H * W * C * 2 > 2 * (160 << 20) and norm_workspace(B, H, W, C, C // Cg, 0) > 0  # streaming has a workspace
+    whole_norm(eng, B, H, W, C, C // Cg, act, dtype, Cg)
+
+
+@pytest.mark.parametrize("G", [128, 64, 512, 32])
+@pytest.mark.parametrize("B,H,W", [(37, 27, 29), (19, 41, 37), (10, 53, 61)])
+def test_many_units_in_small_ctas(eng, B, H, W, G):
+    """The forward kernel's CTAs of 128 threads, from 8 an SM on, in clusters of 2, 4 and 8 (with 512 groups of a
+    channel, whose entries take more of the shared memory, 4 and 8, and CTAs of 256 threads for the largest)."""
+    assert norm_workspace(B, H, W, 512, G, 0) == 0
+    whole_norm(eng, B, H, W, 512, G, "gelu" if G != 64 else "silu", torch.float16 if G != 32 else torch.bfloat16, B + G)
+
+
+@pytest.mark.parametrize("shape", [(1, 3, 3, 2048, 1), (1, 3, 3, 1024, 1), (2, 3, 3, 1024, 2), (1, 1, 17, 2048, 1), (1, 1, 1, 1024, 1)])
+def test_clusters_with_more_ctas_than_pixels_need(eng, shape):
+    """Nine pixels over four CTAs of three: the last has none, and no say in the moments."""
+    whole_norm(eng, *shape, "gelu", torch.float16, shape[2])
+
+
+@pytest.mark.parametrize("act", ["none", "gelu", "silu", "relu"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("H,C,G", [(6, 64, 4), (6, 24, 8), (30000, 64, 2), (30000, 24, 1)])
+def test_a_bad_value_takes_its_whole_group(eng, act, bad, H, C, G):
+    """A NaN or an infinity in x makes all of its group's outputs NaN, for every activation, and no other group's;
+    the gradient of its sample's group too, and the parameters' gradients in its channels."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(2, H, 3, C, device="cuda", generator=g).bfloat16().permute(0, 3, 1, 2)
+    c = C // 2 + 1
+    x[1, c, H // 2, 1] = bad
+    lo, hi = c // (C // G) * (C // G), (c // (C // G) + 1) * (C // G)
+    n = eng.norm_ops
+    y, mean, rstd, codes, scales = n.group_norm_act_forward(x, G, act=act, checkpoint=True)
+    inside = torch.zeros(2, C, dtype=torch.bool, device="cuda")
+    inside[1, lo:hi] = True
+    assert torch.equal(torch.isnan(y).amax(dim=(2, 3)), inside) and torch.equal(torch.isnan(y).all(dim=3).all(dim=2), inside)
+    w = torch.ones(C, device="cuda")
+    dx, dw, _ = n.group_norm_act_backward(torch.ones_like(x), x, mean, rstd, G, w, None, act)
+    assert torch.equal(torch.isnan(dx).all(dim=3).all(dim=2), inside) and torch.equal(torch.isnan(dx).amax(dim=(2, 3)), inside)
+    assert torch.equal(torch.isnan(dw), inside[1])
+    assert (scales == 255).sum() == 1 and scales[1, H // 2, 1, c // 32] == 255
