@@ -39,9 +39,9 @@
 // however long the batch.
 //
 // Measured (both kernels; the framework's 16-bit weight gradient on the CUDA
-// cores in brackets): 16x32x32x768 k7 34.4 us (64.3), 16x32x32x1536 k9 81.5 (182),
-// 8x56x56x1024 k13 114 (310), 8x56x56x128 k31 42 (171), 2x14x14x512 k27 11.2,
-// 56x56x1024 k31 245 with 8 images, 1732 with 64 (285 and 1905 when a chain's end was
+// cores in brackets): 16x32x32x768 k7 34.4 us (64.3), 16x32x32x1536 k9 82.6 (182),
+// 8x56x56x1024 k13 112 (310), 8x56x56x128 k31 44 (171), 2x14x14x512 k27 12.1,
+// 56x56x1024 k31 242 with 8 images, 1701 with 64 (286 and 1908 when a chain's end was
 // a range's: 112 slices, 441 MB of workspace for the 64 images, where 9 are 35 MB).
 // What bounds it is the issue of the instructions around the products, most of
 // all the conversion and transposition of x and dy: at 16x32x32x768 k7 the
@@ -238,46 +238,78 @@ struct Wgrad8 {
     }
   }
 
-  // Row j of dy and row r of x belong to kh = K - 1 - j + r: the two rows' columns j and j + 1 are added.
-  //
-  // The sums go through shared memory (`buf`, the place of x and dy between two images or pieces: [K][kTaps][kSumPitch]),
-  // so that the slice is written 32 channels at a time and the accumulators keep the layout of the products: written
-  // from there, 4 channels at a time, they take 60 registers more than there are at K > 23.  A lane's four channels are
-  // turned by t, which spreads a warp's stores over all banks.
-  // `again`: add to what this thread has written there before.  No other thread writes to these places and a thread's
-  // operations on one place keep their order, so the sums are the same bits on every run.
-  static __device__ __forceinline__ void write(Acc& acc, float* buf, float* slice, int c0, int C, int K, bool again) {
+  // f(j, kw, v) with what this lane has of dw[K - 1 - j][m * kTaps + kw] in the warp's channel ch: row j of dy and row
+  // r of x belong to kh = K - 1 - j + r, so the two rows' columns j and j + 1 are added.
+  template <typename F>
+  static __device__ __forceinline__ void each_sum(Acc& acc, int m, int n, int half, int ch, F f) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    if constexpr (PACK) {
+      float(&d)[4] = acc[ch][0][0][0];
+      f(2 * t, g, d[0] + d[3]);
+      f(2 * t + 1, g, d[1] + __shfl_down_sync(0xffffffffu, d[2], 1));  // column 2t + 2; past the last one j >= K
+    } else {
+      float lo = acc[ch][0][m][n][half * 2], hi = acc[ch][0][m][n][half * 2 + 1];
+      if constexpr (ROWS == 2) {
+        lo += acc[ch][1][m][n][half * 2 + 1];
+        // column 2t + 2 of row 1: the next lane's first, or the next tile's
+        const float own = acc[ch][1][m][n][half * 2];
+        const float next = n + 1 < NT ? acc[ch][1][m][n + 1 < NT ? n + 1 : n][half * 2] : 0.0f;
+        hi += __shfl_sync(0xffffffffu, t == 0 ? next : own, (lane & ~3) | ((t + 1) & 3));
+      }
+      f(n * 8 + 2 * t, half * 8 + g, lo);
+      f(n * 8 + 2 * t + 1, half * 8 + g, hi);
+    }
+  }
+  static constexpr int kHalves = PACK ? 1 : 2;
+
+  // The slice of a range that is one chain, from the accumulators.  c: this warp's first channel.
+  static __device__ __forceinline__ void write(Acc& acc, float* slice, int c, int C, int K) {
+    if (c >= C) return;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int half = 0; half < kHalves; ++half) {
+          float lo[4], hi[4];
+          int j = 0, kw = 0;
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch)
+            each_sum(acc, m, n, half, ch, [&](int row, int tap, float v) {
+              if (row & 1) hi[ch] = v;
+              else lo[ch] = v;
+              j = row & ~1;
+              kw = m * kTaps + tap;
+            });
+          auto put = [&](int kh, const float(&v)[4]) {
+            if (kh >= 0 && kw < K)
+              *reinterpret_cast<float4*>(slice + (static_cast<long long>(kh) * K + kw) * C + c) = make_float4(v[0], v[1], v[2], v[3]);
+          };
+          put(K - 1 - j, lo);
+          put(K - 2 - j, hi);
+        }
+  }
+
+  // The same where a range has several chains: `again` adds to what this thread has put there before.  No other thread
+  // writes to these places and a thread's operations on one place keep their order, so the sums are the same bits on
+  // every run.  The sums go through shared memory (`buf`, the place of x and dy between two images or pieces of one:
+  // [K][kTaps][kSumPitch]), since this is inside the loop: written from the accumulators, 4 channels at a time, they
+  // would take 60 registers more than there are at K > 23.  A lane's four channels are turned by t, which spreads a
+  // warp's stores over all banks.
+  static __device__ __forceinline__ void add(Acc& acc, float* buf, float* slice, int c0, int C, int K, bool again) {
+    const int t = threadIdx.x & 3;
     float* const mine = buf + (threadIdx.x >> 5) * 4;
-    auto put = [&](int j, int kw, int ch, float v) {
-      if (j < K) mine[((K - 1 - j) * kTaps + kw) * kSumPitch + ((ch + t) & 3)] = v;
-    };
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
-      for (int ch = 0; ch < 4; ++ch) {
-        if constexpr (PACK) {
-          float(&d)[4] = acc[ch][0][0][0];
-          put(2 * t, g, ch, d[0] + d[3]);
-          put(2 * t + 1, g, ch, d[1] + __shfl_down_sync(0xffffffffu, d[2], 1));  // column 2t + 2; past the last one j >= K
-        } else {
+      for (int ch = 0; ch < 4; ++ch)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              float lo = acc[ch][0][m][n][half * 2], hi = acc[ch][0][m][n][half * 2 + 1];
-              if constexpr (ROWS == 2) {
-                lo += acc[ch][1][m][n][half * 2 + 1];
-                // column 2t + 2 of row 1: the next lane's first, or the next tile's
-                const float own = acc[ch][1][m][n][half * 2];
-                const float next = n + 1 < NT ? acc[ch][1][m][n + 1 < NT ? n + 1 : n][half * 2] : 0.0f;
-                hi += __shfl_sync(0xffffffffu, t == 0 ? next : own, (lane & ~3) | ((t + 1) & 3));
-              }
-              put(n * 8 + 2 * t, half * 8 + g, ch, lo);
-              put(n * 8 + 2 * t + 1, half * 8 + g, ch, hi);
-            }
-        }
-      }
+          for (int half = 0; half < kHalves; ++half)
+            each_sum(acc, m, n, half, ch, [&](int j, int kw, float v) {
+              if (j < K) mine[((K - 1 - j) * kTaps + kw) * kSumPitch + ((ch + t) & 3)] = v;
+            });
       __syncthreads();
       const int quad = threadIdx.x & 7, c = c0 + quad * 4;
       for (int at = threadIdx.x >> 3; at < K * kTaps; at += kWgThreads / 8) {
@@ -300,7 +332,10 @@ struct Wgrad8 {
 template <int MT, bool PACK>
 constexpr int kWgCtas = PACK ? 3 : MT == 1 ? 2 : 1;
 
-template <int MT, int NT, int ROWS, bool PACK, int TW, int SETS>
+// LONG: ranges of several chains.  A kernel of its own, because what it needs for them costs small calls time (2x2x16 k9,
+// B = 8: 5.3 us, 6.0 with it; 1x64x16 k29, B = 7: 10.4 and 12.4); large ones it serves better than ranges that end where
+// a chain does (28x28x256 k29, B = 64: 158 us with those, 124 so).
+template <int MT, int NT, int ROWS, bool PACK, int TW, int SETS, bool LONG>
 __global__ void __launch_bounds__(kWgThreads, kWgCtas<MT, PACK>) wgrad8_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                             const __half* __restrict__ dy, float* __restrict__ part,
                                                             const Wgrad8Params p) {
@@ -366,20 +401,29 @@ __global__ void __launch_bounds__(kWgThreads, kWgCtas<MT, PACK>) wgrad8_kernel(c
   S::clear(acc);
   int added = 0;         // steps in the accumulators
   bool written = false;  // whether the slice holds sums of steps before them
+  auto end_chain = [&] {
+    const long long slice = static_cast<long long>(blockIdx.z) * p.chunks + blockIdx.y;
+    S::add(acc, reinterpret_cast<float*>(smem), part + slice * p.K * p.K * p.C, c0, p.C, p.K, written);
+  };
 
   const int u1 = min(p.units, static_cast<int>(blockIdx.y + 1) * p.per_chunk);
   int u = blockIdx.y * p.per_chunk;
-  while (true) {  // one image's part of the range at a time, in even pieces where it is longer than a chain
+  while (u < u1) {  // one image's part of the range at a time
     const int b = u / p.unit_rows;
-    const int s0 = u - b * p.unit_rows, rest = min(p.unit_rows - s0, u1 - u), pieces = (rest + S::kMost - 1) / S::kMost;
-    const int steps = rest > S::kMost ? (rest + pieces - 1) / pieces : rest;
-    if (rest <= 0 || added + steps > S::kMost) {
-      const long long slice = static_cast<long long>(blockIdx.z) * p.chunks + blockIdx.y;
-      S::write(acc, reinterpret_cast<float*>(smem), part + slice * p.K * p.K * p.C, c0, p.C, p.K, written);
-      if (rest <= 0) break;
-      S::clear(acc);
-      added = 0;
-      written = true;
+    const int s0 = u - b * p.unit_rows;
+    int steps = min(p.unit_rows - s0, u1 - u);
+    if constexpr (LONG) {  // in even pieces where it is longer than a chain
+      if (steps > S::kMost) {
+        const int pieces = (steps + S::kMost - 1) / S::kMost;
+        steps = (steps + pieces - 1) / pieces;
+      }
+      if (added + steps > S::kMost) {
+        end_chain();
+        S::clear(acc);
+        added = 0;
+        written = true;
+      }
+      added += steps;
     }
     const int top = s0 * kStep + pad - (p.K - 1);  // first row of dy that the first row of x meets
     // of x and dy, this thread's next to fetch; of the exponent bytes, its next to load
@@ -456,8 +500,13 @@ __global__ void __launch_bounds__(kWgThreads, kWgCtas<MT, PACK>) wgrad8_kernel(c
       first -= first >= ring ? ring : 0;
       __syncthreads();
     }
-    added += steps;
     u += steps;
+  }
+  if constexpr (LONG) {
+    end_chain();
+  } else {
+    const long long slice = static_cast<long long>(blockIdx.z) * p.chunks + blockIdx.y;
+    S::write(acc, part + slice * p.K * p.K * p.C, c0 + (tid >> 5) * 4, p.C, p.K);
   }
 }
 
@@ -498,14 +547,15 @@ __global__ void __launch_bounds__(kReduceThreads) wgrad8_reduce_kernel(const flo
 
 // The kernel for K and a tile of columns, its rows a step and its shared memory.
 struct Wgrad8Kernel {
-  const void* fn;
+  const void *fn, *long_fn;
   int step, most, ctas, smem;  // rows a step; steps of a chain; CTAs an SM, by registers
 };
 template <int MT, int NT, int ROWS, bool PACK, int TW, int SETS>
 static Wgrad8Kernel wgrad8_kernel_of(int K) {
   using S = Wgrad8<MT, NT, ROWS, PACK, TW, SETS>;
-  return {reinterpret_cast<const void*>(&wgrad8_kernel<MT, NT, ROWS, PACK, TW, SETS>), S::kStep, S::kMost, kWgCtas<MT, PACK>,
-          S::smem(K)};
+  return {reinterpret_cast<const void*>(&wgrad8_kernel<MT, NT, ROWS, PACK, TW, SETS, false>),
+          reinterpret_cast<const void*>(&wgrad8_kernel<MT, NT, ROWS, PACK, TW, SETS, true>),
+          S::kStep, S::kMost, kWgCtas<MT, PACK>, S::smem(K)};
 }
 static int wgrad8_room(const Wgrad8Kernel& k) { return 228 * 1024 / (k.smem + 1024); }  // CTAs an SM, by shared memory
 // Sets: as many as a step's items of x have threads for.  A step of one set leaves most threads of a narrow tile without
@@ -618,9 +668,10 @@ extern "C" int dwb_conv2d_nhwc_bwd_weight_act8(const void* codes, const void* sc
   float* part = static_cast<float*>(workspace);
   void* a1[] = {&codes, &scales, &dy, &part, &p};
   const Wgrad8Kernel k = wgrad8_kernel_for(K, p.tw);
-  cudaError_t e = allow_large_cta(k.fn);
+  const void* const fn = p.per_chunk > k.most ? k.long_fn : k.fn;
+  cudaError_t e = allow_large_cta(fn);
   if (e == cudaSuccess)
-    e = launch_kernel(k.fn, dim3(static_cast<unsigned>((C + kWgChannels - 1) / kWgChannels), p.chunks, p.col_tiles),
+    e = launch_kernel(fn, dim3(static_cast<unsigned>((C + kWgChannels - 1) / kWgChannels), p.chunks, p.col_tiles),
                       dim3(kWgThreads), a1, k.smem, st);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();

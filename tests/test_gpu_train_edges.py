@@ -150,6 +150,18 @@ def test_weight_gradient_of_one_long_range(eng, K, W, H):
     check_wgrad(eng, B, H, W, C, K, 100 * K + W)
 
 
+@pytest.mark.parametrize("W,H", [(13, 43), (16, 42), (30, 23), (45, 19), (61, 15), (75, 15)])
+@pytest.mark.parametrize("K", [1, 3, 5, 7, 9, 11, 13, 15, 17, 23, 25, 31])
+def test_weight_gradient_of_one_chain(eng, K, W, H):
+    """The same with two images that make one chain at most: the kernel for ranges that end with their chain."""
+    B, ctas = 2, 3 if K <= 7 else 2 if K <= 15 else 1
+    C = 32 * 148 * ctas
+    rows = 1 if K > 15 else 2  # of x that a set takes
+    steps = 128 // (min(-(-W // 16), 4) if W <= 64 else 3) * rows
+    assert wgrad_chunks(B, H, W, C, K) <= 2 and B * H <= steps
+    check_wgrad(eng, B, H, W, C, K, 100 * K + W)
+
+
 @pytest.mark.parametrize("B,H,W,C,K", [(2, 200, 64, 4736, 31), (40, 3, 15, 4736, 27), (1, 300, 33, 4736, 19), (64, 14, 14, 512, 27),
                                        (70, 7, 7, 9464, 13), (9, 56, 56, 2056, 7), (2, 180, 20, 9472, 9), (17, 1, 64, 14208, 5)])
 def test_weight_gradient_of_long_ranges(eng, B, H, W, C, K):
@@ -305,3 +317,17 @@ def test_a_bad_value_takes_its_whole_group(eng, act, bad, H, C, G):
     assert torch.equal(torch.isnan(dx).all(dim=3).all(dim=2), inside) and torch.equal(torch.isnan(dx).amax(dim=(2, 3)), inside)
     assert torch.equal(torch.isnan(dw), inside[1])
     assert (scales == 255).sum() == 1 and scales[1, H // 2, 1, c // 32] == 255
+
+
+def test_compiled_forward_passes(eng):
+    """Under torch.compile the functions trace without a break, with and without gradients asked for."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(2, 9, 11, 64, device="cuda", generator=g).half().permute(0, 3, 1, 2)
+    w = (torch.randn(5, 5, 64, device="cuda", generator=g) / 5).half()
+    v = torch.rand(64, device="cuda", generator=g)
+
+    def run(x, w, v):
+        return eng.group_norm_act(eng.conv2d_nhwc_act8(x, w), 8, v, v, act="gelu", checkpoint=True)
+
+    with torch.no_grad():
+        assert torch.equal(torch.compile(run, fullgraph=True)(x, w, v), run(x, w, v))
