@@ -451,7 +451,8 @@ static bool gn_resident_fill(const GnShape& s, GnPass pass, int slab, int cluste
   p->cluster = cluster;
   p->cluster_log = 0;
   while ((1 << p->cluster_log) < cluster) ++p->cluster_log;
-  p->lane_mul = 65536u / p->lanes + 1;  // exact for thread < 1024: the error of thread / lanes stays below 1 / 64
+  // exact for thread < 256, lanes <= 256: the product is too large by thread / 65536 < 1 / lanes at most
+  p->lane_mul = 65536u / p->lanes + 1;
   p->rows_per_cta = static_cast<int>(rows);
   p->rl = most / p->lanes;
   if (p->rl > p->rows_per_cta) p->rl = p->rows_per_cta;

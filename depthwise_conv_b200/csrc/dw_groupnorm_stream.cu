@@ -681,8 +681,9 @@ bool gn_stream_plan(const GnShape& s, int bytes_per_value, GnStream* q) {
   q->samples = static_cast<int>((s.B + groups - 1) / groups);
   // CTAs of a pass: about as many as run at once (3 an SM), long ones: more, shorter ones pay their ramp more often
   // (32x32x1536, B = 16, gradient: 67 us with 2 and 3 an SM, 70 with 3 and 5; forward 39 us with 3, 45 with 9).  Second
-  // pass: at most 4 an SM and as near as can be, since a few CTAs more than run at once are a turn of their own (56x56x128,
-  // B = 64, gradient from a checkpoint: 83.7 us with 448 CTAs, 77.1 with 576; 32x32x1536, B = 8: 39.5 with 480, 37.2 with 576)
+  // pass: at most 4 for every SM, of which 3 run at once, and as near to that as can be (56x56x128, B = 64, gradient from a
+  // checkpoint: 83.7 us with 448 CTAs, 77.1 with 576; 32x32x1536, B = 8: 39.5 with 480, 37.2 with 576).  Neither pass
+  // fills a whole number of turns: 512 and 576 CTAs are 1.15 and 1.3 of them at 32x32x1536, B = 16
   const long long a_chunk = static_cast<long long>(q->tiles) * q->samples, want = (bytes_per_value > 2 ? 2 : 3) * kSmCount;
   stream_rows(s.P, q->rl, (want + a_chunk - 1) / a_chunk, &q->rows, &q->chunks);
   stream_rows(s.P, q->apply_rl, 4 * kSmCount / (static_cast<long long>(q->apply_tiles) * q->samples), &q->apply_rows,

@@ -39,15 +39,17 @@
 // however long the batch.
 //
 // Measured (both kernels; the framework's 16-bit weight gradient on the CUDA
-// cores in brackets): 16x32x32x768 k7 34.4 us (64.3), 16x32x32x1536 k9 82.6 (182),
-// 8x56x56x1024 k13 112 (310), 8x56x56x128 k31 44 (171), 2x14x14x512 k27 12.1,
+// cores in brackets): 16x32x32x768 k7 36.7 us (64.3), 16x32x32x1536 k9 80.6 (182),
+// 8x56x56x1024 k13 112 (310), 8x56x56x128 k31 43 (171), 2x14x14x512 k27 11.7,
 // 56x56x1024 k31 242 with 8 images, 1701 with 64 (286 and 1908 when a chain's end was
 // a range's: 112 slices, 441 MB of workspace for the 64 images, where 9 are 35 MB).
-// What bounds it is the issue of the instructions around the products, most of
-// all the conversion and transposition of x and dy: at 16x32x32x768 k7 the
-// 38 MB read need 5.8 us and the products' FMAs on the CUDA cores would need
-// 14.8.  Items of 4 channels, which spread a row over twice the threads, were
-// slower; so was one step of read-ahead.
+// What bounds it for small K is latency at two CTAs of 8 warps an SM (one at 64
+// columns from K = 9 on): at 16x32x32x768 k7 the issue slots are used 43% of the
+// time and the tensor pipe 9%, and warps wait for a step's barrier, the
+// shared-memory queue and the copies that a step converts and transposes; the 38 MB
+// read need 5.8 us and the products' FMAs on the CUDA cores would need 14.8.  At
+// K = 31 the tensor pipe is active 54% of the time.  Items of 4 channels, which
+// spread a row over twice the threads, were slower; so was one step of read-ahead.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -560,8 +562,10 @@ static Wgrad8Kernel wgrad8_kernel_of(int K) {
 static int wgrad8_room(const Wgrad8Kernel& k) { return 228 * 1024 / (k.smem + 1024); }  // CTAs an SM, by shared memory
 // Sets: as many as a step's items of x have threads for.  A step of one set leaves most threads of a narrow tile without
 // an item and has a barrier for few products (19x14x8x1424 k9: 40.2 us with one set, 32.4 with two; 8x14x14x512 k27: 21.0
-// with one, 17.7 with four; 8x32x32x1536 k27: 165 with one, 146 with two).  But not where the longer ring then leaves
-// room for fewer CTAs an SM (16x32x32x1536 k11: 86.0 us with one set and two CTAs, 145 with two sets and one).
+// with one, 17.7 with four; 8x32x32x1536 k27: 165 with one, 146 with two).  From K = 9 on not where the longer ring then
+// leaves room for one CTA an SM (16x32x32x1536 k11: 86.0 us with one set and two CTAs, 145 with two sets and one).  Up to
+// K = 7 two sets are better with two CTAs an SM than one with three (inputs in L2: 16x32x32x768 k7 34.2 and 37.8 us,
+// 8x16x16x1536 k3 12.9 and 15.2, 64x56x28x256 k7 65.4 and 72.7).
 template <int TW>
 static Wgrad8Kernel wgrad8_kernel_for(int K) {
   constexpr int kPair = TW <= 32 ? 2 : 1, kOne = TW == 16 ? 4 : TW == 32 ? 2 : 1;

@@ -321,7 +321,8 @@ DWB_API int dwb_act8_decode_nhwc(const void* codes, const void* scales, void* x,
  * dwb_conv2d_nhwc_bwd_weight_act8_workspace reports; no two calls that may overlap
  * share one.  It holds a [K][K][C] of fp32 for every CTA that adds up one 32 channels
  * of it: as many as run at once or a few turns of them (at 56x56x1024, K = 31, 35 MB
- * from 64 images on), whatever the batch.  K odd, 1..31, C % 8 == 0. */
+ * for 16 to 1024 images; for more, less than 1% of codes and dy).  K odd, 1..31,
+ * C % 8 == 0. */
 DWB_API int dwb_conv2d_nhwc_bwd_weight_act8_workspace(int64_t B, int64_t H, int64_t W, int64_t C, int K,
                                                       int64_t* bytes);
 DWB_API int dwb_conv2d_nhwc_bwd_weight_act8(const void* codes, const void* scales, const void* dy, float* dw,
