@@ -623,6 +623,7 @@ static int wgrad8_plan(int64_t B, int64_t H, int64_t W, int64_t C, int K, Wgrad8
       best = time;
       p->per_chunk = static_cast<int>(per);
     }
+    if (per == 1) break;  // there are no more ranges than that
   }
   p->chunks = (p->units + p->per_chunk - 1) / p->per_chunk;
   if (p->chunks < 1) p->chunks = 1;

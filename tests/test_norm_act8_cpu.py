@@ -297,7 +297,10 @@ def test_no_checkpoint_where_no_gradient_is_taken(monkeypatch):
     for args in ((grad(x), v, v), (x, grad(v), None), (x, None, grad(v))):
         gn(*args)
         assert made == ["norm"]
-    # the op itself does what its argument says
+    # the op itself does what its argument says, which is to make one unless told otherwise
+    wg = grad(w)
+    call(torch.ops.depthwise.conv2d_nhwc_act8, x, wg)[0].backward(torch.ones_like(x))
+    assert made == ["conv"] and (wg.grad == 1).all()
     assert torch.ops.depthwise.conv2d_nhwc_act8(x, w)[1].shape == x.shape
     y, codes, scales = torch.ops.depthwise.conv2d_nhwc_act8(x, grad(w), None, False)
     assert codes.numel() == scales.numel() == 0
