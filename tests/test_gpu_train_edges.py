@@ -331,3 +331,38 @@ def test_compiled_forward_passes(eng):
 
     with torch.no_grad():
         assert torch.equal(torch.compile(run, fullgraph=True)(x, w, v), run(x, w, v))
+
+
+@pytest.mark.parametrize("shape,G,K", [((11, 100, 100, 1752), 73, 3), ((3, 61, 45, 4736), 32, 25), ((5, 40, 30, 9472), 1, 11)])
+def test_long_calls_captured_and_replayed_beside_others(eng, shape, G, K):
+    """Calls of many launches, and a weight gradient whose ranges have several chains, captured once and replayed on data
+    that the capture has not seen, while the same calls run eagerly on another stream: the same bits as by themselves."""
+    B, H, W, C = shape
+    assert wgrad_chunks(B, H, W, C, K) * 4 <= B * -(-H // 4)
+    g = torch.Generator(device="cuda").manual_seed(C)
+    data = [[torch.randn(B, H, W, C, device="cuda", generator=g).half().permute(0, 3, 1, 2) for _ in range(2)] for _ in range(3)]
+    w, b = 1 + 0.3 * torch.randn(C, device="cuda", generator=g), 0.3 * torch.randn(C, device="cuda", generator=g)
+
+    def run(x, dy):
+        y, mean, rstd, codes, scales = eng.norm_ops.group_norm_act_forward(x, G, w, b, 1e-5, "gelu", checkpoint=True)
+        first = eng.norm_ops.group_norm_act_backward(dy, x, mean, rstd, G, w, b, "gelu")
+        second = eng.norm_ops.group_norm_act_backward(dy, (codes, scales), mean, rstd, G, w, b, "gelu")
+        return [y, mean, rstd, codes, *first, *second, eng.act8_ops.conv2d_nhwc_backward_weight_act8(codes, scales, dy, K)]
+
+    want = [run(*d) for d in data]
+    x, dy = (t.clone(memory_format=torch.preserve_format) for t in data[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = run(x, dy)
+    side = torch.cuda.Stream()
+    for i in (1, 0, 1):
+        x.copy_(data[i][0])
+        dy.copy_(data[i][1])
+        side.wait_stream(torch.cuda.current_stream())
+        graph.replay()
+        with torch.cuda.stream(side):
+            got = run(*data[2])
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(held, want[i])), i
+        assert all(torch.equal(p, q) for p, q in zip(got, want[2])), i
+    assert eng.device_error() == 0
